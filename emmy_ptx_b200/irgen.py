@@ -15,6 +15,10 @@ schedules Emmy's lowering uses for each kernel family (README.md:17-18, 63-64, 1
 * ``attention_ir`` — one warp per query row, QK dot via WarpShuffle, causal Select, online
                      softmax with Accum ``base`` for the running max / sum, PV Accum (config 5).
 
+Beside them stand the operators of a paged key/value cache, ``cache_write_ir``, ``cache_read_ir`` and
+``paged_attention_ir``: new tokens' keys and values written to the pages (in bytes if wanted), read back, and
+attended to by a chunk of new tokens.
+
 Every builder returns a :class:`Problem`: the IR graph dict, its ``meta.json`` record
 (localrun.py:148-184 format) and the input specification used to make seeded inputs.
 """
@@ -611,6 +615,264 @@ def attention_ir(batch: int = 8, heads: int = 32, seq: int = 4096, dim: int = 12
                    grid=grid, block=threads, rtol=1e-4, atol=1e-6,
                    params={"batch": batch, "heads": heads, "seq": seq, "dim": dim, "causal": causal,
                            "scale": scale, **({"mask": True} if mask else {})})
+
+
+# ---- the paged key/value cache ---------------------------------------------------------------
+#
+# A pool of pages holds the keys and values of many sequences: KC and VC [pages, kv_heads, page, dim], in the
+# activations' 16-bit type or (``quant``) as bytes with one f32 scale per token and head, KS and VS
+# [pages, kv_heads, page].  Sequence b holds lens[b] tokens, the last fresh[b] of them new; token p sits in
+# row p % page of page table[b, p // page].  New token c of a chunk has position lens[b] - fresh[b] + c.
+# Rows c >= fresh[b] are padding, which none of the kernels writes.  A table entry outside [0, pages) holds
+# no tokens, and neither does a position outside [0, max_pages * page): nothing is written there, read
+# from there or attended to.
+
+CACHE_DTYPES = ("bf16", "f16")
+
+
+def _cache_dims(what, dtype, quant, **dims):
+    if dtype not in CACHE_DTYPES:
+        raise ValueError(f"{what} dtype must be one of {', '.join(CACHE_DTYPES)}, not {dtype!r}")
+    if not isinstance(quant, bool):
+        raise ValueError(f"{what} quant must be True or False, not {quant!r}")
+    for k, v in dims.items():
+        if isinstance(v, bool) or not isinstance(v, int) or v < 1:
+            raise ValueError(f"{what} needs {k} >= 1, not {v!r}")
+    if dims["dim"] % 32 or dims["dim"] // 32 not in (1, 2, 4, 8):
+        raise ValueError(f"{what} needs dim in {{32, 64, 128, 256}}")
+    if dims["max_pages"] * dims["page"] >= 1 << 30 or dims["pages"] >= 1 << 30:
+        raise ValueError(f"{what} takes fewer than 2^30 positions a sequence and fewer than 2^30 pages")
+
+
+def _cache_specs(pages, kv_heads, page, dim, dtype, quant, output):
+    cdt = "u8" if quant else dtype
+    dist = ("randint", 1, 256) if quant else ("normal", 1.0)
+    specs = [TensorSpec(n, (pages, kv_heads, page, dim), cdt, dist, output=output) for n in ("KC", "VC")]
+    if quant:
+        specs += [TensorSpec(n, (pages, kv_heads, page), "f32", ("uniform", 0.002, 0.02), output=output)
+                  for n in ("KS", "VS")]
+    return specs
+
+
+def _cache_index_specs(batch, pages, page, max_pages, chunk):
+    return [TensorSpec("table", (batch, max_pages), "i32", ("randint", 0, pages)),
+            TensorSpec("lens", (batch,), "i32", ("randint", chunk, max(max_pages * page, chunk) + 1)),
+            TensorSpec("fresh", (batch,), "i32", ("randint", 0, chunk + 1))]
+
+
+def _in_page(pos, pages, page, max_pages, body):
+    """``body`` with ``pg`` and ``row`` bound to the page and row of position ``pos``, when they exist."""
+    return Cond(Bin("&&", Bin(">=", V(pos), 0), Bin("<", V(pos), max_pages * page)), [
+        Let("slot", Bin("/", V(pos), page)),
+        Let("row", Bin("%", V(pos), page)),
+        Load(["pg"], "table", [V("b"), V("slot")], "i32"),
+        Cond(Bin("&&", Bin(">=", V("pg"), 0), Bin("<", V("pg"), pages)), body),
+    ])
+
+
+def _cells(what, *ext):
+    n = 1
+    for e in ext:
+        n *= e
+    if n >= 1 << 31:
+        raise ValueError(f"{what}: {n} threads are more than one launch of 32-bit thread indices covers")
+    return n
+
+
+def cache_write_ir(batch: int, chunk: int, kv_heads: int, dim: int, pages: int, page: int, max_pages: int,
+                   dtype: str = "bf16", quant: bool = False) -> Problem:
+    """The new tokens' keys and values K, V [batch, chunk, kv_heads, dim] into the pages of their sequences.
+
+    One warp per token and head.  With ``quant`` a row x is stored as bytes 128 + round(x / s) under its
+    scale s = max|x| / 127 (both quotients rounded to f32, the rounding to nearest even): an error of at
+    most half a step s / 2.  A row of zeros has scale 0 and bytes 128; a row that holds an infinity or a NaN
+    gets the scale NaN, so all of it reads back as NaN.  Rows of the cache that belong to no new token are
+    left as they were.  Two new tokens must not share a cache row (one sequence's pages are its own)."""
+    _cache_dims("cache_write_ir", dtype, quant, batch=batch, chunk=chunk, kv_heads=kv_heads, dim=dim, pages=pages,
+                page=page, max_pages=max_pages)
+    cells = _cells("cache_write_ir", batch, chunk, kv_heads, 32)
+    per = dim // 32
+    P = range(per)
+
+    def store(n, cache, scales):
+        xs = [f"{n}{i}" for i in P]
+        out = [Load(xs, n.upper(), [V("b"), V("c"), V("h"), V("d0")], dtype)]
+        at = [V("pg"), V("h"), V("row"), V("d0")]
+        if not quant:
+            return out + [Write(cache, xs, at, dtype)]
+        ab = [f"{n}a{i}" for i in P]
+        zs = [f"{n}z{i}" for i in P]
+        out += [Assign(ab[i], "absolute", [xs[i]]) for i in P]
+        out += [Assign(zs[i], "multiply", [xs[i], Lit(0.0)]) for i in P]        # NaN for an infinity or a NaN
+        if per > 1:
+            out += _tree("maximum", ab, f"{n}mx", f"{n}m") + _tree("add", zs, f"{n}zt", f"{n}z")
+        else:
+            out += [Assign(f"{n}m", "copy", ab), Assign(f"{n}z", "copy", zs)]
+        out += [WarpShuffle([f"{n}m"], [f"{n}m_o"], _combine(f"{n}m", f"{n}m_o", "maximum", "f32")),
+                WarpShuffle([f"{n}z"], [f"{n}z_o"], _combine(f"{n}z", f"{n}z_o", "add", "f32")),
+                Assign(f"{n}u", "divide", [f"{n}m", Lit(127.0)]),
+                Assign(f"{n}s", "add", [f"{n}u", f"{n}z"]),
+                Assign(f"{n}ok", "greater", [f"{n}s", Lit(0.0)], "bool")]
+        for i in P:
+            out += [Assign(f"{n}r{i}", "divide", [xs[i], f"{n}s"]),
+                    Assign(f"{n}q{i}", "rint", [f"{n}r{i}"]),
+                    Assign(f"{n}l{i}", "maximum", [f"{n}q{i}", Lit(-127.0)]),
+                    Assign(f"{n}h{i}", "minimum", [f"{n}l{i}", Lit(127.0)]),
+                    Select(f"{n}c{i}", [(V(f"{n}ok"), f"{n}h{i}"), (None, Lit(0.0))]),
+                    Assign(f"{n}b{i}", "add", [f"{n}c{i}", Lit(128.0)])]
+        return out + [Write(cache, [f"{n}b{i}" for i in P], at, "u8"),
+                      Cond(Bin("==", V("ln"), 0), [Write(scales, [f"{n}s"], [V("pg"), V("h"), V("row")], "f32")])]
+
+    body = [Tile([Axis("b", batch), Axis("c", chunk), Axis("h", kv_heads), Axis("ln", 32)], [
+        Load(["len"], "lens", [V("b")], "i32"),
+        Load(["nn"], "fresh", [V("b")], "i32"),
+        Let("d0", Bin("*", V("ln"), per)),
+        Cond(Bin("<", V("c"), V("nn")), [
+            Let("pos", Bin("+", Bin("-", V("len"), V("nn")), V("c"))),
+            _in_page("pos", pages, page, max_pages, [*store("k", "KC", "KS"), *store("v", "VC", "VS")]),
+        ]),
+    ])]
+    args = [*[TensorSpec(n, (batch, chunk, kv_heads, dim), dtype, ("normal", 1.0)) for n in ("K", "V")],
+            *_cache_index_specs(batch, pages, page, max_pages, chunk),
+            *_cache_specs(pages, kv_heads, page, dim, dtype, quant, True)]
+    params = {"batch": batch, "chunk": chunk, "kv_heads": kv_heads, "dim": dim, "pages": pages, "page": page,
+              "max_pages": max_pages, "dtype": dtype, "quant": quant}
+    return Problem(f"cache_write_{batch}x{chunk}x{kv_heads}x{dim}", "cache", "cache_write",
+                   _graph("cache_write", args, body), args, grid=-(-cells // 128), block=128, params=params)
+
+
+def cache_read_ir(batch: int, length: int, kv_heads: int, dim: int, pages: int, page: int, max_pages: int,
+                  dtype: str = "bf16", quant: bool = False) -> Problem:
+    """KR, VR [batch, length, kv_heads, dim]: the first min(lens[b], length) tokens of every sequence,
+    gathered from their pages in order; with ``quant`` (byte - 128) * scale, rounded once to ``dtype``.
+    Rows past a sequence's end, and rows whose page the table does not name, are left as they were."""
+    _cache_dims("cache_read_ir", dtype, quant, batch=batch, length=length, kv_heads=kv_heads, dim=dim, pages=pages,
+                page=page, max_pages=max_pages)
+    cells = _cells("cache_read_ir", batch, length, kv_heads, 32)
+    per = dim // 32
+    P = range(per)
+
+    def fetch(n, cache, scales, out):
+        xs = [f"{n}{i}" for i in P]
+        st = [Load(xs, cache, [V("pg"), V("h"), V("row"), V("d0")], "u8" if quant else dtype)]
+        if quant:
+            st += [Load([f"{n}s"], scales, [V("pg"), V("h"), V("row")], "f32"),
+                   *[Let(f"{n}f{i}", Bin("-", V(xs[i]), Lit(128.0)), "f32") for i in P],
+                   *[Assign(f"{n}y{i}", "multiply", [f"{n}f{i}", f"{n}s"]) for i in P]]
+            xs = [f"{n}y{i}" for i in P]
+        return st + [Write(out, xs, [V("b"), V("t"), V("h"), V("d0")], dtype)]
+
+    body = [Tile([Axis("b", batch), Axis("t", length), Axis("h", kv_heads), Axis("ln", 32)], [
+        Load(["len"], "lens", [V("b")], "i32"),
+        Let("d0", Bin("*", V("ln"), per)),
+        Cond(Bin("<", V("t"), V("len")), [
+            _in_page("t", pages, page, max_pages, [*fetch("k", "KC", "KS", "KR"), *fetch("v", "VC", "VS", "VR")]),
+        ]),
+    ])]
+    args = [*_cache_specs(pages, kv_heads, page, dim, dtype, quant, False),
+            *_cache_index_specs(batch, pages, page, max_pages, 1)[:2],
+            *[TensorSpec(n, (batch, length, kv_heads, dim), dtype, output=True) for n in ("KR", "VR")]]
+    params = {"batch": batch, "length": length, "kv_heads": kv_heads, "dim": dim, "pages": pages, "page": page,
+              "max_pages": max_pages, "dtype": dtype, "quant": quant}
+    return Problem(f"cache_read_{batch}x{length}x{kv_heads}x{dim}", "cache", "cache_read",
+                   _graph("cache_read", args, body), args, grid=-(-cells // 128), block=128, params=params)
+
+
+def paged_attention_ir(batch: int, chunk: int, heads: int, kv_heads: int, dim: int, pages: int, page: int,
+                       max_pages: int, dtype: str = "bf16", quant: bool = False, window: int | None = None,
+                       sinks: int = 0, scale: float | None = None) -> Problem:
+    """O = softmax(Q K^T * scale) V of a chunk of new tokens over the paged cache, causal, f32 math.
+
+    Q, O [batch, chunk, heads, dim]; query head h reads key head h // (heads / kv_heads).  The new tokens'
+    own keys and values are in the cache already (:func:`cache_write_ir` runs first).  A token at position p
+    sees the keys 0..p, or with ``window`` those of p - window + 1..p and the first ``sinks`` ones.  One warp per
+    query row and the online softmax of :func:`attention_ir` with its safe maximum; keys that are not
+    seen are skipped, so whatever their rows hold cannot reach the result.  A row that sees no key (or
+    only keys whose score is -inf) ends as 0."""
+    _cache_dims("paged_attention_ir", dtype, quant, batch=batch, chunk=chunk, heads=heads, kv_heads=kv_heads, dim=dim,
+                pages=pages, page=page, max_pages=max_pages)
+    if heads % kv_heads:
+        raise ValueError(f"paged_attention_ir needs heads % kv_heads == 0, not {heads} and {kv_heads}")
+    if window is not None and (isinstance(window, bool) or not isinstance(window, int) or not 1 <= window < 1 << 30):
+        raise ValueError(f"paged_attention_ir needs a window of 1..2^30-1 keys or None, not {window!r}")
+    if isinstance(sinks, bool) or not isinstance(sinks, int) or not 0 <= sinks < 1 << 30:
+        raise ValueError(f"paged_attention_ir needs 0 <= sinks < 2^30, not {sinks!r}")
+    if sinks and window is None:
+        raise ValueError("paged_attention_ir: sinks are the first tokens that stay visible behind a window")
+    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    if not (math.isfinite(scale) and scale > 0):
+        raise ValueError(f"paged_attention_ir needs a finite scale above 0, not {scale!r}")
+    cells = _cells("paged_attention_ir", batch, chunk, heads, 32)
+    per, group = dim // 32, heads // kv_heads
+    P = range(per)
+    qs, ks, vs, os_ = ([f"{n}{i}" for i in P] for n in "qkvo")
+    cdt = "u8" if quant else dtype
+    at = [V("pg"), V("kh"), V("row"), V("d0")]
+    if quant:
+        kload = [Load([f"kb{i}" for i in P], "KC", at, cdt), Load(["ksc"], "KS", at[:3], "f32"),
+                 *[Let(ks[i], Bin("-", V(f"kb{i}"), Lit(128.0)), "f32") for i in P]]
+        vload = [Load([f"vb{i}" for i in P], "VC", at, cdt), Load(["vsc"], "VS", at[:3], "f32"),
+                 *[Let(vs[i], Bin("-", V(f"vb{i}"), Lit(128.0)), "f32") for i in P],
+                 Assign("pw", "multiply", ["pe", "vsc"])]
+    else:
+        kload, vload = [Load(ks, "KC", at, cdt)], [Load(vs, "VC", at, cdt)]
+    if per == 1:
+        dot = [Assign("dp", "multiply", [qs[0], ks[0]])]
+    else:
+        dot = [Assign(f"pp{i}", "multiply", [qs[i], ks[i]]) for i in P] + _tree("add", [f"pp{i}" for i in P], "ds", "dp")
+    key = [
+        *kload, *dot,
+        WarpShuffle(["dp"], ["dp_o"], _combine("dp", "dp_o", "add", "f32")),
+        Assign("sr", "multiply", ["dp", Lit(scale)]),
+        *([Assign("sc", "multiply", ["sr", "ksc"])] if quant else [Assign("sc", "copy", ["sr"])]),
+        Assign("mn", "maximum", ["m", "sc"]),
+        Assign("none", "equal", ["mn", Lit(-math.inf)], "bool"),
+        Select("mu", [(V("none"), Lit(0.0)), (None, "mn")]),
+        Assign("dm", "subtract", ["m", "mu"]),
+        Assign("alpha", "exp", ["dm"]),
+        Assign("dd", "subtract", ["sc", "mu"]),
+        Assign("pe", "exp", ["dd"]),
+        Assign("ls", "multiply", ["l", "alpha"]),
+        Accum("l", "add", "pe", base="ls"),
+        *vload,
+        *[Assign(f"os{i}", "multiply", [os_[i], "alpha"]) for i in P],
+        *[Assign(f"pv{i}", "multiply", ["pw" if quant else "pe", vs[i]]) for i in P],
+        *[Accum(os_[i], "add", f"pv{i}", base=f"os{i}") for i in P],
+        Accum("m", "maximum", "sc"),
+    ]
+    seen = [_in_page("kv", pages, page, max_pages, key)]
+    if window is not None:
+        seen = [Cond(Bin("||", Bin(">", Bin("+", V("kv"), window), V("pos")), Bin("<", V("kv"), sinks)), seen)]
+    body = [Tile([Axis("b", batch), Axis("c", chunk), Axis("h", heads), Axis("ln", 32)], [
+        Load(["len"], "lens", [V("b")], "i32"),
+        Load(["nn"], "fresh", [V("b")], "i32"),
+        Let("d0", Bin("*", V("ln"), per)),
+        Cond(Bin("<", V("c"), V("nn")), [
+            Let("pos", Bin("+", Bin("-", V("len"), V("nn")), V("c"))),
+            Let("kh", Bin("/", V("h"), group)),
+            Load(qs, "Q", [V("b"), V("c"), V("h"), V("d0")], dtype),
+            Init("m", "f32", -math.inf),
+            Init("l", "f32", 0.0),
+            *[Init(o, "f32", 0.0) for o in os_],
+            StridedLoop("kv", max_pages * page, 0, 1, seen,
+                        end=Bin("minimum", Bin("+", V("pos"), 1), max_pages * page)),
+            Assign("empty", "equal", ["l", Lit(0.0)], "bool"),
+            Select("den", [(V("empty"), Lit(1.0)), (None, "l")]),
+            *[Assign(f"y{i}", "divide", [os_[i], "den"], dtype) for i in P],
+            Write("O", [f"y{i}" for i in P], [V("b"), V("c"), V("h"), V("d0")], dtype),
+        ]),
+    ])]
+    shape = (batch, chunk, heads, dim)
+    args = [TensorSpec("Q", shape, dtype, ("normal", 1.0)),
+            *_cache_specs(pages, kv_heads, page, dim, dtype, quant, False),
+            *_cache_index_specs(batch, pages, page, max_pages, chunk),
+            TensorSpec("O", shape, dtype, output=True)]
+    params = {"batch": batch, "chunk": chunk, "heads": heads, "kv_heads": kv_heads, "dim": dim, "pages": pages,
+              "page": page, "max_pages": max_pages, "dtype": dtype, "quant": quant, "window": window, "sinks": sinks,
+              "scale": scale, "attention": True}
+    return Problem(f"paged_attention_{batch}x{chunk}x{heads}x{dim}", "cache", "paged_attention",
+                   _graph("paged_attention", args, body), args, grid=-(-cells // 128), block=128, rtol=1e-4,
+                   params=params)
 
 
 #: The five BASELINE configurations at full size.

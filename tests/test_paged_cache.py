@@ -1,0 +1,162 @@
+"""The paged key/value cache operators on the CPU: the IR's meaning (oracle), the emitted CUDA-core kernels and the
+tensor-core form (emulators) against plain float64, with ragged batches, padding, stale rows of NaN, missing
+pages, empty sequences and windows; and what the builders refuse."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from emmy_ptx_b200 import irgen
+from emmy_ptx_b200.codegen.generic import Unsupported
+from emmy_ptx_b200.compiler import compile_graph
+from emmy_ptx_b200.data import from_numpy_storage, to_numpy_storage
+from emmy_ptx_b200.ir import Graph
+from oracle.interp import Interpreter
+from tests import pagedref as R
+from tests.ptxemu import Emulator, Memory
+
+
+def by_oracle(p, t):
+    """The IR's outputs from the interpreter, on outputs that start as ``t`` holds them."""
+    bufs = {a.name: to_numpy_storage(t[a.name]) for a in p.args}
+    Interpreter(Graph.from_dict(p.graph)).run(bufs, p.grid, p.block)
+    return {a.name: from_numpy_storage(bufs[a.name], a.dtype).reshape(a.shape) for a in p.outputs}
+
+
+def by_emulator(p, t, opts=None):
+    """The outputs of the emitted CUDA-core PTX, run instruction by instruction."""
+    mod = compile_graph(Graph.from_dict(p.graph), p.meta(), opts or {})
+    mem = Memory()
+    addr = {a.name: mem.alloc(to_numpy_storage(t[a.name])) for a in p.args}
+    for rec in mod.kernels:
+        emu = Emulator(mod.ptx, rec["entry"])
+        emu.run(rec["grid"][0], rec["block"][0], dict(zip(emu.params, [addr[n] for n in rec["params"]])), mem,
+                rec["dyn_smem"])
+    out = {}
+    for a in p.outputs:
+        host = to_numpy_storage(t[a.name])
+        out[a.name] = from_numpy_storage(mem.array(addr[a.name], host.dtype, (-1,)).copy(), a.dtype).reshape(a.shape)
+    return out
+
+
+def same(got, want, what):
+    """Equal bit for bit, any NaN equal to any other."""
+    if got.dtype.is_floating_point:
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+        got, want = torch.nan_to_num(got.float()), torch.nan_to_num(want.float())
+    assert torch.equal(got, want), f"{what}: {int((got != want).sum())} elements differ"
+
+
+def broken_table(t, pages):
+    """Entries that name no page: below zero, one past the pool, far past it."""
+    t["table"][0, -1] = -1
+    t["table"][-1, 0] = pages
+    if t["table"].shape[1] > 2:
+        t["table"][0, 1] = 2 ** 31 - 1
+
+
+WRITES = [
+    # batch, chunk, kv_heads, dim, page, max_pages, lens, fresh
+    (3, 4, 2, 64, 8, 3, [4, 9, 24], [4, 2, 0]),
+    (2, 1, 1, 128, 16, 2, [1, 32], [1, 1]),
+    (2, 5, 3, 32, 3, 4, [3, 14], [5, 5]),              # positions below 0 and past the last page: not written
+    (1, 3, 1, 256, 1, 5, [5], [2]),
+]
+
+
+@pytest.mark.parametrize("run", [by_oracle, by_emulator])
+@pytest.mark.parametrize("dtype,quant", [("bf16", False), ("f16", False), ("bf16", True), ("f16", True)])
+@pytest.mark.parametrize("case", WRITES, ids=lambda c: "x".join(map(str, c[:6])))
+def test_cache_write(case, dtype, quant, run):
+    B, C, hk, d, page, mp, lens, fresh = case
+    t, pages = R.make("write", B, hk, d, page, mp, lens, fresh, chunk=C, dtype=dtype, quant=quant, seed=B + d)
+    broken_table(t, pages)
+    t["K"][0, 0, 0] = 0.0                                # a row of zeros
+    t["V"][0, 0, 0, 3] = math.inf                        # a row with an infinity, one with a NaN
+    t["V"][-1, -1, -1, 5] = math.nan
+    t["K"][-1, 0, 0] = torch.arange(d).to(t["K"].dtype) / 2      # exact halves: 127/2, rounding to even
+    p = irgen.cache_write_ir(B, C, hk, d, pages, page, mp, dtype, quant)
+    got = run(p, t)
+    want = R.write_ref(t, page, quant)
+    for n in want:
+        same(got[n], want[n], f"{n} {run.__name__}")
+
+
+READS = [(3, 20, 2, 64, 8, 3, [0, 9, 24]), (2, 33, 1, 128, 16, 2, [1, 40]), (1, 7, 3, 32, 3, 2, [-4])]
+
+
+@pytest.mark.parametrize("run", [by_oracle, by_emulator])
+@pytest.mark.parametrize("dtype,quant", [("bf16", False), ("bf16", True), ("f16", True)])
+@pytest.mark.parametrize("case", READS, ids=lambda c: "x".join(map(str, c[:6])))
+def test_cache_read(case, dtype, quant, run):
+    B, L, hk, d, page, mp, lens = case
+    t, pages = R.make("read", B, hk, d, page, mp, lens, [0] * B, length=L, dtype=dtype, quant=quant, seed=L)
+    broken_table(t, pages)
+    p = irgen.cache_read_ir(B, L, hk, d, pages, page, mp, dtype, quant)
+    got = run(p, t)
+    want = R.read_ref(t, page, dtype)
+    for n in want:
+        same(got[n], want[n], f"{n} {run.__name__}")
+
+
+ATTENDS = [
+    # batch, chunk, heads, kv_heads, dim, page, max_pages, lens, fresh, window, sinks
+    (3, 3, 4, 2, 32, 8, 3, [3, 9, 20], [3, 2, 0], None, 0),
+    (2, 1, 3, 1, 64, 4, 4, [1, 16], [1, 1], None, 0),
+    (2, 4, 2, 2, 32, 3, 5, [2, 15], [4, 4], 4, 2),          # two rows at positions below 0: zero
+    (1, 2, 2, 1, 64, 8, 2, [19], [2], 1, 0),                 # past the last page; a window of one
+]
+
+
+@pytest.mark.parametrize("run", [by_oracle, by_emulator])
+@pytest.mark.parametrize("dtype,quant", [("bf16", False), ("f16", True)])
+@pytest.mark.parametrize("case", ATTENDS, ids=lambda c: "x".join(map(str, c[:7])))
+def test_paged_attention_nest(case, dtype, quant, run):
+    B, C, H, hk, d, page, mp, lens, fresh, window, sinks = case
+    t, pages = R.make("attend", B, hk, d, page, mp, lens, fresh, chunk=C, heads=H, dtype=dtype, quant=quant, seed=H)
+    if mp == 3:
+        broken_table(t, pages)
+    p = irgen.paged_attention_ir(B, C, H, hk, d, pages, page, mp, dtype, quant, window, sinks)
+    got = run(p, t) if run is by_oracle else run(p, t, {"patterns": False})
+    ref, bound, _ = R.attention_ref(t, page, window, sinks)
+    R.check(got["O"], ref, bound, run.__name__)
+
+
+def test_offsets_past_32_bits_are_refused_by_the_cuda_core_form():
+    # 2^31 elements and more: the statement-at-a-time emitter computes element offsets in 32 bits
+    p = irgen.cache_write_ir(1, 1, 8, 128, 1 << 17, 16, 4)
+    with pytest.raises(Unsupported, match="32-bit"):
+        compile_graph(Graph.from_dict(p.graph), p.meta(), {"patterns": False})
+    p = irgen.cache_write_ir(1, 1, 8, 128, (1 << 17) - 1, 16, 4)
+    compile_graph(Graph.from_dict(p.graph), p.meta(), {"patterns": False})
+
+
+GOOD = dict(batch=1, chunk=1, kv_heads=1, dim=64, pages=4, page=8, max_pages=2)
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(dim=48), "dim"), (dict(dim=96), "dim"), (dict(page=0), "page"), (dict(kv_heads=True), "kv_heads"),
+    (dict(pages=1 << 30), "pages"), (dict(page=1 << 15, max_pages=1 << 15), "positions"), (dict(batch=-1), "batch"),
+    (dict(chunk=1 << 27), "threads"), (dict(dtype="f32"), "dtype"), (dict(quant=1), "quant"), (dict(chunk=2.0), "chunk"),
+])
+def test_builders_refuse(change, word):
+    kw = {**GOOD, **change}
+    with pytest.raises(ValueError, match=word):
+        irgen.cache_write_ir(**kw)
+    with pytest.raises(ValueError, match=word):
+        irgen.paged_attention_ir(heads=1, **kw)
+    kw["length"] = kw.pop("chunk")
+    with pytest.raises(ValueError, match="length" if word == "chunk" else word):
+        irgen.cache_read_ir(**kw)
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(heads=3, kv_heads=2), "heads"), (dict(window=0), "window"), (dict(window=2.5), "window"), (dict(sinks=2), "sinks"),
+    (dict(window=4, sinks=-1), "sinks"), (dict(scale=math.inf), "scale"), (dict(scale=math.nan), "scale"),
+    (dict(scale=0.0), "scale"), (dict(scale=-0.5), "scale"),
+    (dict(window=1 << 30), "window"),
+])
+def test_paged_attention_refuses(change, word):
+    with pytest.raises(ValueError, match=word):
+        irgen.paged_attention_ir(**{**GOOD, "heads": 2, **change})
