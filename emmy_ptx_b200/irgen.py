@@ -684,8 +684,8 @@ def cache_write_ir(batch: int, chunk: int, kv_heads: int, dim: int, pages: int, 
     """The new tokens' keys and values K, V [batch, chunk, kv_heads, dim] into the pages of their sequences.
 
     One warp per token and head.  With ``quant`` a row x is stored as bytes 128 + round(x / s) under its
-    scale s = max|x| / 127 (both quotients rounded to f32, the rounding to nearest even): an error of at
-    most half a step s / 2.  A row of zeros has scale 0 and bytes 128; a row that holds an infinity or a NaN
+    scale s = max|x| * (1 / 127) (the constant, the product and the quotient in f32, the rounding to nearest
+    even): an error of at most half a step s / 2.  A row of zeros has scale 0 and bytes 128; a row that holds an infinity or a NaN
     gets the scale NaN, so all of it reads back as NaN.  Rows of the cache that belong to no new token are
     left as they were.  Two new tokens must not share a cache row (one sequence's pages are its own)."""
     _cache_dims("cache_write_ir", dtype, quant, batch=batch, chunk=chunk, kv_heads=kv_heads, dim=dim, pages=pages,
@@ -710,7 +710,7 @@ def cache_write_ir(batch: int, chunk: int, kv_heads: int, dim: int, pages: int, 
             out += [Assign(f"{n}m", "copy", ab), Assign(f"{n}z", "copy", zs)]
         out += [WarpShuffle([f"{n}m"], [f"{n}m_o"], _combine(f"{n}m", f"{n}m_o", "maximum", "f32")),
                 WarpShuffle([f"{n}z"], [f"{n}z_o"], _combine(f"{n}z", f"{n}z_o", "add", "f32")),
-                Assign(f"{n}u", "divide", [f"{n}m", Lit(127.0)]),
+                Assign(f"{n}u", "multiply", [f"{n}m", Lit(1.0 / 127.0)]),
                 Assign(f"{n}s", "add", [f"{n}u", f"{n}z"]),
                 Assign(f"{n}ok", "greater", [f"{n}s", Lit(0.0)], "bool")]
         for i in P:

@@ -410,6 +410,92 @@ def match_attention(graph, node):
     return Q, K, V, O, bt, hd, seq, dim, causal, scale, M
 
 
+def _literals(template, data, marks: dict, found: dict) -> None:
+    """The values in ``data`` at the places where ``template`` holds one of ``marks`` (value -> parameter
+    name).  Only reads values out; whether the two agree elsewhere is for the caller to check."""
+    if isinstance(template, bool) or isinstance(data, bool):
+        return
+    if isinstance(template, (int, float)):
+        if template in marks and isinstance(data, (int, float)):
+            found.setdefault(marks[template], data)
+        return
+    if isinstance(template, dict) and isinstance(data, dict):
+        for k in template:
+            if k in data:
+                _literals(template[k], data[k], marks, found)
+    elif isinstance(template, list) and isinstance(data, list):
+        for x, y in zip(template, data):
+            _literals(x, y, marks, found)
+
+
+# parameters of the paged attention that no buffer's shape tells: numbers that stand for them in a template
+_MARK_WINDOW, _MARK_SINKS, _MARK_SCALE = 715827881, 477218587, 0.6180339887498949
+
+
+def match_paged_attention(graph, node):
+    """The keyword arguments of :func:`.irgen.paged_attention_ir` when the kernel is its nest, else None.
+
+    Sizes and types come from the buffers (Q, KC, VC, [KS, VS,] table, lens, fresh -> O, in that order); the
+    scale, the window and the sinks are read where the builder's own nest has them, and then the whole
+    body must equal the nest built with what was found."""
+    vals = graph.values()
+    ins = [vals.get(n) for n in node.inputs]
+    if len(node.outputs) != 1 or len(ins) not in (6, 8) or any(v is None for v in ins):
+        return None
+    O, quant = node.outputs[0], len(ins) == 8
+    Q, KC, table = ins[0], ins[1], ins[5 if quant else 3]
+    if len(Q.shape) != 4 or tuple(O.shape) != tuple(Q.shape) or len(KC.shape) != 4 or len(table.shape) != 2:
+        return None
+    dt = dt_name(Q.dtype)
+    want = [dt, *(["u8"] * 2 + ["f32"] * 2 if quant else [dt] * 2), "i32", "i32", "i32"]
+    if [dt_name(v.dtype) for v in ins] != want or dt_name(O.dtype) != dt:
+        return None
+    (batch, chunk, heads, dim), (pages, kv_heads, page, kd) = Q.shape, KC.shape
+    shapes = [Q.shape, *[KC.shape] * 2, *([KC.shape[:3]] * 2 if quant else []), (batch, table.shape[1]), (batch,), (batch,)]
+    if kd != dim or [tuple(v.shape) for v in ins] != [tuple(x) for x in shapes]:
+        return None
+    kw = dict(batch=batch, chunk=chunk, heads=heads, kv_heads=kv_heads, dim=dim, pages=pages, page=page,
+              max_pages=table.shape[1], dtype=dt, quant=quant)
+    from .irgen import paged_attention_ir
+    names = ["Q", "KC", "VC", *(["KS", "VS"] if quant else []), "table", "lens", "fresh"]
+    rename = {**dict(zip(node.inputs, names)), O.name: "O"}
+    for window, sinks in ((None, 0), (_MARK_WINDOW, _MARK_SINKS)):
+        found: dict = {}
+        try:
+            tmpl = Graph.from_dict(paged_attention_ir(**kw, window=window, sinks=sinks, scale=_MARK_SCALE).graph)
+        except ValueError:
+            return None
+        _literals(_body_data(tmpl.kernels()[0]), _body_data(node),
+                  {_MARK_WINDOW: "window", _MARK_SINKS: "sinks", _MARK_SCALE: "scale"}, found)
+        if "scale" not in found or (window is not None and set(found) != {"window", "sinks", "scale"}):
+            continue
+        full = {**kw, "window": found.get("window"), "sinks": found.get("sinks", 0), "scale": found["scale"]}
+        if is_canonical(node, lambda: paged_attention_ir(**full), rename):
+            return full
+    return None
+
+
+def _lower_paged_attention(node, kw, prefix, options):
+    """The tensor-core entries of a paged attention: one, or two when its units are split."""
+    from .kernels import tc_paged_attention as tpa
+    if not tpa.supported(kw["dim"], kw["heads"], kw["kv_heads"], kw["page"]):
+        return None
+    geo = {k: kw[k] for k in ("batch", "chunk", "heads", "kv_heads", "page", "max_pages", "window", "sinks")}
+    splits, min_tiles = tpa.plan_splits(**geo, sms=int(options.get("sms", 148)))
+    splits = int(options.get("paged_splits", splits))
+    min_tiles = int(options.get("paged_min_tiles", min_tiles))
+    name = node.op.name
+    names = [*node.inputs, node.outputs[0].name]
+    scratch = (f"{prefix}{name}__part", f"{prefix}{name}__ml")
+    main = tpa.paged_attention_entry(name, **kw, names=names, scratch=scratch, splits=splits, min_tiles=min_tiles,
+                                     prefix=prefix)
+    if splits == 1:
+        return main
+    join = tpa.join_entry(f"{name}_join", **geo, dim=kw["dim"], dtype=kw["dtype"], names=names[-3:], scratch=scratch,
+                          splits=splits, min_tiles=min_tiles)
+    return [main, join]
+
+
 def _flat(body):
     out = []
     walk(body, out.append)
@@ -521,4 +607,7 @@ def try_lower(graph, node, kmeta, prefix, options):
         att1["after"] = [f"{name}_vconv1"]
         att0["carveout"] = att1["carveout"] = 100
         return [pre0, att0, pre1, att1]
+    kw = match_paged_attention(graph, node)
+    if kw is not None:
+        return _lower_paged_attention(node, kw, prefix, options)
     return None

@@ -29,7 +29,7 @@ def quantise(x):
     x = x.double()
     bad = ~torch.isfinite(x).all(-1)
     amax = torch.where(torch.isfinite(x), x, 0.0).abs().amax(-1)
-    s = (amax / 127).float()
+    s = amax.float() * torch.tensor(1.0 / 127.0, dtype=torch.float32)
     s = torch.where(bad, torch.full_like(s, math.nan), s)
     ok = s > 0
     r = (x / torch.where(ok, s, torch.ones_like(s)).double()[..., None]).float().double()

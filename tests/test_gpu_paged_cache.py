@@ -1,0 +1,172 @@
+"""The paged key/value cache operators on a B200 against plain float64 (:mod:`tests.pagedref`): every type, ragged
+batches, padding, stale rows of NaN, missing pages, windows, split units, and the calls a serving program
+makes: write then attend then read, captured and replayed, on another stream."""
+import pytest
+import torch
+
+from emmy_ptx_b200 import irgen
+from emmy_ptx_b200.compiler import compile_graph
+from emmy_ptx_b200.ir import Graph
+from emmy_ptx_b200.runtime import Executable
+from tests import pagedref as R
+from tests.test_paged_cache import ATTENDS, READS, TENSOR, WRITES, broken_table, same
+
+pytestmark = pytest.mark.gpu
+
+
+def build(p, opts=None):
+    return Executable(compile_graph(Graph.from_dict(p.graph), p.meta(), opts or {}), device=0)
+
+
+def on_gpu(t):
+    return {k: v.cuda() for k, v in t.items()}
+
+
+def go(p, t, opts=None):
+    ex = build(p, opts)
+    g = on_gpu(t)
+    ex(g)
+    torch.cuda.synchronize()
+    ex.check()
+    kinds = [r["kind"] for r in ex.records]
+    ex.close()
+    return {a.name: g[a.name].cpu() for a in p.outputs}, kinds
+
+
+@pytest.mark.parametrize("dtype,quant", [("bf16", False), ("f16", False), ("bf16", True), ("f16", True)])
+@pytest.mark.parametrize("case", TENSOR, ids=lambda c: "x".join(map(str, c[:7])))
+def test_paged_attention(case, dtype, quant):
+    B, C, H, hk, d, page, mp, lens, fresh, window, sinks, opts = case
+    t, pages = R.make("attend", B, hk, d, page, mp, lens, fresh, chunk=C, heads=H, dtype=dtype, quant=quant, seed=H + C)
+    p = irgen.paged_attention_ir(B, C, H, hk, d, pages, page, mp, dtype, quant, window, sinks)
+    got, kinds = go(p, t, opts)
+    assert kinds[0] == "tcgen05_paged_attention"
+    ref, bound, _ = R.attention_ref(t, page, window, sinks)
+    R.check(got["O"], ref, bound, "tensor cores")
+
+
+@pytest.mark.parametrize("dtype,quant", [("bf16", False), ("f16", True)])
+@pytest.mark.parametrize("case", ATTENDS, ids=lambda c: "x".join(map(str, c[:7])))
+def test_paged_attention_cuda_cores(case, dtype, quant):
+    B, C, H, hk, d, page, mp, lens, fresh, window, sinks = case
+    t, pages = R.make("attend", B, hk, d, page, mp, lens, fresh, chunk=C, heads=H, dtype=dtype, quant=quant, seed=H)
+    if mp == 3:
+        broken_table(t, pages)
+    p = irgen.paged_attention_ir(B, C, H, hk, d, pages, page, mp, dtype, quant, window, sinks)
+    got, _ = go(p, t, {"patterns": False})
+    ref, bound, _ = R.attention_ref(t, page, window, sinks)
+    R.check(got["O"], ref, bound, "CUDA cores")
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("B,C,H,hk,d,page,lens,window,sinks", [
+    (3, 1, 8, 2, 128, 16, [2111, 63, 1024], None, 0),
+    (2, 4, 12, 2, 64, 64, [1500, 700], None, 0),
+    (1, 200, 4, 1, 128, 32, [900], None, 0),
+    (1, 150, 6, 2, 64, 8, [1300], 333, 70),
+    (4, 1, 16, 1, 128, 128, [2000, 1, 129, 800], 500, 4),
+], ids=["decode", "draft", "chunk", "chunk-window", "decode-window"])
+def test_paged_attention_longer(B, C, H, hk, d, page, lens, window, sinks, quant):
+    mp = -(-max(lens) // page) + 1
+    fresh = [min(C, n) for n in lens]
+    t, pages = R.make("attend", B, hk, d, page, mp, lens, fresh, chunk=C, heads=H, quant=quant, seed=d + C, sizes=2.0)
+    p = irgen.paged_attention_ir(B, C, H, hk, d, pages, page, mp, "bf16", quant, window, sinks)
+    got, kinds = go(p, t)
+    assert kinds[0] == "tcgen05_paged_attention"
+    ref, bound, _ = R.attention_ref(t, page, window, sinks)
+    R.check(got["O"], ref, bound, "longer")
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("page", [8, 64])
+def test_paged_attention_missing_pages(page, quant):
+    mp = 320 // page
+    t, pages = R.make("attend", 2, 1, 64, page, mp, [320, 250], [3, 3], chunk=3, heads=2, quant=quant, seed=page)
+    t["table"][0, 1] = -1
+    t["table"][0, mp - 2] = pages
+    t["table"][1, 0] = 2 ** 31 - 1
+    p = irgen.paged_attention_ir(2, 3, 2, 1, 64, pages, page, mp, "bf16", quant)
+    ref, bound, _ = R.attention_ref(t, page)
+    for opts in ({}, {"paged_splits": 2, "paged_min_tiles": 2}):
+        got, _ = go(p, t, opts)
+        R.check(got["O"], ref, bound, "missing pages")
+    t["table"].fill_(-1)
+    got, _ = go(p, t)
+    assert not got["O"][:, :3].any()
+
+
+@pytest.mark.parametrize("dtype,quant", [("bf16", False), ("f16", False), ("bf16", True), ("f16", True)])
+@pytest.mark.parametrize("case", WRITES, ids=lambda c: "x".join(map(str, c[:6])))
+def test_cache_write(case, dtype, quant):
+    B, C, hk, d, page, mp, lens, fresh = case
+    t, pages = R.make("write", B, hk, d, page, mp, lens, fresh, chunk=C, dtype=dtype, quant=quant, seed=B + d)
+    broken_table(t, pages)
+    t["K"][0, 0, 0] = 0.0
+    t["V"][0, 0, 0, 3] = float("inf")
+    t["V"][-1, -1, -1, 5] = float("nan")
+    t["K"][-1, 0, 0] = torch.arange(d).to(t["K"].dtype) / 2
+    p = irgen.cache_write_ir(B, C, hk, d, pages, page, mp, dtype, quant)
+    got, _ = go(p, t)
+    want = R.write_ref(t, page, quant)
+    for n in want:
+        same(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("dtype,quant", [("bf16", False), ("bf16", True), ("f16", True)])
+@pytest.mark.parametrize("case", READS, ids=lambda c: "x".join(map(str, c[:6])))
+def test_cache_read(case, dtype, quant):
+    B, L, hk, d, page, mp, lens = case
+    t, pages = R.make("read", B, hk, d, page, mp, lens, [0] * B, length=L, dtype=dtype, quant=quant, seed=L)
+    broken_table(t, pages)
+    p = irgen.cache_read_ir(B, L, hk, d, pages, page, mp, dtype, quant)
+    got, _ = go(p, t)
+    want = R.read_ref(t, page, dtype)
+    for n in want:
+        same(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_a_serving_step_captured_and_replayed(quant):
+    """Write, attend and read back, as one decode step after another from one captured graph, on a stream of
+    its own; lengths and inputs change between replays, as they do in serving."""
+    B, H, hk, d, page, mp = 2, 4, 2, 64, 16, 6
+    t, pages = R.make("write", B, hk, d, page, mp, [30, 61], [1, 1], quant=quant, seed=3)
+    a, _ = R.make("attend", B, hk, d, page, mp, [30, 61], [1, 1], heads=H, quant=quant, seed=4)
+    r, _ = R.make("read", B, hk, d, page, mp, [30, 61], [1, 1], length=mp * page, quant=quant, seed=5)
+    t = {**r, **a, **t}
+    common = (hk, d, pages, page, mp, "bf16", quant)
+    steps = [build(irgen.cache_write_ir(B, 1, *common)), build(irgen.paged_attention_ir(B, 1, H, *common),
+             {"paged_splits": 2, "paged_min_tiles": 1}), build(irgen.cache_read_ir(B, mp * page, *common))]
+    g = on_gpu(t)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        for ex in steps:
+            ex(g)                                            # warm-up: modules loaded, descriptors made
+        with torch.cuda.graph(graph, stream=s):
+            for ex in steps:
+                ex(g)
+    s.synchronize()
+    host = {k: v.clone() for k, v in t.items()}
+    host.update({k: v.cpu() for k, v in g.items()})          # the state after the warm-up
+    gen = torch.Generator().manual_seed(9)
+    for step in range(3):
+        host["lens"] = host["lens"] + 1
+        for n in ("K", "V", "Q"):
+            host[n] = torch.randn(host[n].shape, generator=gen).to(host[n].dtype)
+        for n in ("lens", "K", "V", "Q"):
+            g[n].copy_(host[n])
+        torch.cuda.current_stream().synchronize()
+        with torch.cuda.stream(s):
+            graph.replay()
+        s.synchronize()
+        host.update(R.write_ref(host, page, quant))
+        ref, bound, _ = R.attention_ref(host, page)
+        R.check(g["O"], ref, bound, f"step {step}")
+        back = R.read_ref(host, page, "bf16")
+        host.update(back)
+        for n in ("KC", "VC", "KR", "VR"):
+            same(g[n].cpu(), host[n], f"{n} step {step}")
+    for ex in steps:
+        ex.check()

@@ -1,9 +1,9 @@
 """The paged key/value cache operators on the CPU: the IR's meaning (oracle), the emitted CUDA-core kernels and the
 tensor-core form (emulators) against plain float64, with ragged batches, padding, stale rows of NaN, missing
 pages, empty sequences and windows; and what the builders refuse."""
+import json
 import math
 
-import numpy as np
 import pytest
 import torch
 
@@ -13,6 +13,7 @@ from emmy_ptx_b200.compiler import compile_graph
 from emmy_ptx_b200.data import from_numpy_storage, to_numpy_storage
 from emmy_ptx_b200.ir import Graph
 from oracle.interp import Interpreter
+from tests import pagedemu as PE
 from tests import pagedref as R
 from tests.ptxemu import Emulator, Memory
 
@@ -160,3 +161,87 @@ def test_builders_refuse(change, word):
 def test_paged_attention_refuses(change, word):
     with pytest.raises(ValueError, match=word):
         irgen.paged_attention_ir(**{**GOOD, "heads": 2, **change})
+
+
+# ---- the tensor-core form --------------------------------------------------------------------
+
+TENSOR = [
+    # batch, chunk, heads, kv_heads, dim, page, max_pages, lens, fresh, window, sinks, options
+    (2, 1, 2, 1, 64, 16, 8, [1, 128], [1, 1], None, 0, {}),
+    (3, 1, 4, 2, 128, 32, 6, [190, 0, 64], [1, 0, 1], None, 0, {}),
+    (1, 1, 6, 2, 64, 64, 5, [300], [1], None, 0, {"paged_splits": 3, "paged_min_tiles": 1}),
+    (2, 5, 3, 1, 64, 8, 20, [77, 160], [5, 3], None, 0, {"paged_splits": 2, "paged_min_tiles": 1}),
+    (1, 70, 5, 1, 64, 128, 2, [150], [70], None, 0, {}),                     # 25 tokens a tile, 125 rows
+    (1, 130, 1, 1, 128, 64, 3, [140], [130], None, 0, {}),                   # a tile of 128 tokens and one of 2
+    (2, 1, 2, 2, 64, 16, 20, [320, 40], [1, 1], 70, 3, {}),                  # sink tile, then the window's
+    (1, 40, 2, 1, 64, 32, 12, [380], [40], 100, 5, {"paged_splits": 2, "paged_min_tiles": 1}),
+    (1, 9, 2, 1, 64, 64, 4, [256], [9], 1, 0, {}),
+    (1, 9, 2, 1, 64, 64, 4, [200], [9], 3, 150, {}),                         # more sinks than a tile
+    (2, 6, 2, 1, 64, 16, 2, [4, 40], [6, 6], None, 0, {}),                   # positions below 0, past the table
+]
+
+
+@pytest.mark.parametrize("dtype,quant", [("bf16", False), ("f16", False), ("bf16", True), ("f16", True)])
+@pytest.mark.parametrize("case", TENSOR, ids=lambda c: "x".join(map(str, c[:7])))
+def test_paged_attention_tensor_cores_emulated(case, dtype, quant):
+    B, C, H, hk, d, page, mp, lens, fresh, window, sinks, opts = case
+    t, pages = R.make("attend", B, hk, d, page, mp, lens, fresh, chunk=C, heads=H, dtype=dtype, quant=quant, seed=H + C)
+    p = irgen.paged_attention_ir(B, C, H, hk, d, pages, page, mp, dtype, quant, window, sinks)
+    got, code, mod = PE.run(p, t, opts)
+    assert code == 0
+    kinds = [k["kind"] for k in mod.kernels]
+    assert kinds == ["tcgen05_paged_attention"] + ["paged_attention_join"] * (opts.get("paged_splits", 1) > 1)
+    ref, bound, _ = R.attention_ref(t, page, window, sinks)
+    R.check(got["O"], ref, bound, "tensor cores")
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("page", [8, 64])
+def test_paged_attention_late_completions_and_missing_pages(page, quant):
+    # asynchronous work completes as late as the barriers allow; table entries name no page
+    mp = 320 // page
+    t, pages = R.make("attend", 2, 1, 64, page, mp, [320, 250], [3, 3], chunk=3, heads=2, quant=quant, seed=page)
+    t["table"][0, 1] = -1
+    t["table"][0, mp - 2] = pages
+    t["table"][1, 0] = 2 ** 31 - 1
+    p = irgen.paged_attention_ir(2, 3, 2, 1, 64, pages, page, mp, "bf16", quant)
+    got, code, _ = PE.run(p, t, {"paged_splits": 2, "paged_min_tiles": 2}, defer=True)
+    assert code == 0
+    ref, bound, _ = R.attention_ref(t, page)
+    R.check(got["O"], ref, bound, "late completions")
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_paged_attention_all_pages_missing_is_zero(quant):
+    t, pages = R.make("attend", 1, 1, 64, 16, 8, [100], [2], chunk=2, heads=2, quant=quant)
+    t["table"].fill_(-1)
+    p = irgen.paged_attention_ir(1, 2, 2, 1, 64, pages, 16, 8, "bf16", quant)
+    for opts in ({}, {"paged_splits": 2, "paged_min_tiles": 1}):
+        got, code, _ = PE.run(p, t, opts)
+        assert code == 0 and not got["O"].any()
+
+
+def test_paged_attention_lowering_rule():
+    """What the tensor cores take: head dim 64 or 128, a group of at most 128 heads, pages of 8, 16, 32 rows or whole
+    tiles; a changed nest stays on the CUDA cores."""
+    def kind(change=None, **kw):
+        base = dict(batch=1, chunk=1, heads=2, kv_heads=1, dim=64, pages=4, page=16, max_pages=2)
+        p = irgen.paged_attention_ir(**{**base, **kw})
+        if change:
+            change(p.graph["nodes"]["paged_attention"])
+        return compile_graph(Graph.from_dict(p.graph), p.meta()).kernels[0]["kind"]
+    assert kind() == "tcgen05_paged_attention"
+    assert kind(dim=128, page=192, window=3, sinks=1, scale=0.25) == "tcgen05_paged_attention"
+    for kw in (dict(dim=32), dict(dim=256), dict(page=4), dict(page=24), dict(page=96), dict(heads=129)):
+        assert kind(**kw) == "generic", kw
+
+    def swap(node):                                        # K and V exchanged in the nest
+        s = json.dumps(node["op_fields"]).replace('"KC"', '"XX"').replace('"VC"', '"KC"').replace('"XX"', '"VC"')
+        node["op_fields"] = json.loads(s)
+    assert kind(swap) == "generic"
+
+    def late(node):                                        # the causal limit one key further
+        s = json.dumps(node["op_fields"])
+        i = s.index('"minimum"')
+        node["op_fields"] = json.loads(s[:i] + s[i:].replace('"right": 1', '"right": 2', 1))
+    assert kind(late) == "generic"
