@@ -14,6 +14,7 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 
 namespace {
@@ -412,6 +413,109 @@ int emmy_tmap_encode_tiled(void* tmap, int dtype, uint32_t rank, uint64_t global
                 static_cast<CUtensorMapL2promotion>(l2_promotion),
                 static_cast<CUtensorMapFloatOOBfill>(oob_fill)),
             "cuTensorMapEncodeTiled");
+}
+
+// ---- launch plans ---------------------------------------------------------------------------
+namespace {
+struct PlanTmap {
+  uint32_t param, rank, box[5], elem[5];
+  int dtype, swizzle, l2promo;
+  uint64_t dims[5], strides[4];
+};
+struct Plan {
+  void* function;
+  uint32_t grid[3], block[3], cluster[3], dyn_smem, flags, nparams, ntmaps, has_tail;
+  uint32_t align[EMMY_PLAN_MAX_PARAMS];
+  PlanTmap tmaps[EMMY_PLAN_MAX_TMAPS];
+  uint64_t tail;
+};
+}  // namespace
+
+int emmy_plan_create(void* function, const uint32_t grid[3], const uint32_t block[3],
+                     const uint32_t cluster[3], uint32_t dyn_smem, uint32_t flags,
+                     const uint32_t* align, uint32_t nparams, void** plan) {
+  if (!function || !grid || !block || !plan || (nparams && !align))
+    return fail(EMMY_ERR_BAD_ARG, "null plan argument");
+  if (nparams > EMMY_PLAN_MAX_PARAMS) return fail(EMMY_ERR_BAD_ARG, "a plan takes at most %d parameters", EMMY_PLAN_MAX_PARAMS);
+  if (flags & ~static_cast<uint32_t>(EMMY_LAUNCH_PDL)) return fail(EMMY_ERR_BAD_ARG, "unknown launch flags 0x%x", flags);
+  Plan* p = new (std::nothrow) Plan();
+  if (!p) return fail(EMMY_ERR_BAD_ARG, "out of host memory");
+  p->function = function;
+  for (int i = 0; i < 3; ++i) {
+    p->grid[i] = grid[i];
+    p->block[i] = block[i];
+    p->cluster[i] = cluster ? cluster[i] : 1;
+  }
+  p->dyn_smem = dyn_smem;
+  p->flags = flags;
+  p->nparams = nparams;
+  for (uint32_t i = 0; i < nparams; ++i) p->align[i] = align[i];
+  *plan = p;
+  return 0;
+}
+
+int emmy_plan_add_tmap(void* plan, uint32_t param, int dtype, uint32_t rank, const uint64_t* dims,
+                       const uint64_t* strides_bytes, const uint32_t* box, int swizzle, int l2_promotion) {
+  Plan* p = static_cast<Plan*>(plan);
+  if (!p || !dims || !box || (rank > 1 && !strides_bytes)) return fail(EMMY_ERR_BAD_ARG, "null plan argument");
+  if (rank < 1 || rank > 5) return fail(EMMY_ERR_BAD_ARG, "tensor rank %u out of range", rank);
+  if (param >= p->nparams) return fail(EMMY_ERR_BAD_ARG, "tensor map of parameter %u of %u", param, p->nparams);
+  if (p->ntmaps >= EMMY_PLAN_MAX_TMAPS) return fail(EMMY_ERR_BAD_ARG, "a plan takes at most %d tensor maps", EMMY_PLAN_MAX_TMAPS);
+  PlanTmap& t = p->tmaps[p->ntmaps++];
+  t.param = param;
+  t.rank = rank;
+  t.dtype = dtype;
+  t.swizzle = swizzle;
+  t.l2promo = l2_promotion;
+  for (uint32_t i = 0; i < rank; ++i) {
+    t.dims[i] = dims[i];
+    t.box[i] = box[i];
+    t.elem[i] = 1;
+    if (i + 1 < rank) t.strides[i] = strides_bytes[i];
+  }
+  return 0;
+}
+
+int emmy_plan_set_tail(void* plan, uint64_t value) {
+  Plan* p = static_cast<Plan*>(plan);
+  if (!p) return fail(EMMY_ERR_BAD_ARG, "null plan");
+  p->tail = value;
+  p->has_tail = 1;
+  return 0;
+}
+
+int emmy_plan_launch(void* plan, const uint64_t* params, uint32_t nparams, void* stream) {
+  const Plan* p = static_cast<const Plan*>(plan);
+  if (!p || (nparams && !params)) return fail(EMMY_ERR_BAD_ARG, "null plan argument");
+  if (nparams != p->nparams) return fail(EMMY_ERR_BAD_ARG, "plan of %u parameters launched with %u", p->nparams, nparams);
+  // everything a launch needs lives on this call's stack, so calls may overlap
+  uint64_t vals[EMMY_PLAN_MAX_PARAMS + 1];
+  alignas(64) CUtensorMap maps[EMMY_PLAN_MAX_TMAPS];
+  void* args[EMMY_PLAN_MAX_PARAMS + EMMY_PLAN_MAX_TMAPS + 1];
+  uint32_t n = 0;
+  for (uint32_t i = 0; i < nparams; ++i) {
+    if (p->align[i] > 1 && params[i] % p->align[i])
+      return fail(EMMY_ERR_BAD_ARG, "parameter %u must be %u-byte aligned", i, p->align[i]);
+    vals[i] = params[i];
+    args[n++] = &vals[i];
+  }
+  for (uint32_t k = 0; k < p->ntmaps; ++k) {
+    const PlanTmap& t = p->tmaps[k];
+    if (int rc = emmy_tmap_encode_tiled(&maps[k], t.dtype, t.rank, params[t.param], t.dims, t.strides, t.box, t.elem, 0,
+                                        t.swizzle, t.l2promo, 0))
+      return rc;
+    args[n++] = &maps[k];
+  }
+  if (p->has_tail) {
+    vals[nparams] = p->tail;
+    args[n++] = &vals[nparams];
+  }
+  return emmy_launch_ex(p->function, p->grid, p->block, p->cluster, p->dyn_smem, stream, args, n, p->flags);
+}
+
+int emmy_plan_destroy(void* plan) {
+  delete static_cast<Plan*>(plan);
+  return 0;
 }
 
 int emmy_event_create(void** event) {

@@ -95,17 +95,17 @@ def geometry(chunk, heads, kv_heads):
 
 
 def plan_splits(batch, chunk, heads, kv_heads, page, max_pages, window, sinks, sms=148):
-    """(splits, least tiles of a part).  Parts are worth at least ``min_tiles`` tiles, enough that their f32
-    rows (written and read once) stay a small share of the keys read; and there are at most as many as fill
-    the GPU six times over, which evens out ragged batches."""
+    """(splits, least tiles of a part): one part where the units fill the GPU's two CTAs an SM, otherwise as many
+    parts as fill it, of at least 8 tiles.  Splitting more costs more than it evens out here: a part of 128 rows
+    writes and the join reads 64 KiB of f32, as much as two tiles of keys and values (a 2048-token chunk over
+    8192 keys ran at 876 TFLOP/s in one part and 647 in up to four)."""
     group, tq, ntile, rows = geometry(chunk, heads, kv_heads)
     longest = -(-max_pages * page // BKV)
     if window is not None:
         longest = min(longest, -(-sinks // BKV) + (window + min(tq, chunk) - 1) // BKV + 2)
-    min_tiles = max(4, rows // 4)
+    min_tiles = 8
     units = batch * kv_heads * ntile
-    splits = max(1, min(-(-longest // min_tiles), -(-6 * 2 * sms // units), 128))
-    return splits, min_tiles
+    return max(1, min(longest // min_tiles, 2 * sms // units)), min_tiles
 
 
 def _unit(e, k, b_len, b_new, c0, splits, min_tiles, tq, chunk, cap, window, sinks):
@@ -138,7 +138,7 @@ def _unit(e, k, b_len, b_new, c0, splits, min_tiles, tq, chunk, cap, window, sin
 def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_pages, dtype, quant, window, sinks,
                           scale, names, scratch, splits, min_tiles, prefix=""):
     """The launch record and PTX; ``names``: Q, KC, VC, (KS, VS,) table, lens, fresh, O; ``scratch``: the parts'
-    buffer names."""
+    buffer, all their O rows and then their m and l."""
     D = dim
     group, tq, ntile, rows = geometry(chunk, heads, kv_heads)
     units = batch * kv_heads * ntile
@@ -183,6 +183,7 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     cta = o("mov.u32", "%ctaid.x")
     err, o_ptr = gptr("p_err"), gptr("p_O")
     if splits > 1:
+        e("griddepcontrol.launch_dependents;")                  # the join's blocks may come up and wait
         unit, sp = o("div.u32", cta, splits), o("rem.u32", cta, splits)
     else:
         unit, sp = cta, None
@@ -848,7 +849,7 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
             e("tcgen05.wait::ld.sync.aligned;")
             for i in range(4):
                 e(f"@{p_row} st.global.v8.f32 [{pa}+{128 * c + 32 * i}], {{{', '.join(regs[8 * i:8 * i + 8])}}};")
-        mla = at(gptr("p_ml"), wide(pi, 8))
+        mla = at(at(gptr("p_part"), grid * rows * D * 4), wide(pi, 8))
         # the parts' O and l stand for 2^-negm; a part that saw nothing has m = -inf
         meff = o("sub.f32", mref, _f32(lift), cls="f")
         e(f"@{p_row} st.global.v2.f32 [{mla}], {{{meff}, {lsum}}};")
@@ -872,9 +873,8 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     params += [("table", tn, 4), ("lens", ln, 4), ("fresh", fn, 4), ("O", on, 32)]
     sc_spec = []
     if splits > 1:
-        params += [("part", scratch[0], 32), ("ml", scratch[1], 8)]
-        sc_spec = [{"name": scratch[0], "dtype": "f32", "shape": [grid * rows, D]},
-                   {"name": scratch[1], "dtype": "f32", "shape": [grid * rows, 2]}]
+        params += [("part", scratch, 32)]
+        sc_spec = [{"name": scratch, "dtype": "f32", "shape": [grid * rows, D + 2], "per_call": True}]
     tmaps = []
     if not quant:
         es = 2
@@ -897,10 +897,11 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
 
 
 def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype, window, sinks, names, scratch, splits,
-               min_tiles):
+               min_tiles, locate=None):
     """The second entry: rows whose unit was split, o = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.  One block a row;
     its four warps take every fourth part, so that a row of 100 parts is 25 loads deep.  Rows of units that
-    fit one part are written already and return at once."""
+    fit one part are written already and return at once.  ``locate`` finds a row's parts (the default: ``splits`` parts
+    a unit, of at least ``min_tiles`` tiles each)."""
     D = dim
     group, tq, ntile, rows = geometry(chunk, heads, kv_heads)
     per_lane = D // 32
@@ -915,31 +916,51 @@ def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype,
 
     tid = o("mov.u32", "%tid.x")
     warp, lane = o("shr.u32", tid, 5), o("and.b32", tid, 31)
+    e("griddepcontrol.wait;")                                   # the parts are written
     row = o("mov.u32", "%ctaid.x")
     h, bc = o("rem.u32", row, heads), o("div.u32", row, heads)
     c, b = o("rem.u32", bc, chunk), o("div.u32", bc, chunk)
     b_len = o("ld.global.nc.u32", f"[{at(gptr('p_lens'), b, 4)}]")
     b_new = o("ld.global.nc.u32", f"[{at(gptr('p_fresh'), b, 4)}]")
     e(f"@{e.cond('ge.s32', c, b_new)} ret;")
-    tile = o("div.u32", c, tq)
-    c0 = o("mul.lo.u32", tile, tq)
-    w = _unit(e, None, b_len, b_new, c0, splits, min_tiles, tq, chunk, max_pages * page, window, sinks)
-    e(f"@{e.cond('le.u32', w['total'], w['per'])} ret;")
-    nact = o("div.u32", o("sub.u32", o("add.u32", w["total"], w["per"]), 1), w["per"])
-    kvh = o("div.u32", h, group)
-    unit = o("mad.lo.u32", o("sub.u32", ntile - 1, tile), batch, b)
-    unit = o("mad.lo.u32", unit, kv_heads, kvh)
-    rowl = o("mad.lo.u32", o("sub.u32", c, c0), group, o("rem.u32", h, group))
-    base = o("mad.lo.u32", o("mul.lo.u32", unit, splits), rows, rowl)         # part 0's row; parts are ``rows`` apart
-    ml, part = gptr("p_ml"), gptr("p_part")
+    if locate is None:
+        tile = o("div.u32", c, tq)
+        c0 = o("mul.lo.u32", tile, tq)
+        w = _unit(e, None, b_len, b_new, c0, splits, min_tiles, tq, chunk, max_pages * page, window, sinks)
+        e(f"@{e.cond('le.u32', w['total'], w['per'])} ret;")
+        nact = o("div.u32", o("sub.u32", o("add.u32", w["total"], w["per"]), 1), w["per"])
+        unit = o("mad.lo.u32", o("sub.u32", ntile - 1, tile), batch, b)
+        unit = o("mad.lo.u32", unit, kv_heads, o("div.u32", h, group))
+        rowl = o("mad.lo.u32", o("sub.u32", c, c0), group, o("rem.u32", h, group))
+        base = o("mad.lo.u32", o("mul.lo.u32", unit, splits), rows, rowl)     # part 0's row; parts are ``rows`` apart
+        part_rows = batch * kv_heads * ntile * splits * rows
+
+        def part_row(s_):
+            return o("mad.lo.u32", s_, rows, base)
+    else:
+        def zero_row(p_none):
+            """A row that sees no key, where ``p_none``: 0."""
+            l_ = e.L("nz")
+            e(f"@!{p_none} bra {l_};")
+            e(f"@{e.cond('ge.u32', tid, D // 2)} ret;")
+            e(f"st.global.b32 [{at(at(gptr('p_O'), row, D * 2), tid, 4)}], {o('mov.b32', 0)};")
+            e("ret;")
+            e.label(l_)
+        nact, part_row, part_rows = locate(e, lambda x, y: o("add.s64", x, y, cls="rd"), gptr, lane, b, c, h, zero_row)
+    part = gptr("p_part")
+    ml = o("add.s64", part, part_rows * D * 4, cls="rd")
     # the largest reference of the row's parts (every warp on its own)
     m = o("mov.b32", "0fFF800000", cls="f")
-    for k in range(-(-splits // 32)):
-        s = o("add.u32", lane, 32 * k)
-        ok = e.cond("lt.u32", s, nact)
-        v = o("mov.b32", "0fFF800000", cls="f")
-        e(f"@{ok} ld.global.f32 {v}, [{at(ml, o('mad.lo.u32', s, rows, base), 8)}];")
-        e(f"max.f32 {m}, {m}, {v};")
+    s = o("mov.u32", lane)
+    l_m, l_md = e.L("m"), e.L("md")
+    e.label(l_m)
+    e(f"@{e.cond('ge.u32', o('and.b32', s, -32), nact)} bra {l_md};")           # the same for the warp
+    v = o("mov.b32", "0fFF800000", cls="f")
+    e(f"@{e.cond('lt.u32', s, nact)} ld.global.f32 {v}, [{at(ml, part_row(s), 8)}];")
+    e(f"max.f32 {m}, {m}, {v};")
+    e(f"add.u32 {s}, {s}, 32;")
+    e(f"bra {l_m};")
+    e.label(l_md)
     for d in (16, 8, 4, 2, 1):
         e(f"max.f32 {m}, {m}, {o('shfl.sync.bfly.b32', m, d, 31, -1, cls='f')};")
     e(f"@{e.cond('eq.f32', m, '0fFF800000')} mov.b32 {m}, 0f00000000;")
@@ -956,7 +977,7 @@ def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype,
     for u in range(UN):
         su = o("add.u32", s, 4 * u)
         ok = e.cond("lt.u32", su, nact)
-        idx = o("mad.lo.u32", su, rows, base)
+        idx = part_row(su)
         ms, ls = o("mov.b32", "0fFF800000", cls="f"), o("mov.b32", "0f00000000", cls="f")
         e(f"@{ok} ld.global.v2.f32 {{{ms}, {ls}}}, [{at(ml, idx, 8)}];")
         xs = [o("mov.b32", "0f00000000", cls="f") for _ in range(per_lane)]
@@ -996,11 +1017,11 @@ def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype,
     oa = at(at(gptr("p_O"), row, D * 2), tid, 4)
     e(f"st.global.b32 [{oa}], {word};")
     ln, fn, on = names
-    params = [("lens", ln, 4), ("fresh", fn, 4), ("O", on, 4), ("part", scratch[0], 32), ("ml", scratch[1], 8)]
+    params = [("lens", ln, 4), ("fresh", fn, 4), ("O", on, 4), ("part", scratch, 32)]
     text = [f".visible .entry {name}(", ",\n".join(f"\t.param .u64 p_{p}" for p, _, _ in params), ")",
             ".reqntid 128, 1, 1", "{"]
     text += e.decls() + e.lines + ["\tret;", "}"]
     return {"name": name, "kind": "paged_attention_join", "params": [n for _, n, _ in params], "raw_entry": text,
             "raw_decls": [f".shared .align 16 .b8 {name}_sum[{4 * D * 4}];", f".shared .align 16 .b8 {name}_l[16];"],
             "grid": [batch * chunk * heads, 1, 1], "block": [128, 1, 1], "dyn_smem": 0,
-            "align": {n: a_ for _, n, a_ in params}, "zero_outputs": []}
+            "align": {n: a_ for _, n, a_ in params}, "zero_outputs": [], "pdl": True}

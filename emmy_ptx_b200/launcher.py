@@ -38,6 +38,13 @@ SIGNATURES = {
                            ctypes.c_uint32],
     "emmy_tmap_encode_tiled": [vp, ctypes.c_int, ctypes.c_uint32, ctypes.c_uint64, c_u64p, c_u64p, c_u32p,
                                c_u32p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int],
+    "emmy_plan_create": [vp, c_u32p, c_u32p, c_u32p, ctypes.c_uint32, ctypes.c_uint32, c_u32p, ctypes.c_uint32,
+                         ctypes.POINTER(vp)],
+    "emmy_plan_add_tmap": [vp, ctypes.c_uint32, ctypes.c_int, ctypes.c_uint32, c_u64p, c_u64p, c_u32p, ctypes.c_int,
+                           ctypes.c_int],
+    "emmy_plan_set_tail": [vp, ctypes.c_uint64],
+    "emmy_plan_launch": [vp, c_u64p, ctypes.c_uint32, vp],
+    "emmy_plan_destroy": [vp],
     "emmy_event_create": [ctypes.POINTER(vp)],
     "emmy_event_destroy": [vp],
     "emmy_event_record": [vp, vp],
@@ -216,6 +223,37 @@ class Device:
         check(self.lib.emmy_launch_ex(fn, dims3(grid), dims3(block), dims3(cluster), int(dyn_smem),
                                       vp(stream or 0), args, n, LAUNCH_PDL if pdl else 0), "emmy_launch_ex")
         self.launches += 1
+
+    def plan(self, fn, grid, block, dyn_smem: int, align, cluster=(1, 1, 1), pdl: bool = False, tmaps=(),
+             tail: int | None = None):
+        """A launch plan (see ``emmy_plan_create``): ``tmaps`` is a list of (parameter index, dtype code, dims,
+        strides in bytes, box, swizzle code, L2 promotion), ``tail`` the last 64-bit parameter."""
+        self._use()
+        h = vp()
+        n = len(align)
+        check(self.lib.emmy_plan_create(fn, dims3(grid), dims3(block), dims3(cluster), int(dyn_smem),
+                                        LAUNCH_PDL if pdl else 0, (ctypes.c_uint32 * n)(*align), n, ctypes.byref(h)),
+              "emmy_plan_create")
+        for param, dtype, dims, strides, box, swizzle, l2 in tmaps:
+            r = len(dims)
+            check(self.lib.emmy_plan_add_tmap(h, param, dtype, r, (ctypes.c_uint64 * r)(*dims),
+                                              (ctypes.c_uint64 * max(r - 1, 1))(*strides), (ctypes.c_uint32 * r)(*box),
+                                              swizzle, l2), "emmy_plan_add_tmap")
+        if tail is not None:
+            check(self.lib.emmy_plan_set_tail(h, tail), "emmy_plan_set_tail")
+        return h
+
+    def launch_plan(self, plan, params, stream: int) -> None:
+        """Launch ``plan`` with ``params`` (a ctypes array of 64-bit values) on ``stream``."""
+        if Device._active != self.index:
+            self._use()
+        rc = self.lib.emmy_plan_launch(plan, params, len(params), stream)
+        if rc:
+            check(rc, "emmy_plan_launch")
+        self.launches += 1
+
+    def destroy_plan(self, plan) -> None:
+        check(self.lib.emmy_plan_destroy(plan), "emmy_plan_destroy")
 
     def tmap_encode_tiled(self, out_buf, dtype: int, gaddr: int, dims, strides_bytes, box, elem_strides=None,
                           swizzle: int = 0, l2promo: int = 2, oob_fill: int = 0, interleave: int = 0) -> None:

@@ -475,25 +475,81 @@ def match_paged_attention(graph, node):
     return None
 
 
-def _lower_paged_attention(node, kw, prefix, options):
-    """The tensor-core entries of a paged attention: one, or two when its units are split."""
-    from .kernels import tc_paged_attention as tpa
-    if not tpa.supported(kw["dim"], kw["heads"], kw["kv_heads"], kw["page"]):
+def match_cache_copy(graph, node):
+    """("write" or "read", keyword arguments of its builder) when the kernel is the nest of
+    :func:`.irgen.cache_write_ir` or :func:`.irgen.cache_read_ir`, else None.  Every parameter is a buffer's
+    size or type."""
+    from .irgen import cache_read_ir, cache_write_ir
+    vals = graph.values()
+    ins, outs = [vals.get(n) for n in node.inputs], list(node.outputs)
+    if any(v is None for v in ins):
         return None
+    if len(ins) == 5 and len(outs) in (2, 4):
+        kind, build, quant, cache, table = "write", cache_write_ir, len(outs) == 4, outs[0], ins[2]
+        names = ["K", "V", "table", "lens", "fresh"], ["KC", "VC", "KS", "VS"]
+        x = ins[0]
+    elif len(ins) in (4, 6) and len(outs) == 2:
+        kind, build, quant, cache, table = "read", cache_read_ir, len(ins) == 6, ins[0], ins[-2]
+        names = ["KC", "VC", *(["KS", "VS"] if len(ins) == 6 else []), "table", "lens"], ["KR", "VR"]
+        x = outs[0]
+    else:
+        return None
+    if len(cache.shape) != 4 or len(x.shape) != 4 or len(table.shape) != 2:
+        return None
+    kw = dict(batch=x.shape[0], kv_heads=x.shape[2], dim=x.shape[3], pages=cache.shape[0], page=cache.shape[2],
+              max_pages=table.shape[1], dtype=dt_name(x.dtype), quant=quant)
+    kw["chunk" if kind == "write" else "length"] = x.shape[1]
+    try:
+        p = build(**kw)
+    except ValueError:
+        return None
+    want = {a.name: (tuple(a.shape), a.dtype) for a in p.args}
+    got = {**dict(zip(names[0], ins)), **dict(zip(names[1], outs))}
+    if any((tuple(v.shape), dt_name(v.dtype)) != want[n] for n, v in got.items()):
+        return None
+    if not is_canonical(node, p, {v.name: n for n, v in got.items()}):
+        return None
+    return kind, kw
+
+
+def _args_of(graph, node) -> list:
+    """Name, type and shape of every tensor of the kernel, for the runtime's checks."""
+    vals = graph.values()
+    return [{"name": v.name, "dtype": dt_name(v.dtype), "shape": list(v.shape)}
+            for v in [*(vals[n] for n in node.inputs), *node.outputs]]
+
+
+def _lower_paged_attention(graph, node, kw, prefix, options):
+    """The tensor-core entries of a paged attention: one, or two when its units are split.  Units of few rows
+    (a decode step, a short draft) are bound by the cache's bytes and take the register form."""
+    from .kernels import paged_rows as pr, tc_paged_attention as tpa
     geo = {k: kw[k] for k in ("batch", "chunk", "heads", "kv_heads", "page", "max_pages", "window", "sinks")}
-    splits, min_tiles = tpa.plan_splits(**geo, sms=int(options.get("sms", 148)))
-    splits = int(options.get("paged_splits", splits))
-    min_tiles = int(options.get("paged_min_tiles", min_tiles))
+    sms = int(options.get("sms", 148))
+    rows = kw["chunk"] * (kw["heads"] // kw["kv_heads"])
+    few = (pr.supported(kw["dim"], kw["chunk"], kw["heads"], kw["kv_heads"], kw["page"])
+           and rows <= int(options.get("paged_rows", pr.MAX_ROWS)))
     name = node.op.name
     names = [*node.inputs, node.outputs[0].name]
-    scratch = (f"{prefix}{name}__part", f"{prefix}{name}__ml")
-    main = tpa.paged_attention_entry(name, **kw, names=names, scratch=scratch, splits=splits, min_tiles=min_tiles,
-                                     prefix=prefix)
-    if splits == 1:
-        return main
-    join = tpa.join_entry(f"{name}_join", **geo, dim=kw["dim"], dtype=kw["dtype"], names=names[-3:], scratch=scratch,
-                          splits=splits, min_tiles=min_tiles)
-    return [main, join]
+    scratch = f"{prefix}{name}__part"
+    jkw = dict(**geo, dim=kw["dim"], dtype=kw["dtype"], names=names[-3:], scratch=scratch)
+    if few:
+        ctas = pr.plan_ctas(**{k: v for k, v in geo.items() if k != "heads"}, sms=sms)
+        if "paged_splits" in options:
+            n = int(options["paged_splits"])
+            ctas = n * kw["batch"] * kw["kv_heads"] if n > 1 and kw["batch"] <= pr.MAX_SPREAD_BATCH else 0
+        least = int(options.get("paged_min_tiles", pr.MIN_TILES))
+        main = pr.paged_rows_entry(name, **kw, names=names, scratch=scratch, ctas=ctas, min_tiles=least, prefix=prefix)
+        join = pr.spread_join_entry(f"{name}_join", **jkw, ctas=ctas, min_tiles=least) if ctas else None
+    elif tpa.supported(kw["dim"], kw["heads"], kw["kv_heads"], kw["page"]):
+        splits, least = tpa.plan_splits(**geo, sms=sms)
+        splits, least = int(options.get("paged_splits", splits)), int(options.get("paged_min_tiles", least))
+        main = tpa.paged_attention_entry(name, **kw, names=names, scratch=scratch, splits=splits, min_tiles=least,
+                                         prefix=prefix)
+        join = tpa.join_entry(f"{name}_join", **jkw, splits=splits, min_tiles=least) if splits > 1 else None
+    else:
+        return None
+    main["args"] = _args_of(graph, node)
+    return [main, join] if join else main
 
 
 def _flat(body):
@@ -609,5 +665,11 @@ def try_lower(graph, node, kmeta, prefix, options):
         return [pre0, att0, pre1, att1]
     kw = match_paged_attention(graph, node)
     if kw is not None:
-        return _lower_paged_attention(node, kw, prefix, options)
+        return _lower_paged_attention(graph, node, kw, prefix, options)
+    hit = match_cache_copy(graph, node)
+    if hit is not None:
+        from .kernels import paged_copy
+        build = paged_copy.cache_write_entry if hit[0] == "write" else paged_copy.cache_read_entry
+        rec = build(node.op.name, **hit[1], names=[*node.inputs, *[v.name for v in node.outputs]])
+        return {**rec, "args": _args_of(graph, node)}
     return None

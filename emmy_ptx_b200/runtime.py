@@ -6,6 +6,10 @@ record lists (``zero_outputs``, tools/stress.py:106-111), checks every pointer's
 what the emitted code assumes, encodes TMA descriptors for tensor-core kernels, and launches
 the entries in order on the caller's stream.  Buffers are caller-owned tensors on the device.
 
+Modules whose records list their tensors (``"args"``: the paged-cache operators) go a shorter way: each entry has a
+launch plan in the C library, a call checks its tensors against the list and passes pointers, and scratch
+that a record marks ``"per_call"`` is allocated by the call.
+
 An entry whose record says ``"stream": 1`` runs on the Executable's side stream instead, so that it
 overlaps the main stream's next entries; ``"after": [entry, ...]`` names entries it must follow
 (on the other stream: a fork or join through an event).  The side stream always rejoins the caller's
@@ -16,7 +20,7 @@ from __future__ import annotations
 import ctypes
 
 from .compiler import CompiledModule, compile_ir
-from .launcher import Device
+from .launcher import Device, EmmyError
 from .data import torch_dtype
 
 _TMAP_DTYPE = {"u8": 0, "u32": 2, "i32": 3, "f16": 6, "f32": 7, "f64": 8, "bf16": 9}   # CUtensorMapDataType (cuda.h)
@@ -56,7 +60,7 @@ class Executable:
         self.scratch: dict = {}
         for rec in compiled.kernels:
             for spec in rec.get("scratch", []):
-                if spec["name"] not in self.scratch:
+                if spec["name"] not in self.scratch and not spec.get("per_call"):
                     self.scratch[spec["name"]] = self._device_tensor(tuple(spec["shape"]), torch_dtype(spec["dtype"]))
                     if spec.get("zeroed"):
                         # a self-zeroing accumulator: zero once here, every launch leaves it zero
@@ -75,6 +79,68 @@ class Executable:
         if any(spec.get("kind") == "errword" for rec in compiled.kernels for spec in rec.get("extra", [])):
             self.err = self._device_tensor((4,), torch.int32)
             self.err.zero_()
+        # a module whose first record lists its tensors ("args") is launched from plans
+        self.plans = None
+        if compiled.kernels and compiled.kernels[0].get("args"):
+            self._make_plans()
+
+    def _make_plans(self) -> None:
+        """One launch plan per entry, and what a call's tensors must be."""
+        import torch
+        self._args = [(a["name"], torch_dtype(a["dtype"]), tuple(a["shape"])) for a in self.records[0]["args"]]
+        self._calls = []
+        self._temp = {}                      # scratch each call allocates: name -> (element count, dtype)
+        self.plans = []
+        for rec, fn in zip(self.records, self.funcs):
+            for spec in rec.get("scratch", []):
+                n = 1
+                for x in spec["shape"]:
+                    n *= int(x)
+                self._temp[spec["name"]] = (n, torch_dtype(spec["dtype"]))
+            names = rec["params"]
+            tmaps = [(names.index(s["tensor"]), _TMAP_DTYPE[s["dtype"]], s["dims"], s["strides"], s["box"],
+                      _SWIZZLE[s.get("swizzle", "128B")], s.get("l2promo", 2)) for s in rec.get("tmaps", [])]
+            self.plans.append(self.dev.plan(
+                fn, rec["grid"], rec["block"], rec.get("dyn_smem", 0), [int(rec["align"].get(n, 1)) for n in names],
+                cluster=rec.get("cluster", (1, 1, 1)), pdl=bool(rec.get("pdl")), tmaps=tmaps,
+                tail=self.err.data_ptr() if rec.get("extra") else None))
+            self._calls.append((names, ctypes.c_uint64 * len(names)))
+
+    def _run_plans(self, tensors: dict, stream) -> None:
+        """Check the call's tensors (type, shape, layout, device), allocate its scratch on its stream and launch
+        every entry.  Scratch is the call's own (torch's allocator, so a captured call's belongs to its
+        graph): calls of one Executable may overlap on the GPU as long as what they write does not."""
+        import torch
+        ptrs = {}
+        for name, dtype, shape in self._args:
+            t = tensors.get(name)
+            if t is None:
+                raise ValueError(f"kernel {self.records[0]['entry']!r} needs the tensor {name!r}")
+            if t.dtype is not dtype or t.shape != shape or t.get_device() != self.index or not t.is_contiguous():
+                raise ValueError(
+                    f"{name!r} must be a contiguous {dtype} tensor of shape {list(shape)} on cuda:{self.index}, not "
+                    f"{'a strided' if not t.is_contiguous() else 'a'} {t.dtype} of shape {list(t.shape)} on {t.device}")
+            ptrs[name] = t.data_ptr()
+        keep = []
+        if self._temp:
+            device = f"cuda:{self.index}"
+            if stream is None:
+                keep = [torch.empty(n, dtype=dt, device=device) for n, dt in self._temp.values()]
+            else:
+                with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+                    keep = [torch.empty(n, dtype=dt, device=device) for n, dt in self._temp.values()]
+            for name, t in zip(self._temp, keep):
+                ptrs[name] = t.data_ptr()
+        if stream is None:
+            stream = torch.cuda.current_stream(self.index).cuda_stream
+        for plan, (names, arr), rec in zip(self.plans, self._calls, self.records):
+            try:
+                self.dev.launch_plan(plan, arr(*[ptrs[n] for n in names]), stream)
+            except EmmyError:
+                for n in names:
+                    if ptrs[n] % int(rec["align"].get(n, 1)):
+                        raise ValueError(f"{n!r} must be {rec['align'][n]}-byte aligned for kernel {rec['entry']!r}") from None
+                raise
 
     def _device_tensor(self, shape, dtype):
         """Device memory the Executable owns (scratch between entries, the error word)."""
@@ -186,6 +252,8 @@ class Executable:
         the side stream, forked from ``stream`` at the first such entry and joined back at the end.
         ``zero=False`` skips the output zeroing (for replaying kernels only)."""
         import torch
+        if self.plans is not None:
+            return self._run_plans(tensors, stream)
         if stream is None:
             stream = torch.cuda.current_stream(self.index).cuda_stream
         if self.side is None:
@@ -216,6 +284,10 @@ class Executable:
         return self.dev.launches
 
     def close(self) -> None:
+        for plan in self.plans or ():
+            self.dev.destroy_plan(plan)
+        if self.plans:
+            self.plans = []
         if self.module is not None:
             self.dev.unload(self.module)
             self.module = None

@@ -114,6 +114,24 @@ int emmy_tmap_encode_tiled(void* tmap, int dtype, uint32_t rank, uint64_t global
                            const uint32_t* box, const uint32_t* elem_strides,
                            int interleave, int swizzle, int l2_promotion, int oob_fill);
 
+/* A launch plan: everything of a launch that does not change from call to call, so that a latency-bound
+ * step (one decode token) pays one call with its pointers.  The plan holds the function, its geometry,
+ * the alignment each pointer must have, the tensor maps to encode from pointers (in parameter order,
+ * after the pointers) and one last 64-bit value (the status word's address).  emmy_plan_launch checks
+ * the pointers' alignment (EMMY_ERR_BAD_ARG), encodes the maps and launches; it keeps its working
+ * memory on the stack, so calls on one plan may overlap.  A plan must be destroyed before its module
+ * is unloaded.  No reference counterpart. */
+#define EMMY_PLAN_MAX_PARAMS 16
+#define EMMY_PLAN_MAX_TMAPS 4
+int emmy_plan_create(void* function, const uint32_t grid[3], const uint32_t block[3],
+                     const uint32_t cluster[3], uint32_t dyn_smem, uint32_t flags,
+                     const uint32_t* align, uint32_t nparams, void** plan);
+int emmy_plan_add_tmap(void* plan, uint32_t param, int dtype, uint32_t rank, const uint64_t* dims,
+                       const uint64_t* strides_bytes, const uint32_t* box, int swizzle, int l2_promotion);
+int emmy_plan_set_tail(void* plan, uint64_t value);
+int emmy_plan_launch(void* plan, const uint64_t* params, uint32_t nparams, void* stream);
+int emmy_plan_destroy(void* plan);
+
 /* Events and synchronisation (tools/bench.py:66-83). */
 int emmy_event_create(void** event);
 int emmy_event_destroy(void* event);

@@ -1,5 +1,5 @@
-"""Runs the paged attention's tensor-core entries in the CPU emulator (:mod:`tests.tcemu`), with the packed
-16-bit subtraction its byte conversion uses; test infrastructure only."""
+"""Runs the paged attention's tensor-core entries in the CPU emulator (:mod:`tests.tcemu`), with what they
+use beyond it: packed 16-bit subtractions, warp matrix products and plain bulk copies; test infrastructure only."""
 from __future__ import annotations
 
 import numpy as np
@@ -12,14 +12,65 @@ from tests.tcemu import TcEmulator, _halves_to_float
 from oracle.interp import f32_to_bf16_bits
 
 
+_OWN = ("popc.b32", "sub.rn.bf16x2", "sub.rn.f16x2", "mma.sync", "cp.async.bulk.shared")
+
+
 class PagedEmulator(TcEmulator):
+    """``mma.sync`` m16n8k16 is a warp's collective; plain bulk copies complete like TMA boxes."""
+
     @staticmethod
     def _decode(x):
-        if not x.label and x.op.startswith(("sub.rn.bf16x2", "sub.rn.f16x2")):
-            return (7,)
+        if not x.label and x.op.startswith(_OWN):
+            return (7,)                                     # straight to _extra
         return TcEmulator._decode(x)
 
+    def _tma_write(self, dst, tm, cs, mb, smem, mem):
+        if isinstance(tm, tuple):
+            smem[dst:dst + tm[2]] = mem.load(tm[1], tm[2])
+            return self._complete_tx(mb, tm[2])
+        return super()._tma_write(dst, tm, cs, mb, smem, mem)
+
+    def _collective(self, members, args):
+        if not members[0].coll[0].startswith("mma.sync"):
+            return super()._collective(members, args)
+        ins = self.ins[members[0].pc]
+        groups = [[r.strip() for r in o.strip().strip("{}").split(",")] for o in ins.ops]
+        D, A, B, C = groups
+        bf = int("bf16" in ins.op)
+        lanes = sorted(members, key=lambda t: t.lane)
+        halves = lambda v: _halves_to_float(np.array([v & 0xFFFF, v >> 16 & 0xFFFF], np.uint16), bf)
+        a, b, c = np.zeros((16, 16)), np.zeros((16, 8)), np.zeros((16, 8))
+        for t in lanes:
+            g, q = t.lane >> 2, t.lane & 3
+            for r in range(4):
+                a[g + 8 * (r & 1), 2 * q + 8 * (r >> 1):2 * q + 8 * (r >> 1) + 2] = halves(t.regs[A[r]])
+                c[g + 8 * (r >> 1), 2 * q + (r & 1)] = np.uint32(t.regs[C[r]]).view(np.float32)
+            for r in range(2):
+                b[2 * q + 8 * r:2 * q + 8 * r + 2, g] = halves(t.regs[B[r]])
+        with np.errstate(all="ignore"):
+            d = (a @ b + c).astype(np.float32)
+        for t in lanes:
+            g, q = t.lane >> 2, t.lane & 3
+            for r in range(4):
+                t.regs[D[r]] = int(d[g + 8 * (r >> 1), 2 * q + (r & 1)].view(np.uint32))
+
     def _extra(self, th, x, op, ops, regs, val, addr, smem, mem):
+        if op.startswith("popc.b32"):
+            regs[ops[0]] = bin(val(ops[1]) & 0xFFFFFFFF).count("1")
+            return "cont"
+        if op.startswith("mma.sync"):
+            th.pc -= 1
+            th.state, th.coll = "coll", (op, 0xFFFFFFFF)
+            return "block"
+        if op.startswith("cp.async.bulk.shared::cluster.global"):
+            dst, src, n, mb = addr(ops[0]) & 0xFFFFFFFF, addr(ops[1]), val(ops[2]), addr(ops[3]) & 0xFFFFFFFF
+            assert dst % 16 == 0 and src % 16 == 0 and n % 16 == 0 and dst + n <= len(smem), (dst, src, n)
+            if self.defer:
+                self.queue_tma.append((dst, ("bulk", src, n), None, mb, mem))
+            else:
+                smem[dst:dst + n] = mem.load(src, n)
+                self._complete_tx(mb, n)
+            return "cont"
         if op.startswith(("sub.rn.bf16x2", "sub.rn.f16x2")):
             bf = "bf16" in op
             a, b = (np.array([val(o) & 0xFFFF, (val(o) >> 16) & 0xFFFF], np.uint16) for o in ops[1:3])

@@ -9,7 +9,7 @@ from emmy_ptx_b200.compiler import compile_graph
 from emmy_ptx_b200.ir import Graph
 from emmy_ptx_b200.runtime import Executable
 from tests import pagedref as R
-from tests.test_paged_cache import ATTENDS, READS, TENSOR, WRITES, broken_table, same
+from tests.test_paged_cache import ATTENDS, FORMS, READS, TENSOR, WRITES, awkward_rows, broken_table, form_opts, same
 
 pytestmark = pytest.mark.gpu
 
@@ -34,15 +34,16 @@ def go(p, t, opts=None):
 
 
 @pytest.mark.parametrize("dtype,quant", [("bf16", False), ("f16", False), ("bf16", True), ("f16", True)])
-@pytest.mark.parametrize("case", TENSOR, ids=lambda c: "x".join(map(str, c[:7])))
-def test_paged_attention(case, dtype, quant):
-    B, C, H, hk, d, page, mp, lens, fresh, window, sinks, opts = case
+@pytest.mark.parametrize("form,case", [(f, c) for f in FORMS for c in TENSOR if form_opts(f, c)],
+                         ids=lambda c: c if isinstance(c, str) else "x".join(map(str, c[:7])))
+def test_paged_attention(form, case, dtype, quant):
+    B, C, H, hk, d, page, mp, lens, fresh, window, sinks, _ = case
     t, pages = R.make("attend", B, hk, d, page, mp, lens, fresh, chunk=C, heads=H, dtype=dtype, quant=quant, seed=H + C)
     p = irgen.paged_attention_ir(B, C, H, hk, d, pages, page, mp, dtype, quant, window, sinks)
-    got, kinds = go(p, t, opts)
-    assert kinds[0] == "tcgen05_paged_attention"
+    got, kinds = go(p, t, form_opts(form, case))
+    assert kinds[0] == FORMS[form]
     ref, bound, _ = R.attention_ref(t, page, window, sinks)
-    R.check(got["O"], ref, bound, "tensor cores")
+    R.check(got["O"], ref, bound, form)
 
 
 @pytest.mark.parametrize("dtype,quant", [("bf16", False), ("f16", True)])
@@ -58,6 +59,7 @@ def test_paged_attention_cuda_cores(case, dtype, quant):
     R.check(got["O"], ref, bound, "CUDA cores")
 
 
+@pytest.mark.parametrize("rows", [0, 64])
 @pytest.mark.parametrize("quant", [False, True])
 @pytest.mark.parametrize("B,C,H,hk,d,page,lens,window,sinks", [
     (3, 1, 8, 2, 128, 16, [2111, 63, 1024], None, 0),
@@ -66,13 +68,13 @@ def test_paged_attention_cuda_cores(case, dtype, quant):
     (1, 150, 6, 2, 64, 8, [1300], 333, 70),
     (4, 1, 16, 1, 128, 128, [2000, 1, 129, 800], 500, 4),
 ], ids=["decode", "draft", "chunk", "chunk-window", "decode-window"])
-def test_paged_attention_longer(B, C, H, hk, d, page, lens, window, sinks, quant):
+def test_paged_attention_longer(B, C, H, hk, d, page, lens, window, sinks, quant, rows):
     mp = -(-max(lens) // page) + 1
     fresh = [min(C, n) for n in lens]
     t, pages = R.make("attend", B, hk, d, page, mp, lens, fresh, chunk=C, heads=H, quant=quant, seed=d + C, sizes=2.0)
     p = irgen.paged_attention_ir(B, C, H, hk, d, pages, page, mp, "bf16", quant, window, sinks)
-    got, kinds = go(p, t)
-    assert kinds[0] == "tcgen05_paged_attention"
+    got, kinds = go(p, t, {"paged_rows": rows})
+    assert kinds[0] == FORMS["rows" if C * (H // hk) <= rows else "tiles"]
     ref, bound, _ = R.attention_ref(t, page, window, sinks)
     R.check(got["O"], ref, bound, "longer")
 
@@ -87,12 +89,14 @@ def test_paged_attention_missing_pages(page, quant):
     t["table"][1, 0] = 2 ** 31 - 1
     p = irgen.paged_attention_ir(2, 3, 2, 1, 64, pages, page, mp, "bf16", quant)
     ref, bound, _ = R.attention_ref(t, page)
-    for opts in ({}, {"paged_splits": 2, "paged_min_tiles": 2}):
-        got, _ = go(p, t, opts)
-        R.check(got["O"], ref, bound, "missing pages")
+    for rows in (0, 64):
+        for opts in ({}, {"paged_splits": 2, "paged_min_tiles": 2}):
+            got, _ = go(p, t, {**opts, "paged_rows": rows})
+            R.check(got["O"], ref, bound, "missing pages")
     t["table"].fill_(-1)
-    got, _ = go(p, t)
-    assert not got["O"][:, :3].any()
+    for rows in (0, 64):
+        got, _ = go(p, t, {"paged_rows": rows})
+        assert not got["O"][:, :3].any()
 
 
 @pytest.mark.parametrize("dtype,quant", [("bf16", False), ("f16", False), ("bf16", True), ("f16", True)])
@@ -104,12 +108,28 @@ def test_cache_write(case, dtype, quant):
     t["K"][0, 0, 0] = 0.0
     t["V"][0, 0, 0, 3] = float("inf")
     t["V"][-1, -1, -1, 5] = float("nan")
-    t["K"][-1, 0, 0] = torch.arange(d).to(t["K"].dtype) / 2
+    awkward_rows(t, d)
     p = irgen.cache_write_ir(B, C, hk, d, pages, page, mp, dtype, quant)
-    got, _ = go(p, t)
     want = R.write_ref(t, page, quant)
-    for n in want:
-        same(got[n], want[n], n)
+    for opts, kind in (({}, "cache_write"), ({"patterns": False}, "generic")):
+        got, kinds = go(p, t, opts)
+        assert kinds == [kind]
+        for n in want:
+            same(got[n], want[n], f"{n} {kind}")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_cache_write_many_quotients(dtype):
+    # a million rows' worth of quotients, many of them next to a half
+    t, pages = R.make("write", 4, 8, 128, 64, 8, [512] * 4, [512] * 4, chunk=512, dtype=dtype, quant=True, seed=21)
+    p = irgen.cache_write_ir(4, 512, 8, 128, pages, 64, 8, dtype, True)
+    got, _ = go(p, t)
+    for x in "KV":
+        by, s = R.quantise(t[x])
+        pg = t["table"].long().repeat_interleave(64, 1)
+        row = (torch.arange(512) % 64).expand(4, 512)
+        same(got[x + "C"][pg, :, row], by, x)
+        same(got[x + "S"][pg, :, row], s, x)
 
 
 @pytest.mark.parametrize("dtype,quant", [("bf16", False), ("bf16", True), ("f16", True)])
@@ -119,10 +139,12 @@ def test_cache_read(case, dtype, quant):
     t, pages = R.make("read", B, hk, d, page, mp, lens, [0] * B, length=L, dtype=dtype, quant=quant, seed=L)
     broken_table(t, pages)
     p = irgen.cache_read_ir(B, L, hk, d, pages, page, mp, dtype, quant)
-    got, _ = go(p, t)
     want = R.read_ref(t, page, dtype)
-    for n in want:
-        same(got[n], want[n], n)
+    for opts, kind in (({}, "cache_read"), ({"patterns": False}, "generic")):
+        got, kinds = go(p, t, opts)
+        assert kinds == [kind]
+        for n in want:
+            same(got[n], want[n], f"{n} {kind}")
 
 
 @pytest.mark.parametrize("quant", [False, True])

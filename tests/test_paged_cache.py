@@ -1,21 +1,23 @@
 """The paged key/value cache operators on the CPU: the IR's meaning (oracle), the emitted CUDA-core kernels and the
 tensor-core form (emulators) against plain float64, with ragged batches, padding, stale rows of NaN, missing
 pages, empty sequences and windows; and what the builders refuse."""
+import ctypes
 import json
 import math
 
 import pytest
 import torch
 
-from emmy_ptx_b200 import irgen
+from emmy_ptx_b200 import irgen, launcher
 from emmy_ptx_b200.codegen.generic import Unsupported
 from emmy_ptx_b200.compiler import compile_graph
 from emmy_ptx_b200.data import from_numpy_storage, to_numpy_storage
 from emmy_ptx_b200.ir import Graph
+from emmy_ptx_b200.launcher import EmmyError
+from emmy_ptx_b200.runtime import Executable
 from oracle.interp import Interpreter
 from tests import pagedemu as PE
 from tests import pagedref as R
-from tests.ptxemu import Emulator, Memory
 
 
 def by_oracle(p, t):
@@ -25,20 +27,18 @@ def by_oracle(p, t):
     return {a.name: from_numpy_storage(bufs[a.name], a.dtype).reshape(a.shape) for a in p.outputs}
 
 
-def by_emulator(p, t, opts=None):
-    """The outputs of the emitted CUDA-core PTX, run instruction by instruction."""
-    mod = compile_graph(Graph.from_dict(p.graph), p.meta(), opts or {})
-    mem = Memory()
-    addr = {a.name: mem.alloc(to_numpy_storage(t[a.name])) for a in p.args}
-    for rec in mod.kernels:
-        emu = Emulator(mod.ptx, rec["entry"])
-        emu.run(rec["grid"][0], rec["block"][0], dict(zip(emu.params, [addr[n] for n in rec["params"]])), mem,
-                rec["dyn_smem"])
-    out = {}
-    for a in p.outputs:
-        host = to_numpy_storage(t[a.name])
-        out[a.name] = from_numpy_storage(mem.array(addr[a.name], host.dtype, (-1,)).copy(), a.dtype).reshape(a.shape)
-    return out
+def by_emitter(p, t):
+    """The outputs of the statement-at-a-time CUDA-core PTX, run instruction by instruction."""
+    got, code, mod = PE.run(p, t, {"patterns": False})
+    assert code == 0 and [r["kind"] for r in mod.kernels] == ["generic"]
+    return got
+
+
+def by_kernel(p, t):
+    """The outputs of the hand-written kernel the nest is lowered to."""
+    got, code, mod = PE.run(p, t)
+    assert code == 0 and [r["kind"] for r in mod.kernels] == [p.entry]
+    return got
 
 
 def same(got, want, what):
@@ -57,6 +57,17 @@ def broken_table(t, pages):
         t["table"][0, 1] = 2 ** 31 - 1
 
 
+def awkward_rows(t, d):
+    """Rows for the byte rounding: a scale of exactly 1 with quotients at halves (to even) and their neighbours, a row
+    of the type's smallest numbers (the scale's own steps are coarse or it is 0), one of its largest."""
+    x = (torch.arange(d) % 64 + 0.5) * (1 - 2 * (torch.arange(d) % 2))
+    x[0] = 127.0
+    t["K"][-1, 0, 0] = x.to(t["K"].dtype)
+    tiny, big = torch.finfo(t["K"].dtype).smallest_normal, torch.finfo(t["K"].dtype).max
+    t["V"][-1, 0, 0] = (x * (tiny / 100)).to(t["V"].dtype)
+    t["V"][0, -1, -1] = (x / 127 * big).to(t["V"].dtype)
+
+
 WRITES = [
     # batch, chunk, kv_heads, dim, page, max_pages, lens, fresh
     (3, 4, 2, 64, 8, 3, [4, 9, 24], [4, 2, 0]),
@@ -66,7 +77,7 @@ WRITES = [
 ]
 
 
-@pytest.mark.parametrize("run", [by_oracle, by_emulator])
+@pytest.mark.parametrize("run", [by_oracle, by_emitter, by_kernel])
 @pytest.mark.parametrize("dtype,quant", [("bf16", False), ("f16", False), ("bf16", True), ("f16", True)])
 @pytest.mark.parametrize("case", WRITES, ids=lambda c: "x".join(map(str, c[:6])))
 def test_cache_write(case, dtype, quant, run):
@@ -76,7 +87,7 @@ def test_cache_write(case, dtype, quant, run):
     t["K"][0, 0, 0] = 0.0                                # a row of zeros
     t["V"][0, 0, 0, 3] = math.inf                        # a row with an infinity, one with a NaN
     t["V"][-1, -1, -1, 5] = math.nan
-    t["K"][-1, 0, 0] = torch.arange(d).to(t["K"].dtype) / 2      # exact halves: 127/2, rounding to even
+    awkward_rows(t, d)
     p = irgen.cache_write_ir(B, C, hk, d, pages, page, mp, dtype, quant)
     got = run(p, t)
     want = R.write_ref(t, page, quant)
@@ -87,7 +98,7 @@ def test_cache_write(case, dtype, quant, run):
 READS = [(3, 20, 2, 64, 8, 3, [0, 9, 24]), (2, 33, 1, 128, 16, 2, [1, 40]), (1, 7, 3, 32, 3, 2, [-4])]
 
 
-@pytest.mark.parametrize("run", [by_oracle, by_emulator])
+@pytest.mark.parametrize("run", [by_oracle, by_emitter, by_kernel])
 @pytest.mark.parametrize("dtype,quant", [("bf16", False), ("bf16", True), ("f16", True)])
 @pytest.mark.parametrize("case", READS, ids=lambda c: "x".join(map(str, c[:6])))
 def test_cache_read(case, dtype, quant, run):
@@ -110,7 +121,7 @@ ATTENDS = [
 ]
 
 
-@pytest.mark.parametrize("run", [by_oracle, by_emulator])
+@pytest.mark.parametrize("run", [by_oracle, by_emitter])
 @pytest.mark.parametrize("dtype,quant", [("bf16", False), ("f16", True)])
 @pytest.mark.parametrize("case", ATTENDS, ids=lambda c: "x".join(map(str, c[:7])))
 def test_paged_attention_nest(case, dtype, quant, run):
@@ -119,7 +130,7 @@ def test_paged_attention_nest(case, dtype, quant, run):
     if mp == 3:
         broken_table(t, pages)
     p = irgen.paged_attention_ir(B, C, H, hk, d, pages, page, mp, dtype, quant, window, sinks)
-    got = run(p, t) if run is by_oracle else run(p, t, {"patterns": False})
+    got = run(p, t)
     ref, bound, _ = R.attention_ref(t, page, window, sinks)
     R.check(got["O"], ref, bound, run.__name__)
 
@@ -178,26 +189,39 @@ TENSOR = [
     (1, 9, 2, 1, 64, 64, 4, [256], [9], 1, 0, {}),
     (1, 9, 2, 1, 64, 64, 4, [200], [9], 3, 150, {}),                         # more sinks than a tile
     (2, 6, 2, 1, 64, 16, 2, [4, 40], [6, 6], None, 0, {}),                   # positions below 0, past the table
+    (2, 5, 7, 1, 128, 8, 20, [77, 160], [5, 3], 40, 3, {"paged_splits": 2, "paged_min_tiles": 1}),   # 35 rows
+    (1, 8, 8, 1, 64, 16, 9, [131], [8], None, 0, {}),                         # 64 rows
 ]
+FORMS = {"rows": "paged_attention_rows", "tiles": "tcgen05_paged_attention"}
+
+
+def form_opts(form, case):
+    """The options that make a case take one form, or None when it cannot."""
+    if form == "rows" and case[1] * (case[2] // case[3]) > 64:
+        return None
+    return {**case[-1], "paged_rows": 64 if form == "rows" else 0}
 
 
 @pytest.mark.parametrize("dtype,quant", [("bf16", False), ("f16", False), ("bf16", True), ("f16", True)])
-@pytest.mark.parametrize("case", TENSOR, ids=lambda c: "x".join(map(str, c[:7])))
-def test_paged_attention_tensor_cores_emulated(case, dtype, quant):
-    B, C, H, hk, d, page, mp, lens, fresh, window, sinks, opts = case
+@pytest.mark.parametrize("form,case", [(f, c) for f in FORMS for c in TENSOR if form_opts(f, c)],
+                         ids=lambda c: c if isinstance(c, str) else "x".join(map(str, c[:7])))
+def test_paged_attention_tensor_cores_emulated(form, case, dtype, quant):
+    B, C, H, hk, d, page, mp, lens, fresh, window, sinks, _ = case
+    opts = form_opts(form, case)
     t, pages = R.make("attend", B, hk, d, page, mp, lens, fresh, chunk=C, heads=H, dtype=dtype, quant=quant, seed=H + C)
     p = irgen.paged_attention_ir(B, C, H, hk, d, pages, page, mp, dtype, quant, window, sinks)
     got, code, mod = PE.run(p, t, opts)
     assert code == 0
     kinds = [k["kind"] for k in mod.kernels]
-    assert kinds == ["tcgen05_paged_attention"] + ["paged_attention_join"] * (opts.get("paged_splits", 1) > 1)
+    assert kinds == [FORMS[form]] + ["paged_attention_join"] * (opts.get("paged_splits", 1) > 1)
     ref, bound, _ = R.attention_ref(t, page, window, sinks)
-    R.check(got["O"], ref, bound, "tensor cores")
+    R.check(got["O"], ref, bound, form)
 
 
+@pytest.mark.parametrize("rows", [0, 64])
 @pytest.mark.parametrize("quant", [False, True])
 @pytest.mark.parametrize("page", [8, 64])
-def test_paged_attention_late_completions_and_missing_pages(page, quant):
+def test_paged_attention_late_completions_and_missing_pages(page, quant, rows):
     # asynchronous work completes as late as the barriers allow; table entries name no page
     mp = 320 // page
     t, pages = R.make("attend", 2, 1, 64, page, mp, [320, 250], [3, 3], chunk=3, heads=2, quant=quant, seed=page)
@@ -205,34 +229,51 @@ def test_paged_attention_late_completions_and_missing_pages(page, quant):
     t["table"][0, mp - 2] = pages
     t["table"][1, 0] = 2 ** 31 - 1
     p = irgen.paged_attention_ir(2, 3, 2, 1, 64, pages, page, mp, "bf16", quant)
-    got, code, _ = PE.run(p, t, {"paged_splits": 2, "paged_min_tiles": 2}, defer=True)
+    got, code, _ = PE.run(p, t, {"paged_splits": 2, "paged_min_tiles": 2, "paged_rows": rows}, defer=True)
     assert code == 0
     ref, bound, _ = R.attention_ref(t, page)
     R.check(got["O"], ref, bound, "late completions")
 
 
+@pytest.mark.parametrize("missing", range(0, 17, 2))
+def test_paged_attention_a_missing_page_masks_no_other(missing):
+    # the masks of a ring stage that held a missing page must be gone when the next block comes to it
+    t, pages = R.make("attend", 1, 1, 64, 16, 17, [271], [9], chunk=9, heads=2, quant=bool(missing % 4), seed=missing)
+    t["table"][0, missing] = -1
+    p = irgen.paged_attention_ir(1, 9, 2, 1, 64, pages, 16, 17, "bf16", bool(missing % 4))
+    ref, bound, _ = R.attention_ref(t, 16)
+    for rows in (0, 64):
+        got, code, _ = PE.run(p, t, {"paged_rows": rows})
+        assert code == 0
+        R.check(got["O"], ref, bound, f"rows {rows}")
+
+
+@pytest.mark.parametrize("rows", [0, 64])
 @pytest.mark.parametrize("quant", [False, True])
-def test_paged_attention_all_pages_missing_is_zero(quant):
+def test_paged_attention_all_pages_missing_is_zero(quant, rows):
     t, pages = R.make("attend", 1, 1, 64, 16, 8, [100], [2], chunk=2, heads=2, quant=quant)
     t["table"].fill_(-1)
     p = irgen.paged_attention_ir(1, 2, 2, 1, 64, pages, 16, 8, "bf16", quant)
     for opts in ({}, {"paged_splits": 2, "paged_min_tiles": 1}):
-        got, code, _ = PE.run(p, t, opts)
+        got, code, _ = PE.run(p, t, {**opts, "paged_rows": rows})
         assert code == 0 and not got["O"].any()
 
 
 def test_paged_attention_lowering_rule():
-    """What the tensor cores take: head dim 64 or 128, a group of at most 128 heads, pages of 8, 16, 32 rows or whole
-    tiles; a changed nest stays on the CUDA cores."""
+    """What the tensor cores take: head dim 64 or 128; pages of whole 8-row pieces for at most 64 rows a unit, and
+    above that a group of at most 128 heads and pages that tile 64 keys; a changed nest stays on the CUDA
+    cores."""
     def kind(change=None, **kw):
         base = dict(batch=1, chunk=1, heads=2, kv_heads=1, dim=64, pages=4, page=16, max_pages=2)
         p = irgen.paged_attention_ir(**{**base, **kw})
         if change:
             change(p.graph["nodes"]["paged_attention"])
         return compile_graph(Graph.from_dict(p.graph), p.meta()).kernels[0]["kind"]
-    assert kind() == "tcgen05_paged_attention"
-    assert kind(dim=128, page=192, window=3, sinks=1, scale=0.25) == "tcgen05_paged_attention"
-    for kw in (dict(dim=32), dict(dim=256), dict(page=4), dict(page=24), dict(page=96), dict(heads=129)):
+    assert kind() == kind(page=24) == kind(heads=64) == kind(chunk=32) == "paged_attention_rows"
+    assert kind(heads=65) == kind(chunk=33) == "tcgen05_paged_attention"
+    assert kind(chunk=40, dim=128, page=192, window=3, sinks=1, scale=0.25) == "tcgen05_paged_attention"
+    for kw in (dict(dim=32), dict(dim=256), dict(page=4), dict(page=12), dict(heads=129), dict(chunk=40, page=24),
+               dict(chunk=40, page=96)):
         assert kind(**kw) == "generic", kw
 
     def swap(node):                                        # K and V exchanged in the nest
@@ -245,3 +286,110 @@ def test_paged_attention_lowering_rule():
         i = s.index('"minimum"')
         node["op_fields"] = json.loads(s[:i] + s[i:].replace('"right": 1', '"right": 2', 1))
     assert kind(late) == "generic"
+
+
+# ---- the runtime's side, through a device that only records ----------------------------------------------
+
+
+class PlanDevice:
+    """Stands in for :class:`launcher.Device`: keeps the plans it is given and the parameters they are launched
+    with."""
+
+    def __init__(self):
+        self.plans, self.log = [], []
+
+    def load_ptx(self, ptx):
+        return "module"
+
+    def function(self, mod, entry):
+        return entry
+
+    def set_max_dyn_smem(self, fn, nbytes):
+        pass
+
+    def plan(self, fn, grid, block, dyn_smem, align, cluster=(1, 1, 1), pdl=False, tmaps=(), tail=None):
+        self.plans.append(dict(fn=fn, grid=grid, align=align, pdl=pdl, tmaps=tmaps, tail=tail))
+        return len(self.plans) - 1
+
+    def launch_plan(self, plan, params, stream):
+        for a, x in zip(self.plans[plan]["align"], params):
+            if x % a:
+                raise EmmyError(10003, "emmy_plan_launch", "aligned")
+        self.log.append((self.plans[plan]["fn"], list(params), stream))
+
+    def destroy_plan(self, plan):
+        self.log.append(("destroyed", plan))
+
+    def unload(self, mod):
+        pass
+
+
+class HostExecutable(Executable):
+    def _device_tensor(self, shape, dtype):
+        return torch.empty(shape, dtype=dtype)
+
+
+@pytest.fixture
+def exe(monkeypatch):
+    dev = PlanDevice()
+    monkeypatch.setattr(launcher.Device, "get", classmethod(lambda cls, index=0: dev))
+    t, pages = R.make("attend", 2, 1, 64, 16, 8, [100, 20], [40, 3], chunk=40, heads=4)
+    p = irgen.paged_attention_ir(2, 40, 4, 1, 64, pages, 16, 8)
+    ex = HostExecutable(compile_graph(Graph.from_dict(p.graph), p.meta()), device=0)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)          # CPU tensors pass for cuda:0's
+    return ex, t, dev
+
+
+def test_a_plan_gets_pointers_maps_and_the_status_word(exe):
+    ex, t, dev = exe
+    ex.run(t, 55)
+    (fn, params, stream), = dev.log
+    rec = ex.records[0]
+    assert (fn, stream) == ("paged_attention", 55) and rec["kind"] == "tcgen05_paged_attention"
+    assert params == [t[n].data_ptr() for n in rec["params"]]
+    plan, = dev.plans
+    assert [m[0] for m in plan["tmaps"]] == [rec["params"].index(n) for n in ("KC", "VC")]
+    assert plan["tail"] == ex.err.data_ptr()
+    ex.close()
+    assert dev.log[-1] == ("destroyed", 0)
+
+
+@pytest.mark.parametrize("name,make", [
+    ("Q", lambda t: t["Q"].float()), ("Q", lambda t: t["Q"][:, :39]), ("KC", lambda t: t["KC"].transpose(1, 2)),
+    ("lens", lambda t: t["lens"].long()), ("table", lambda t: t["table"].repeat(1, 2)[:, ::2]),
+    ("O", lambda t: t["O"].transpose(0, 1)), ("fresh", lambda t: None),
+    ("O", lambda t: torch.empty(t["O"].numel() + 1, dtype=t["O"].dtype)[1:].view(t["O"].shape)),
+], ids=["type", "shape", "order", "index-type", "strides", "transposed", "missing", "alignment"])
+def test_tensors_of_another_kind_are_refused_before_a_launch(exe, name, make):
+    ex, t, dev = exe
+    with pytest.raises(ValueError, match=repr(name)):
+        ex.run({**t, name: make(t)}, 55)
+    assert dev.log == []
+
+
+def test_tensors_of_another_device_are_refused(exe, monkeypatch):
+    ex, t, dev = exe
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: -1)
+    with pytest.raises(ValueError, match="cuda:0"):
+        ex.run(t, 55)
+    assert dev.log == []
+
+
+def test_plan_arguments_are_checked_before_the_driver():
+    lib = launcher.load_library()
+    u3 = (ctypes.c_uint32 * 3)(1, 1, 1)
+    al = (ctypes.c_uint32 * 17)(*[16] * 17)
+    fn, h = ctypes.c_void_p(0x1000), ctypes.c_void_p()
+    assert lib.emmy_plan_create(None, u3, u3, None, 0, 0, al, 1, ctypes.byref(h)) != 0
+    assert lib.emmy_plan_create(fn, u3, u3, None, 0, 0x80, al, 1, ctypes.byref(h)) != 0
+    assert lib.emmy_plan_create(fn, u3, u3, None, 0, 0, al, 17, ctypes.byref(h)) != 0 and "16" in launcher.last_error()
+    assert lib.emmy_plan_create(fn, u3, u3, None, 0, 0, al, 2, ctypes.byref(h)) == 0
+    d = (ctypes.c_uint64 * 2)(64, 64)
+    b = (ctypes.c_uint32 * 2)(64, 8)
+    assert lib.emmy_plan_add_tmap(h, 2, 9, 2, d, d, b, 3, 2) != 0            # a parameter the plan does not have
+    assert lib.emmy_plan_add_tmap(h, 0, 9, 6, d, d, b, 3, 2) != 0
+    assert lib.emmy_plan_launch(h, d, 1, None) != 0 and "2 parameters" in launcher.last_error()
+    bad = (ctypes.c_uint64 * 2)(64, 72)
+    assert lib.emmy_plan_launch(h, bad, 2, None) != 0 and "parameter 1" in launcher.last_error()
+    assert lib.emmy_plan_launch(None, d, 2, None) != 0
+    assert lib.emmy_plan_destroy(h) == 0
