@@ -30,11 +30,13 @@ through TMA, MMA, TMEM and back.
 """
 from __future__ import annotations
 
+import math
+
 from .ptxasm import wait_bar_warp
 from .tc_paged_attention import F16_LIFT, LOG2E, RESCALE, _E, _f32, _unit, join_entry
 
 MAX_ROWS = 64
-BLK = 16                         # keys of a block (the second product's K)
+QUANT_LIFT = 6.0                 # bytes: P's exponent is lifted by one less, since its scale may be twice vref
 ERR_ROWS = 77                    # a block's copy never completed
 
 
@@ -47,24 +49,33 @@ def shape(dim, chunk, heads, kv_heads, quant):
     """(rows, 16-row tiles, warps, ring stages, bytes of a stage) of a CTA."""
     rows = chunk * (heads // kv_heads)
     mt = -(-rows // 16)
-    warps = {1: 4, 2: 4, 3: 6, 4: 8}[mt]
-    stage_bytes = 2 * BLK * dim * (1 if quant else 2)
-    stages = STAGES[stage_bytes]
-    return rows, mt, warps, stages, stage_bytes
+    warps = {1: 4, 2: 4, 3: 3, 4: 4}[mt]
+    stage_bytes = 2 * block_keys(quant) * dim * (1 if quant else 2)
+    return rows, mt, warps, (16384 if quant else 8192) // stage_bytes, stage_bytes
 
 
-# blocks of a warp's ring by the bytes of a block: 64 KiB a CTA of four warps, so that three are on an SM
-STAGES = {8192: 2, 4096: 4, 2048: 6}
+def max_registers(rows, quant) -> int:
+    """Registers a thread: 128 for at most 8 rows of a 16-bit cache, where 16 warps an SM with one 8 KiB block each
+    keep HBM busy (a batch of 48 at 137 us; 139 with 168 registers); 168 where there is more arithmetic (the same
+    batch in bytes: 90 us with two blocks a warp, 94 at 128 registers)."""
+    return 128 if rows <= 8 and not quant else 168
+
+
+def block_keys(quant) -> int:
+    """Keys of a block: 16, the second product's depth; 32 for bytes, which have more work a byte to share."""
+    return 32 if quant else 16
 
 
 MAX_SPREAD_BATCH = 128           # sequences whose lengths each CTA takes prefix sums of
 MIN_TILES = 4                    # a run's least tiles: one for each of four warps
 
 
-def plan_ctas(batch, chunk, kv_heads, page, max_pages, window, sinks, sms=148):
+def plan_ctas(batch, chunk, heads, kv_heads, dim, quant, page, max_pages, window, sinks, sms=148):
     """CTAs to spread the tiles over, or 0 for one CTA a unit: for sequences of at most 8 tiles (a second launch
     would cost more than their keys), for windows when there are units for every SM (all units are alike
-    then) and for batches whose prefix sums would take long (they have many units)."""
+    then) and for batches whose prefix sums would take long (they have many units).  Twice as many as are on the GPU
+    at a time for few rows (a batch of 48 in bytes: 90 us against 92 with one wave); one wave for more rows,
+    whose parts cost more (a draft of 40 rows: 47 us against 55)."""
     longest = -(-max_pages * page // 64)
     units = batch * kv_heads
     if window is not None:
@@ -73,7 +84,9 @@ def plan_ctas(batch, chunk, kv_heads, page, max_pages, window, sinks, sms=148):
             return 0
     if longest <= 8 or batch > MAX_SPREAD_BATCH or units * longest >= 1 << 31:
         return 0
-    return 3 * sms
+    rows, _, warps, _, _ = shape(dim, chunk, heads, kv_heads, quant)
+    resident = 65536 // (max_registers(rows, quant) * 32 * warps)
+    return (2 if rows <= 8 else 1) * resident * sms
 
 
 def _tiles_of(e, at, lens_ptr, fresh_ptr, b, ok, chunk, cap, window, sinks):
@@ -98,12 +111,19 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
     grid = ctas or batch * kv_heads
     few = rows <= 8                          # the tile's upper 8 rows are not there
     half = dtype == "f16"
-    p_f16 = half and not quant
+    p_f16 = half or quant                    # P and V in f16; otherwise bf16, P in two parts
+    q_f16 = half or quant                    # Q and K in f16
     es = 1 if quant else 2
     row_b = D * es                           # a cache row
     cap = max_pages * page
     ksteps, nts = D // 16, D // 8
     nk = row_b // 64                         # 16-byte pieces a lane takes of a K row
+    BLK = block_keys(quant)
+    NT, KB = BLK // 8, BLK // 16             # 8-key tiles of S and 16-key steps of P V in a block
+    bpt = 64 // BLK                          # blocks of a 64-key tile
+    prow = math.gcd(page, BLK)               # rows of a block that lie on one page at least
+    pieces = range(BLK // prow)
+    sc_b = 2 * BLK * 4 if quant else 0       # bytes of a block's scales
     bw = min(row_b, 128)                     # bytes of a box row, and the swizzle's span
     boxes = row_b // bw
     v_ld = 8 if (quant and D == 64) else 16  # bytes of a lane's V pieces
@@ -130,8 +150,12 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
     raw = o("mov.u32", smem_sym)
     sbase = o("and.b32", o("add.u32", raw, 1023), -1024)
     wbase = o("mad.lo.u32", warp, stages * stage_b, sbase)    # this warp's ring
-    scal = o("mad.lo.u32", warp, stages * 128, o("add.u32", sbase, warps * stages * stage_b))     # its keys' scales
-    bars = o("add.u32", o("mad.lo.u32", warp, stages * 8, sbase), warps * stages * (stage_b + 128))
+    scal = o("mad.lo.u32", warp, stages * sc_b, o("add.u32", sbase, warps * stages * stage_b))     # its keys' scales
+    # the rings and scales, or where the warps meet (m, l and O of each, rows padded by 4 banks)
+    RW = 8 if few else 16                                      # rows a warp holds
+    orow = D * 4 + 16
+    area = max(warps * stages * (stage_b + sc_b), warps * RW * (orow + 8))
+    bars = o("add.u32", o("mad.lo.u32", warp, stages * 8, sbase), area)
     # this lane's pieces, from a stage: K rows 8 a + g at k_at[i] + 8 a rows, V rows 8 a + 2 t + j at v_at[j] + 8 a rows,
     # each box BLK rows on; the swizzle exchanges 16-byte pieces by the row's place in its 128 bytes x 8
     if bw == 128:
@@ -148,8 +172,7 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
             x_ = o("mad.lo.u32", o("xor.b32", o("shr.u32", g, 1), t), 16, o("shl.b32", r_, 6))
             v_at.append(o("mad.lo.u32", o("and.b32", g, 1), 8, x_))
     v_off = BLK * row_b                                       # V behind K
-    k_imm = [[(hb * BLK + 8 * a) * bw for hb in range(boxes)] for a in range(2)]
-    assert warps * (8 if few else 16) * (D * 4 + 24) <= warps * stages * (stage_b + 128)      # the warps' meeting fits
+    k_imm = [[(hb * BLK + 8 * a) * bw for hb in range(boxes)] for a in range(NT)]
     err = gptr("p_err")
     tk, tv = [o("cvta.param.u64", o("mov.u64", f"p_tm{x}", cls="rd"), cls="rd") for x in "KV"]
     p_l0 = e.cond("eq.u32", lane, 0)
@@ -161,9 +184,9 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
     e("fence.proxy.async.shared::cta;")
     e.label(l_init)
     e("bar.warp.sync -1;")
-    # a bit for each ring stage: its barrier's phase; it holds a block that needs masks; of those, the lower and the
-    # upper half lie on no page
-    phase, edge, gone0, gone1 = (o("mov.u32", 0) for _ in range(4))
+    # a bit for each ring stage: its barrier's phase; it holds a block that needs masks; a piece of it lies on no page
+    phase, edge = o("mov.u32", 0), o("mov.u32", 0)
+    gone = [o("mov.u32", 0) for _ in pieces]
     failed = o("mov.u32", 0)
     lens_ptr, fresh_ptr = gptr("p_lens"), gptr("p_fresh")
     l_exit, l_seg, l_find = e.L("exit"), e.L("seg"), e.L("find")
@@ -227,8 +250,8 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
         t_ = o("div.u32", r, group)
         return o("add.u32", o("mad.lo.u32", t_, heads, base_row), o("sub.u32", r, o("mul.lo.u32", t_, group)))
 
-    # blocks of 16 keys, without those of the last tile that lie past the end
-    nblk = o("shl.b32", nb, 2)
+    # blocks of keys, without those of the last tile that lie past the end
+    nblk = o("mul.lo.u32", nb, bpt)
 
     def tile_of(j):
         i = o("add.u32", j, i0) if i0 is not None else j
@@ -239,27 +262,26 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
 
     def key_of(n):
         """The first key of the part's block n."""
-        return o("mad.lo.u32", o("and.b32", n, 3), BLK, o("shl.b32", tile_of(o("shr.u32", n, 2)), 6))
+        return o("mad.lo.u32", o("and.b32", n, bpt - 1), BLK, o("shl.b32", tile_of(o("div.u32", n, bpt)), 6))
 
     last0 = key_of(o("sub.u32", nblk, 1))                     # total = 0: no blocks, whatever this gives
     over = o("max.s32", o("sub.s32", o("add.u32", last0, BLK), end), 0)
     p_any = e.cond("ne.u32", nb, 0)
-    e(f"@{p_any} sub.u32 {nblk}, {nblk}, {o('shr.u32', over, 4)};")
+    e(f"@{p_any} sub.u32 {nblk}, {nblk}, {o('div.u32', over, BLK)};")
     e(f"@{e.cond('ne.u32', failed, 0)} mov.u32 {nblk}, 0;")
 
     table = at(gptr("p_table"), wide(b, 4 * max_pages))
     if quant:
         ksp, vsp = gptr("p_KS"), gptr("p_VS")
-    halves = (0,) if page % BLK == 0 else (0, 1)              # 8-row halves of a block that lie on pages of their own
     mtile = o("rem.u32", warp, mt) if mt > 1 else None
     stream = o("div.u32", warp, mt) if mt > 1 else warp
 
     def fetch(n, regs):
-        """The page of each half of block n, or -1 (past the blocks, outside the table or the pool)."""
+        """The page of each piece of block n, or -1 (past the blocks, or outside the table)."""
         ok = e.cond("lt.u32", n, nblk)
         k0 = key_of(n)
-        for h in halves:
-            slot = o("div.u32", o("add.u32", k0, 8 * h) if h else k0, page)
+        for h in pieces:
+            slot = o("div.u32", o("add.u32", k0, prow * h) if h else k0, page)
             okh = e.cond("lt.u32", slot, max_pages)
             e(f"and.pred {okh}, {okh}, {ok};")
             e(f"mov.u32 {regs[h]}, -1;")
@@ -274,7 +296,7 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
         e(f"@{e.cond('ge.u32', n, nblk)} bra {l_no};")
         k0 = key_of(n)
         last = o("add.u32", k0, BLK)
-        okp = [e.cond("lt.u32", regs[h], pages) for h in halves]
+        okp = [e.cond("lt.u32", regs[h], pages) for h in pieces]
         # plain: every row of the unit sees every key of the block
         plain = e.cond("le.s32", last, o("add.s32", pos0, 1))
         p_ = e.cond("le.u32", last, end)
@@ -287,32 +309,31 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
             e(f"and.pred {plain}, {plain}, {p1};")
         e(f"or.b32 {edge}, {edge}, {sbit};")
         e(f"@{plain} sub.u32 {edge}, {edge}, {sbit};")
-        for x, p_ in zip((gone0, gone1), (okp[0], okp[-1])):
+        for x, p_ in zip(gone, okp):
             e(f"or.b32 {x}, {x}, {sbit};")
             e(f"@{p_} sub.u32 {x}, {x}, {sbit};")
         e(f"@!{p_l0} bra {l_no};")
         nbytes = o("mov.u32", stage_b)
         if quant:
             for p_ in okp:
-                e(f"@{p_} add.u32 {nbytes}, {nbytes}, {128 // len(halves)};")
+                e(f"@{p_} add.u32 {nbytes}, {nbytes}, {8 * prow};")
         e(f"mbarrier.arrive.expect_tx.shared::cta.b64 _, [{bar}], {nbytes};")
         dst = o("add.u32", wbase, so)
-        rows_h = BLK // len(halves)
+        rows_at = [o("rem.u32", o("add.u32", k0, prow * h) if h else k0, page) for h in pieces]
         for x, tm in enumerate((tk, tv)):
-            for h in halves:
+            for h in pieces:
                 pgc = o("selp.b32", regs[h], -1, okp[h])       # outside the pool: the box reads zeros
-                ro = o("rem.u32", o("add.u32", k0, 8 * h) if h else k0, page)
+                ro = rows_at[h]
                 for hb in range(boxes):
                     e(f"cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-                      f"[{dst}+{x * v_off + (hb * BLK + 8 * h) * bw}], [{tm}, {{{64 * hb}, {ro}, {kvh}, {pgc}}}], [{bar}];")
+                      f"[{dst}+{x * v_off + (hb * BLK + prow * h) * bw}], [{tm}, {{{64 * hb}, {ro}, {kvh}, {pgc}}}], [{bar}];")
         if quant:
-            sd = o("add.u32", scal, o("mul.lo.u32", o("div.u32", so, stage_b), 128))
-            for h in halves:
-                ro = o("rem.u32", o("add.u32", k0, 8 * h) if h else k0, page)
-                off = o("mad.wide.u32", regs[h], kv_heads * page * 4, wide(o("add.u32", hoff, ro), 4), cls="rd")
+            sd = o("mad.lo.u32", o("div.u32", so, stage_b), sc_b, scal)
+            for h in pieces:
+                off = o("mad.wide.u32", regs[h], kv_heads * page * 4, wide(o("add.u32", hoff, rows_at[h]), 4), cls="rd")
                 for x, ptr in enumerate((ksp, vsp)):
                     e(f"@{okp[h]} cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes "
-                      f"[{sd}+{64 * x + 32 * h}], [{at(ptr, off)}], {4 * rows_h}, [{bar}];")
+                      f"[{sd}+{4 * (BLK * x + prow * h)}], [{at(ptr, off)}], {4 * prow}, [{bar}];")
         e.label(l_no)
 
     # ---- Q: the rows of this warp's tile, in the order the keys' bytes come ------------------
@@ -320,7 +341,7 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
     r0 = o("mad.lo.u32", mtile, 16, g) if mt > 1 else g
     qa = [[None] * 4 for _ in range(ksteps)]
     zero = o("mov.b32", 0)
-    pos = []
+    pos, crow = [], []                                         # positions; scale * log2(e) for the row's scores
     for h in hs:
         r_ = o("add.u32", r0, 8 * h) if h else r0
         okr = e.cond("lt.u32", r_, vrows)
@@ -329,40 +350,54 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
         per_p = 32 if quant else 16
         np_ = nk // boxes                                      # pieces a lane takes of a box row
         src = at(src, wide(t, np_ * per_p))
+        got = []
         for hb in range(boxes):
             for i in range(np_):
-                ws = []
                 for x in range(per_p // 16):
                     d_ = [o("mov.b32", 0) for _ in range(4)]
                     e(f"@{okr} ld.global.nc.v4.b32 {{{', '.join(d_)}}}, [{src}+{hb * 128 + i * per_p + 16 * x}];")
-                    ws += d_
-                for s_ in range(len(ws) // 2):                 # two registers a k-step
-                    ks = (hb * np_ + i) * (len(ws) // 2) + s_
-                    qa[ks][h], qa[ks][2 + h] = ws[2 * s_], ws[2 * s_ + 1]
+                    got += d_
+        if q_f16 and not half:
+            # bf16 to f16: the row times a power of two that brings its largest number to 2^14 (at most 2^40), exact
+            # but for numbers 2^-28 of the largest and less; the scores take the inverse
+            big = None
+            for x in got:
+                a_ = o("and.b32", x, "0x7FFF7FFF")
+                big = a_ if big is None else o("max.u16x2", big, a_)
+            big = o("max.u32", o("and.b32", big, 65535), o("shr.u32", big, 16))
+            for d_ in (1, 2):
+                big = o("max.u32", big, o("shfl.sync.bfly.b32", big, d_, 31, -1))
+            ex = o("sub.s32", 127 + 14, o("shr.u32", big, 7))     # 14 less the largest's exponent
+            ex = o("min.s32", ex, 40)
+            up = o("shl.b32", o("add.s32", ex, 127), 23, cls="f")
+            down = o("shl.b32", o("sub.s32", 127, ex), 23, cls="f")
+            crow.append(o("mul.f32", down, cscale, cls="f"))
+            got = [o("cvt.rn.f16x2.f32", o("mul.f32", o("and.b32", x, -65536, cls="f"), up, cls="f"),
+                     o("mul.f32", o("shl.b32", x, 16, cls="f"), up, cls="f")) for x in got]
+        else:
+            crow.append(cscale)
+        for ks in range(ksteps):                               # two registers a k-step
+            qa[ks][h], qa[ks][2 + h] = got[2 * ks], got[2 * ks + 1]
         tok = o("div.u32", r_, group) if group > 1 else r_
         pos.append(o("min.s32", o("add.s32", pos0, tok), pos1))
     if few:
         for ks in range(ksteps):
             qa[ks][1] = qa[ks][3] = zero
 
-    fz = o("mov.b32", "0f00000000", cls="f")
-    acc = [[o("mov.b32", "0f00000000", cls="f") for _ in range(2 * len(hs))] for _ in range(nts)]
+    # four registers a tile, also where its upper rows are not there: products take them in fours, and sharing the
+    # upper two between tiles cost more moves than it saved registers
+    acc = [[o("mov.b32", "0f00000000", cls="f") for _ in range(4)] for _ in range(nts)]
     m = [o("mov.b32", "0fFF800000", cls="f") for _ in hs]
     l = [o("mov.b32", "0f00000000", cls="f") for _ in hs]
-    dump = [e.r("f"), e.r("f")]
-    ty = "f16.f16" if half else "bf16.bf16"
+    ty = "f16.f16" if q_f16 else "bf16.bf16"
     pty = "f16.f16" if p_f16 else "bf16.bf16"
 
     def mma(tys, d, a_, b_, c):
         e(f"mma.sync.aligned.m16n8k16.row.col.f32.{tys}.f32 {{{', '.join(d)}}}, {{{', '.join(a_)}}}, "
           f"{{{', '.join(b_)}}}, {{{', '.join(c)}}};")
 
-    def both(x):
-        """The four accumulator registers of a tile whose upper rows may not be there."""
-        return (x + dump, x + [fz, fz]) if few else (x, x)
-
     # ---- the ring: ``stages`` blocks ahead --------------------------------------------------
-    pg = [e.r() for _ in range(2)]
+    pg = [e.r() for _ in pieces]
     nn = o("mov.u32", stream)                                  # the next block to copy
     for s_ in range(stages):
         fetch(nn, pg)
@@ -372,16 +407,14 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
     n = o("mov.u32", stream)
     rd, rbit = o("mov.u32", 0), o("mov.u32", 1)                # the stage to read next, and its bit
     l_fail = e.L("fail")
+    lift = 0.0 if not p_f16 else QUANT_LIFT if quant else F16_LIFT
     if quant:
-        c4300, c4380 = o("mov.b32", "0x43004300"), o("mov.b32", "0x43804380")
         c64, c1152 = o("mov.b32", "0x64646464"), o("mov.b32", "0x64806480")
-
-    def widen(t_):
-        """Two bytes in the low bytes of 16-bit lanes (the high ones arbitrary) less 128, exact in bf16."""
-        m_ = o("lop3.b32", t_, "0x007F007F", c4300, "0xEA")
-        c_ = o("lop3.b32", t_, "0x00800080", c4380, "0x6A")
-        return o("sub.rn.bf16x2", m_, c_)
-
+        c6400 = o("mov.b32", "0x64006400")
+        # P carries the values' scales over vref, a power of two at least half the largest scale the warp's rows met:
+        # P is at most 2^15 in f16, and what is 2^-20 of the largest scale's still has 11 bits
+        vref = o("mov.b32", "0f00800000", cls="f")
+        vinv = o("mov.b32", "0f7E800000", cls="f")
     l_top, l_done = e.L("blk"), e.L("blkd")
     e.label(l_top)
     e(f"@{e.cond('ge.u32', n, nblk)} bra {l_done};")
@@ -390,41 +423,41 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
     wait_bar_warp(e, bar, par, err, ERR_ROWS, l_fail)
     e(f"xor.b32 {phase}, {phase}, {rbit};")
     so = o("add.u32", wbase, o("mul.lo.u32", rd, stage_b))
-    sc = o("add.u32", scal, o("mad.lo.u32", rd, 128, o("shl.b32", t, 3)))
+    if quant:
+        sc = o("add.u32", o("mad.lo.u32", rd, sc_b, scal), o("shl.b32", t, 3))
     ka = [o("add.u32", so, x) for x in k_at]
     va = [o("add.u32", so, x) for x in v_at]
-    # S = Q K^T of 16 keys: two n-tiles of 8
-    sv = []
-    for a in range(2):
+    # S = Q K^T, 8 keys a tile
+    sv, ys = [], []
+    for a in range(NT):
         bs = []
         for i in range(nk):
             d_ = [e.r() for _ in range(4)]
             e(f"ld.shared.v4.b32 {{{', '.join(d_)}}}, [{ka[i % len(ka)]}+{k_imm[a][i // len(ka)]}];")
             if not quant:
                 bs += [(d_[0], d_[1]), (d_[2], d_[3])]
-            else:
-                for x in d_:
-                    if half:
-                        bs.append(tuple(o("sub.rn.f16x2", o("prmt.b32", x, c64, sel), c1152) for sel in ("0x4140", "0x4342")))
-                    else:
-                        bs.append(tuple(widen(o("prmt.b32", x, zero, sel)) for sel in ("0x4140", "0x4342")))
-        cur = [o("mov.b32", "0f00000000", cls="f") for _ in range(2 * len(hs))]
+            else:                                              # 1024 + b less 1152
+                bs += [tuple(o("sub.rn.f16x2", o("prmt.b32", x, c64, sel), c1152) for sel in ("0x4140", "0x4342"))
+                       for x in d_]
+        cur = [o("mov.b32", "0f00000000", cls="f") for _ in range(4)]
         for ks in range(ksteps):
-            dd, cc = both(cur)
-            mma(ty, dd, qa[ks], bs[ks], cc)
+            mma(ty, cur, qa[ks], bs[ks], cur)
         if quant:
-            f_ = [e.r("f"), e.r("f")]
+            f_, y_ = [e.r("f"), e.r("f")], [e.r("f"), e.r("f")]
             e(f"ld.shared.v2.f32 {{{f_[0]}, {f_[1]}}}, [{sc}+{32 * a}];")
-            for x in range(len(cur)):
+            e(f"ld.shared.v2.f32 {{{y_[0]}, {y_[1]}}}, [{sc}+{4 * BLK + 32 * a}];")
+            for x in range(2 * len(hs)):
                 e(f"mul.f32 {cur[x]}, {cur[x]}, {f_[x & 1]};")
+            ys.append(y_)
         sv.append(cur)
     # which keys each row sees; blocks that every row sees whole skip this
     l_seen = e.L("seen")
     live = [e.cond("eq.u32", lane, lane) for _ in range(4)]
-    sees = {(a, j, h): e.cond("eq.u32", lane, lane) for a in range(2) for j in range(2) for h in hs}
-    e(f"@{e.cond('eq.u32', o('and.b32', edge, rbit), 0)} bra {l_seen};")
+    sees = {(a, j, h): e.cond("eq.u32", lane, lane) for a in range(NT) for j in range(2) for h in hs}
+    whole = e.cond("eq.u32", o("and.b32", edge, rbit), 0)
+    e(f"@{whole} bra {l_seen};")
     key0 = key_of(n)
-    pk = [e.cond("eq.u32", o("and.b32", x, rbit), 0) for x in (gone0, gone1)]
+    pk = [e.cond("eq.u32", o("and.b32", x, rbit), 0) for x in gone]
     if not quant:
         for r_ in range(4):
             key = o("add.u32", o("add.u32", key0, 8 * (r_ // 2) + r_ % 2), tt2)
@@ -433,34 +466,56 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
                 p1, p2 = e.cond("ge.u32", key, w["lo"]), e.cond("lt.u32", key, sinks)
                 e(f"or.pred {p1}, {p1}, {p2};")
                 e(f"and.pred {live[r_]}, {live[r_]}, {p1};")
-    for a in range(2):
+    for a in range(NT):
         for j in range(2):
             key = o("add.u32", o("add.u32", key0, 8 * a + j), tt2)
+            any_ = None
             for h in hs:
                 ps = sees[a, j, h]
                 e(f"setp.le.s32 {ps}, {key}, {pos[h]};")
-                e(f"and.pred {ps}, {ps}, {pk[a]};")
+                e(f"and.pred {ps}, {ps}, {pk[8 * a // prow]};")
                 if window is not None:
                     p1 = e.cond("gt.s32", o("add.s32", key, window), pos[h])
                     p2 = e.cond("lt.s32", key, sinks)
                     e(f"or.pred {p1}, {p1}, {p2};")
                     e(f"and.pred {ps}, {ps}, {p1};")
                 e(f"@!{ps} mov.b32 {sv[a][2 * h + j]}, 0fFF800000;")
+                if quant and any_ is None:
+                    any_ = o("selp.u32", 1, 0, ps)
+                elif quant:
+                    e(f"@{ps} mov.u32 {any_}, 1;")
+            if quant:                                          # scales of keys that this lane's rows do not see
+                e(f"@{e.cond('eq.u32', any_, 0)} mov.b32 {ys[a][j]}, 0f00000000;")
     e.label(l_seen)
-    # raise the rows' references where a score passed them by 2^8
+    # raise the rows' references where a score passed them by 2^8, and vref where a scale reached twice it
     mx, need = [], None
     for h in hs:
-        x = o("max.f32", sv[0][2 * h], sv[0][2 * h + 1], cls="f")
-        y = o("max.f32", sv[1][2 * h], sv[1][2 * h + 1], cls="f")
-        mx.append(o("mul.f32", o("max.f32", x, y, cls="f"), cscale, cls="f"))
+        x = None
+        for a in range(NT):
+            y = o("max.f32", sv[a][2 * h], sv[a][2 * h + 1], cls="f")
+            x = y if x is None else o("max.f32", x, y, cls="f")
+        mx.append(o("mul.f32", x, crow[h], cls="f"))
         p_ = e.cond("gt.f32", mx[h], o("add.f32", m[h], _f32(RESCALE), cls="f"))
         if need is None:
             need = p_
         else:
             e(f"or.pred {need}, {need}, {p_};")
+    if quant:
+        ymax = o("mov.b32", "0f00000000", cls="f")
+        for a in range(NT):
+            e(f"max.f32 {ymax}, {ymax}, {o('max.f32', ys[a][0], ys[a][1], cls='f')};")    # a NaN drops out
+        p_ = e.cond("ge.f32", o("mul.f32", ymax, vinv, cls="f"), "0f40000000")
+        e(f"or.pred {need}, {need}, {p_};")
     anyneed = o("vote.sync.any.pred", need, -1, cls="p")
     l_keep = e.L("keep")
     e(f"@!{anyneed} bra {l_keep};")
+    if quant:
+        yb = o("redux.sync.max.u32", o("mov.b32", ymax), -1)
+        yb = o("min.u32", o("and.b32", yb, "0x7F800000"), "0x7E000000")
+        yb = o("max.u32", yb, o("mov.b32", vref))
+        e(f"mov.b32 {vinv}, {o('sub.u32', '0x7F000000', yb)};")                     # a power of two's inverse
+        vscale = o("mul.f32", vref, vinv, cls="f")
+        e(f"mov.b32 {vref}, {yb};")
     for h in hs:
         for d_ in (1, 2):
             e(f"max.f32 {mx[h]}, {mx[h]}, {o('shfl.sync.bfly.b32', mx[h], d_, 31, -1, cls='f')};")
@@ -469,73 +524,83 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
         e(f"@{e.cond('eq.f32', mn, '0fFF800000')} mov.b32 {al}, 0f3F800000;")   # nothing seen yet
         e(f"mov.b32 {m[h]}, {mn};")
         e(f"mul.f32 {l[h]}, {l[h]}, {al};")
+        if quant:
+            al = o("mul.f32", al, vscale, cls="f")
         for nt in range(nts):
             for j in range(2):
                 e(f"mul.f32 {acc[nt][2 * h + j]}, {acc[nt][2 * h + j]}, {al};")
     e.label(l_keep)
-    lift = F16_LIFT if p_f16 else 0.0
     for h in hs:
         neg = o("sub.f32", o("mov.b32", _f32(lift), cls="f"), m[h], cls="f")
         e(f"@{e.cond('eq.f32', m[h], '0fFF800000')} mov.b32 {neg}, 0f00000000;")
-        for a in range(2):
+        part_sum = []
+        for a in range(NT):
             for j in range(2):
                 x = sv[a][2 * h + j]
-                e(f"fma.rn.f32 {x}, {x}, {cscale}, {neg};")
+                e(f"fma.rn.f32 {x}, {x}, {crow[h]}, {neg};")
                 e(f"ex2.approx.ftz.f32 {x}, {x};")
-        s0 = o("add.f32", sv[0][2 * h], sv[0][2 * h + 1], cls="f")
-        s1 = o("add.f32", sv[1][2 * h], sv[1][2 * h + 1], cls="f")
-        e(f"add.f32 {l[h]}, {l[h]}, {o('add.f32', s0, s1, cls='f')};")
+            part_sum.append(o("add.f32", sv[a][2 * h], sv[a][2 * h + 1], cls="f"))
+        while len(part_sum) > 1:
+            part_sum = [o("add.f32", part_sum[i], part_sum[i + 1], cls="f") for i in range(0, len(part_sum), 2)]
+        e(f"add.f32 {l[h]}, {l[h]}, {part_sum[0]};")
     if quant:
+        for a in range(NT):
+            for j in range(2):
+                e(f"mul.f32 {ys[a][j]}, {ys[a][j]}, {vinv};")
+                for h in hs:
+                    e(f"mul.f32 {sv[a][2 * h + j]}, {sv[a][2 * h + j]}, {ys[a][j]};")
+        # a scale that some rows do not see may be NaN: their weights are 0
+        l_ok = e.L("whole")
+        e(f"@{whole} bra {l_ok};")
+        for (a, j, h), ps in sees.items():
+            e(f"@!{ps} mov.b32 {sv[a][2 * h + j]}, 0f00000000;")
+        e.label(l_ok)
+    for kb in range(KB):
+        # P as the second product's A: rows g (and g + 8), keys 2t, 2t+1 and 8 further
+        pa = [[None] * 4 for _ in range(1 if p_f16 else 2)]
         for a in range(2):
-            f_ = [e.r("f"), e.r("f")]
-            e(f"ld.shared.v2.f32 {{{f_[0]}, {f_[1]}}}, [{sc}+{64 + 32 * a}];")
-            for h in hs:
-                for j in range(2):
-                    x = sv[a][2 * h + j]
-                    # (a masked key's scale may be NaN)
-                    e(f"selp.f32 {x}, {o('mul.f32', x, f_[j], cls='f')}, 0f00000000, {sees[a, j, h]};")
-    # P as the second product's A: rows g (and g + 8), keys 2t, 2t+1 and 8 further
-    pa = [[None] * 4 for _ in range(1 if p_f16 else 2)]
-    for a in range(2):
-        for h in (0, 1):
-            if h not in hs:
+            for h in (0, 1):
+                if h not in hs:
+                    for part in pa:
+                        part[2 * a + h] = zero
+                    continue
+                x0, x1 = sv[2 * kb + a][2 * h], sv[2 * kb + a][2 * h + 1]
+                if p_f16:
+                    pa[0][2 * a + h] = o("cvt.rn.f16x2.f32", x1, x0)
+                else:
+                    pa[0][2 * a + h] = o("prmt.b32", x0, x1, "0x7632")
+                    d0 = o("sub.f32", x0, o("and.b32", x0, -65536, cls="f"), cls="f")
+                    d1 = o("sub.f32", x1, o("and.b32", x1, -65536, cls="f"), cls="f")
+                    pa[1][2 * a + h] = o("prmt.b32", d0, d1, "0x7632")
+        for i in range(nv):
+            vr = []
+            for r_ in range(4):                                # rows 2t, 2t+1, 2t+8, 2t+9
+                d_ = [e.r() for _ in range(v_ld // 4)]
+                off = v_off + (i * BLK + 16 * kb + 8 * (r_ // 2)) * bw
+                e(f"ld.shared.v{len(d_)}.b32 {{{', '.join(d_)}}}, [{va[r_ % 2]}+{off}];")
+                vr.append(d_)
+            if not quant:
+                # rows that no row of the unit sees may hold anything: P is 0 there, so they become 0 too
+                l_live = e.L("live")
+                e(f"@{whole} bra {l_live};")
+                for r_ in range(4):
+                    for x in vr[r_]:
+                        e(f"@!{live[r_]} mov.b32 {x}, 0;")
+                e.label(l_live)
+            per_piece = v_ld // es
+            for x in range(per_piece):
+                nt = i * per_piece + x
+                bb = []
+                for k in range(2):
+                    lo_, hi_ = vr[2 * k], vr[2 * k + 1]
+                    if quant:                                  # byte x of both rows, 1024 + b less 1152
+                        t_ = o("prmt.b32", lo_[x // 4], hi_[x // 4], f"0x{4 + x % 4}{4 + x % 4}{x % 4}{x % 4}")
+                        t_ = o("lop3.b32", t_, "0x00FF00FF", c6400, "0xEA")
+                        bb.append(o("sub.rn.f16x2", t_, c1152))
+                    else:
+                        bb.append(o("prmt.b32", lo_[x // 2], hi_[x // 2], "0x7632" if x % 2 else "0x5410"))
                 for part in pa:
-                    part[2 * a + h] = zero
-                continue
-            x0, x1 = sv[a][2 * h], sv[a][2 * h + 1]
-            if p_f16:
-                pa[0][2 * a + h] = o("cvt.rn.f16x2.f32", x1, x0)
-            else:
-                pa[0][2 * a + h] = o("prmt.b32", x0, x1, "0x7632")
-                d0 = o("sub.f32", x0, o("and.b32", x0, -65536, cls="f"), cls="f")
-                d1 = o("sub.f32", x1, o("and.b32", x1, -65536, cls="f"), cls="f")
-                pa[1][2 * a + h] = o("prmt.b32", d0, d1, "0x7632")
-    for i in range(nv):
-        vr = []
-        for r_ in range(4):                                    # rows 2t, 2t+1, 2t+8, 2t+9
-            d_ = [e.r() for _ in range(v_ld // 4)]
-            e(f"ld.shared.v{len(d_)}.b32 {{{', '.join(d_)}}}, [{va[r_ % 2]}+{v_off + (i * BLK + 8 * (r_ // 2)) * bw}];")
-            vr.append(d_)
-        if not quant:
-            # rows that no row of the unit sees may hold anything: P is 0 there, so they become 0 too
-            l_live = e.L("live")
-            e(f"@{e.cond('eq.u32', o('and.b32', edge, rbit), 0)} bra {l_live};")
-            for r_ in range(4):
-                for x in vr[r_]:
-                    e(f"@!{live[r_]} mov.b32 {x}, 0;")
-            e.label(l_live)
-        per_piece = v_ld // es
-        for x in range(per_piece):
-            nt = i * per_piece + x
-            if quant:
-                sel = f"0x{4 + x % 4}{4 + x % 4}{x % 4}{x % 4}"      # byte x of both rows, twice each
-                bb = tuple(widen(o("prmt.b32", vr[2 * k][x // 4], vr[2 * k + 1][x // 4], sel)) for k in range(2))
-            else:
-                sel = "0x7632" if x % 2 else "0x5410"
-                bb = tuple(o("prmt.b32", vr[2 * k][x // 2], vr[2 * k + 1][x // 2], sel) for k in range(2))
-            for part in pa:
-                dd, cc = both(acc[nt])
-                mma(pty, dd, part, bb, cc)
+                    mma(pty, acc[nt], part, bb, acc[nt])
     e("bar.warp.sync -1;")                                     # every lane has read the stage
     copy(nn, pg, rbit, o("mul.lo.u32", rd, stage_b), bar)
     e(f"add.u32 {nn}, {nn}, {streams};")
@@ -559,8 +624,6 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
         for d_ in (1, 2):
             e(f"add.f32 {l[h]}, {l[h]}, {o('shfl.sync.bfly.b32', l[h], d_, 31, -1, cls='f')};")
     e("bar.sync 0;")
-    RW = 8 if few else 16                                      # rows a warp holds
-    orow = D * 4 + 16                                          # a row of O, padded by 4 banks
     obase = o("mad.lo.u32", warp, RW * orow, sbase)
     mlb = o("add.u32", sbase, warps * RW * orow)
 
@@ -575,6 +638,8 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
             for j in range(2):
                 for x0 in range(0, piece, 4):
                     vals = [acc[i * piece + x0 + x][2 * h + j] for x in range(4)]
+                    if quant:
+                        vals = [o("mul.f32", x, vref, cls="f") for x in vals]
                     e(f"st.shared.v4.f32 [{ra}+{(i * span + j * piece + x0) * 4}], {{{', '.join(vals)}}};")
         ma = o("mad.lo.u32", o("mad.lo.u32", warp, RW, rr), 8, mlb)
         e(f"@{p_t0} st.shared.v2.f32 [{ma}], {{{m[h]}, {l[h]}}};")
@@ -664,12 +729,13 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
         sc_spec = [{"name": scratch, "dtype": "f32", "shape": [2 * ctas * rows, D + 2], "per_call": True}]
     plist = [f"\t.param .u64 p_{p}" for p, _, _ in params]
     plist += [f"\t.param .align 64 .b8 p_tm{x}[128]" for x in "KV"] + ["\t.param .u64 p_err"]
-    text = [f".visible .entry {name}(", ",\n".join(plist), ")", f".reqntid {threads}, 1, 1", "{"]
+    text = [f".visible .entry {name}(", ",\n".join(plist), ")", f".reqntid {threads}, 1, 1"]
+    text += [f".maxnreg {max_registers(rows, quant)}", "{"]
     text += e.decls() + e.lines + ["\tret;", "}"]
-    dyn = max(warps * stages * (stage_b + 128), warps * RW * (orow + 8)) + warps * stages * 8 + 1024
+    dyn = area + warps * stages * 8 + 1024
     es_name = "u8" if quant else dtype
     tmaps = [{"name": f"tm{x}", "tensor": nm, "dtype": es_name, "dims": [D, page, kv_heads, pages],
-              "strides": [row_b, page * row_b, kv_heads * page * row_b], "box": [bw // es, BLK // len(halves), 1, 1],
+              "strides": [row_b, page * row_b, kv_heads * page * row_b], "box": [bw // es, prow, 1, 1],
               "swizzle": f"{bw}B"} for x, nm in (("K", kn), ("V", vn))]
     return {
         "name": name, "kind": "paged_attention_rows", "params": [n for _, n, _ in params], "raw_entry": text,

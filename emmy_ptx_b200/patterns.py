@@ -533,7 +533,7 @@ def _lower_paged_attention(graph, node, kw, prefix, options):
     scratch = f"{prefix}{name}__part"
     jkw = dict(**geo, dim=kw["dim"], dtype=kw["dtype"], names=names[-3:], scratch=scratch)
     if few:
-        ctas = pr.plan_ctas(**{k: v for k, v in geo.items() if k != "heads"}, sms=sms)
+        ctas = pr.plan_ctas(**geo, dim=kw["dim"], quant=kw["quant"], sms=sms)
         if "paged_splits" in options:
             n = int(options["paged_splits"])
             ctas = n * kw["batch"] * kw["kv_heads"] if n > 1 and kw["batch"] <= pr.MAX_SPREAD_BATCH else 0
