@@ -14,17 +14,19 @@ tiles fit one part writes O itself.  Two CTAs share an SM (half its TMEM columns
 one's loads and softmax run beside the other's products.
 
 **Roles.**  One thread issues the ``tcgen05.mma``: S(j+1) = Q K_(j+1)^T into one of two 64-column score buffers,
-then O += P(j) V_j.  Four softmax warps hold one row a thread; warps without a row take no part, so a decode step
-costs one warp's softmax.  16-bit caches are loaded by TMA, one box per page of the tile (at most 64 rows), with
-the page numbers fetched 32 at a time one batch ahead.  For a cache of bytes four warps load 16 bytes a thread a
-tile ahead, convert and store into the tiles' swizzled layout: a byte b is b - 128, exact in bf16
-(0x4300 | (b & 127) is 128 + (b & 127), less 128 or 256) and in f16 (0x6400 | b is 1024 + b, less 1152), so no
-product is rounded.  The keys' scales multiply the scores' columns, the values' scales multiply P.
+then O += P(j) V_j.  Four softmax warps hold one row a thread; warps without a row take no part.  A warp loads by
+TMA, one box per page of the tile (at most 64 rows), with the page numbers fetched 32 at a time one batch ahead.  For
+a cache of bytes the boxes land in a raw ring, and two warps convert them into the tiles the products read: with
+0x64 as its upper half a byte b is the f16 number 1024 + b, less 1152 it is b - 128, exactly.  Each quarter warp
+takes 64 bytes of rows r and r ^ 5, which the raw ring's swizzle and the tile's put into different banks.  The
+keys' scales multiply the scores' columns, the values' scales multiply P.
 
 **Numerics.**  The score buffers, the running reference and sum, and O are f32.  P is rounded for the tensor core:
 f16 caches take f16 P, to nearest (2^-11), with 2^7 put on the exponent so that small weights keep their bits;
-bf16 caches and bytes (whose P carries a scale of any size) take P as two bf16 parts, truncated, 2^-14 together.
-O is rescaled only when the row's maximum grew by more than 2^8.
+bf16 caches take P as two bf16 parts, truncated, 2^-14 together.  Bytes are multiplied in f16: a bf16 Q row is
+brought to 2^14 by a power of two (exact but for numbers 2^-28 of its largest), and P carries the values' scales over
+a running power of two, at least half the largest scale so far, so that it stays below 2^15 and what is 2^-20 of the
+largest still has 11 bits.  O is rescaled only when the row's maximum grew by more than 2^8, or that power did.
 
 **What is masked.**  Scores past the row's own position, outside its window or of a page that the table does not
 name become -inf; a row that sees nothing ends as 0.  Rows of a V tile that no row of the CTA sees are zeroed in
@@ -49,8 +51,10 @@ F16_LIFT = 7.0                   # f16 P is 2^(s - m + 7): at most 2^15, and 2^-
 ERR_LOAD, ERR_MMA, ERR_SOFTMAX, ERR_EPILOGUE, ERR_DRAIN, ERR_Q = 71, 72, 73, 74, 75, 76
 
 # shared memory behind the tiles: barriers, the TMEM slot, two mask words per tile (a ring of 4 tiles) and, for
-# bytes, the keys' and values' scales of 4 tiles.  A ring of 4 is enough: the loads of tile j + 4 wait for
-# S(j + 2), which is issued after P(j) is complete, so nobody reads slot j any more.
+# bytes, the keys' and values' scales of 4 tiles with the power the latter stand over, Q's row factors and the raw
+# scales.  A ring of 4 is enough: tile j + 4 comes in after tile j + 2 was converted, whose V waits for the product
+# of tile j + 1, so nobody reads slot j any more.  Bytes use the ring barriers 0 and 1 for the raw stages, 2 for the
+# converted K and 3 for the converted V.
 QFULL = 0
 FULL = 8
 EMPTY = FULL + 8 * STAGES
@@ -61,7 +65,11 @@ SLOT = PFREE + 16
 KMASK = 192
 KSC = 256
 VSC = KSC + 4 * BKV * 4
-AUX_BYTES = VSC + 4 * BKV * 4
+VREF = 224                       # 4 floats
+QSC = VSC + 4 * BKV * 4
+RAWSC = QSC + 4 * ROWS
+AUX_BYTES = RAWSC + 2 * 2 * BKV * 4
+QUANT_LIFT = 6.0                 # bytes: P may carry up to twice the power its scales stand over
 
 
 def _f32(v: float) -> str:
@@ -143,8 +151,9 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     group, tq, ntile, rows = geometry(chunk, heads, kv_heads)
     units = batch * kv_heads * ntile
     grid = units * splits
-    half = dtype == "f16"                    # the Q K^T operands' type
-    p_f16 = half and not quant               # P and V in f16; otherwise bf16, P in two parts
+    half = dtype == "f16" or quant           # the operands' type; in bf16 P comes in two parts
+    p_f16 = half
+    raw_b = BKV * D if quant else 0          # raw bytes of a K or V tile
     row_b = D * 2
     q_bytes, q_box = ROWS * row_b, ROWS * 128
     kv_bytes, kv_box = BKV * row_b, BKV * 128
@@ -153,7 +162,7 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     pieces = max(1, BKV // page)             # pages of a tile
     box_rows = min(page, BKV)
     if quant:
-        threads, soft0, mma_warp = 288, 4, 8
+        threads, soft0, mma_warp = 256, 4, 1
     else:
         threads, soft0, mma_warp = 192, 2, 1
     idesc_qk = idesc_f16(ROWS, BKV, False, False, half=half)
@@ -238,14 +247,16 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     raw = o("mov.u32", smem_sym)
     sQ = o("and.b32", o("add.u32", raw, 1023), -1024)
     sKV = o("add.u32", sQ, q_bytes)
-    bars = o("add.u32", sKV, STAGES * kv_bytes)
+    # bytes: two raw tiles, then one converted K and V
+    sRaw = o("add.u32", sKV, 2 * kv_bytes) if quant else None
+    bars = o("add.u32", sKV, 2 * kv_bytes + 4 * raw_b if quant else STAGES * kv_bytes)
     nwarps = o("shr.u32", o("add.u32", vrows, 31), 5)          # softmax warps that have a row
     l_init = e.L("noinit")
     e(f"@{e.cond('ne.u32', tid, 0)} bra {l_init};")
     e(f"mbarrier.init.shared::cta.b64 [{bars}+{QFULL}], {nwarps};")
     for s in range(STAGES):
-        e(f"mbarrier.init.shared::cta.b64 [{bars}+{FULL + 8 * s}], {2 if quant else 1};")
-        e(f"mbarrier.init.shared::cta.b64 [{bars}+{EMPTY + 8 * s}], 1;")
+        e(f"mbarrier.init.shared::cta.b64 [{bars}+{FULL + 8 * s}], {2 if quant and s >= 2 else 1};")
+        e(f"mbarrier.init.shared::cta.b64 [{bars}+{EMPTY + 8 * s}], {2 if quant and s < 2 else 1};")
     for u in range(2):
         e(f"mbarrier.init.shared::cta.b64 [{bars}+{SFULL + 8 * u}], 1;")
         e(f"mbarrier.init.shared::cta.b64 [{bars}+{PFULL + 8 * u}], {nwarps};")
@@ -288,7 +299,10 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         return e.cond("lt.u32", pg, pages)
 
     # ------------------------------------------------------------------ loads
-    if not quant:
+    l_conv = e.L("conv")
+    if quant:
+        e(f"@{e.cond('ge.u32', warp, 2)} bra {l_conv};")
+    if True:
         tk, tv = [o("cvta.param.u64", o("mov.u64", f"p_tm{x}", cls="rd"), cls="rd") for x in "KV"]
         per_batch = 32 // pieces                               # tiles whose pages one lane-load fetches
         sub = o("div.u32", lane, pieces) if pieces > 1 else lane
@@ -343,171 +357,134 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
             vt = tile_of(j)
             pgc = o("selp.b32", mine, -1, valid(mine))         # outside the pool: the box reads zeros
             roff = o("mul.lo.u32", o("rem.u32", vt, page // BKV), BKV) if page > BKV else 0
-            for kv, tm in enumerate((tk, tv)):
-                st_ = 2 * u + kv
+            ma = o("mad.lo.u32", o("and.b32", j, 3), 8, bars)
+
+            def arm(st_, nbytes, first):
+                """Waits for ring stage st_, notes the mask words with a tile's first box, expects the bytes."""
                 wait_bar_warp(e, f"{bars}+{EMPTY + 8 * st_}", o("xor.b32", ph, 1), err, ERR_LOAD, l_done)
-                if kv == 0:
-                    ma = o("mad.lo.u32", o("and.b32", j, 3), 8, bars)
+                if first:
                     e(f"@{p_l0} st.shared.v2.b32 [{ma}+{KMASK}], {{{words[0]}, {words[1]}}};")
-                e(f"@{p_l0} mbarrier.arrive.expect_tx.shared::cta.b64 _, [{bars}+{FULL + 8 * st_}], {kv_bytes};")
+                e(f"@{p_l0} mbarrier.arrive.expect_tx.shared::cta.b64 _, [{bars}+{FULL + 8 * st_}], {nbytes};")
                 e(f"mov.u32 {armed[st_]}, {ph};")
                 e("bar.warp.sync -1;")
-                for h in range(boxes):
-                    dst = o("add.u32", sKV, st_ * kv_bytes + h * kv_box)
+
+            def box(tm, x, dst, st_):
+                if pieces > 1:
+                    dst = o("mad.lo.u32", piece, page * min(128, row_b if not quant else D), dst)
+                e(f"@{p_pc} cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+                  f"[{dst}], [{tm}, {{{x}, {roff}, {kvh}, {pgc}}}], [{bars}+{FULL + 8 * st_}];")
+
+            if quant:
+                ok_ = valid(mine)
+                here = o("and.b32", o("vote.sync.ballot.b32", ok_, -1), (1 << pieces) - 1)
+                arm(u, o("mad.lo.u32", o("popc.b32", here), 2 * box_rows * 4, 2 * raw_b), True)
+                e(f"and.pred {ok_}, {ok_}, {p_pc};")
+                for kv, (tm, scp) in enumerate(((tk, gptr("p_KS")), (tv, gptr("p_VS")))):
+                    box(tm, 0, o("add.u32", sRaw, (2 * u + kv) * raw_b), u)
+                    first = o("mad.lo.u32", kvh, page, roff)
+                    off = o("mad.wide.u32", mine, kv_heads * page * 4, wide(first, 4), cls="rd")
+                    sd = o("add.u32", bars, RAWSC + (2 * u + kv) * BKV * 4)
                     if pieces > 1:
-                        dst = o("mad.lo.u32", piece, page * 128, dst)
-                    e(f"@{p_pc} cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-                      f"[{dst}], [{tm}, {{{64 * h}, {roff}, {kvh}, {pgc}}}], [{bars}+{FULL + 8 * st_}];")
+                        sd = o("mad.lo.u32", piece, page * 4, sd)
+                    e(f"@{ok_} cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [{sd}], [{at(scp, off)}], "
+                      f"{box_rows * 4}, [{bars}+{FULL + 8 * u}];")
+            else:
+                for kv, tm in enumerate((tk, tv)):
+                    arm(2 * u + kv, kv_bytes, kv == 0)
+                    for h in range(boxes):
+                        box(tm, 64 * h, o("add.u32", sKV, (2 * u + kv) * kv_bytes + h * kv_box), 2 * u + kv)
             e(f"add.u32 {j}, {j}, 1;")
         e(f"bra {l_top};")
         e.label(l_done)
-        for s in range(STAGES):
+        for s in range(2 if quant else STAGES):
             skip = e.L("nodrain")
             e(f"@{e.cond('eq.u32', armed[s], 2)} bra {skip};")
             wait_bar_warp(e, f"{bars}+{FULL + 8 * s}", armed[s], err, ERR_DRAIN, skip)
             e.label(skip)
         e(f"bra {l_end};")
-    else:
-        # warps 0, 1 load K and both scales, warps 2, 3 load V; thread t of 64 takes 16 bytes of rows
-        # t / 4 + 16 k, k = 0..3, in each 64-byte half (4 lanes a row half: whole 32-byte sectors, and the
-        # 16-byte stores of 8 lanes fall into 8 different bank groups)
+    if quant:
+        # ---------------------------------------------------------------- bytes to f16 (warps 2 and 3)
+        e.label(l_conv)
         t64 = o("and.b32", tid, 63)
-        p_v = e.cond("ge.u32", warp, 2)
-        isv = o("selp.u32", 1, 0, p_v)
-        pool = o("selp.b64", gptr("p_VC"), gptr("p_KC"), p_v, cls="rd")
-        ks_ptr, vs_ptr = gptr("p_KS"), gptr("p_VS")
-        rsub, chunk16 = o("shr.u32", t64, 2), o("and.b32", t64, 3)
-        npg = 1 if pieces == 1 else 4
-
-        def key_rows(j):
-            """(first key of the part's tile j, whether there is one)."""
-            return o("shl.b32", tile_of(j), 6), e.cond("lt.u32", j, nb)
-
-        def entries(j, regs):
-            """The pages of this thread's rows of tile j: one for all, or one for each of its four; and the
-            page of row t64, whose scales it loads."""
-            k0, ok = key_rows(j)
-            todo = [(regs[0], k0)] if npg == 1 else [(regs[k], o("add.u32", k0, o("add.u32", rsub, 16 * k)))
-                                                     for k in range(4)]
-            if npg > 1:
-                todo.append((regs[4], o("add.u32", k0, t64)))
-            for dst, key in todo:
-                okk = e.cond("lt.u32", key, w["end"])
-                e(f"and.pred {okk}, {okk}, {ok};")
-                entry(dst, o("div.u32", key, page), okk)
-
-        def place(pg, key):
-            """Row of the pool, flattened over pages, heads and rows (64 bits), of ``key`` on page ``pg``."""
-            r_ = o("mul.wide.u32", pg, kv_heads * page, cls="rd")
-            in_page = o("rem.u32", key, page)
-            return at(r_, wide(o("mad.lo.u32", kvh, page, in_page), 1))
-
-        def data(j, regs, dst, sc):
-            """Loads tile j: 16 bytes per row and half into ``dst``, the scales of row t64 into ``sc``; rows without
-            a key read as byte 128, which is 0."""
-            k0, ok = key_rows(j)
-            for k in range(4):
-                key = o("add.u32", k0, o("add.u32", rsub, 16 * k))
-                pg = regs[0] if npg == 1 else regs[k]
-                p_ = e.cond("lt.u32", key, w["end"])
-                e(f"and.pred {p_}, {p_}, {ok};")
-                e(f"and.pred {p_}, {p_}, {valid(pg)};")
-                a_ = at(at(pool, o("mul.lo.s64", place(pg, key), D, cls="rd")), wide(chunk16, 16))
-                for h in range(boxes):
-                    d_ = dst[h * 4 + k]
-                    for x in d_:
-                        e(f"mov.b32 {x}, 0x80808080;")
-                    e(f"@{p_} ld.global.nc.L1::no_allocate.v4.b32 {{{', '.join(d_)}}}, [{a_}+{64 * h}];")
-            l_ = e.L("noscale")
-            for x in sc:
-                e(f"mov.b32 {x}, 0f00000000;")
-            e(f"mov.u32 {sc_ok}, 0;")
-            e(f"@{p_v} bra {l_};")
-            key = o("add.u32", k0, t64)
-            pg = regs[0] if npg == 1 else regs[4]
-            p_ = e.cond("lt.u32", key, w["end"])
-            e(f"and.pred {p_}, {p_}, {ok};")
-            e(f"and.pred {p_}, {p_}, {valid(pg)};")
-            off = o("mul.lo.s64", place(pg, key), 4, cls="rd")
-            e(f"@{p_} ld.global.nc.f32 {sc[0]}, [{at(ks_ptr, off)}];")
-            e(f"@{p_} ld.global.nc.f32 {sc[1]}, [{at(vs_ptr, off)}];")
-            e(f"selp.u32 {sc_ok}, 1, 0, {p_};")
-            e.label(l_)
-
-        pgs = [e.r() for _ in range(1 if npg == 1 else 5)]
-        bufs = [[[e.r() for _ in range(4)] for _ in range(4 * boxes)] for _ in range(2)]
-        scs = [[e.r("f"), e.r("f")] for _ in range(2)]
-        oks = [e.r() for _ in range(2)]
+        quarter, u8_ = o("shr.u32", t64, 3), o("and.b32", t64, 7)
+        piece4, odd = o("and.b32", u8_, 3), o("shr.u32", u8_, 2)
+        rlow = o("xor.b32", o("shl.b32", quarter, 1), o("mul.lo.u32", odd, 5))       # row within 16
+        c64, c1152 = o("mov.b32", "0x64646464"), o("mov.b32", "0x64806480")
+        if D == 128:                                            # 16-byte pieces by the row's low three bits
+            raw_at = [o("mad.lo.u32", o("xor.b32", o("add.u32", piece4, 4 * h), o("and.b32", rlow, 7)), 16,
+                        o("shl.b32", rlow, 7)) for h in range(2)]
+        else:                                                   # 64-byte rows: by bits 1 and 2
+            raw_at = [o("mad.lo.u32", o("xor.b32", piece4, o("and.b32", o("shr.u32", rlow, 1), 3)), 16,
+                        o("shl.b32", rlow, 6))]
+        out_at = [o("mad.lo.u32", o("xor.b32", o("mad.lo.u32", piece4, 2, i), o("and.b32", rlow, 7)), 16,
+                    o("shl.b32", rlow, 7)) for i in range(2)]
+        p_l0c = e.cond("eq.u32", lane, 0)
+        p_w2 = e.cond("eq.u32", warp, 2)
+        vpow = o("mov.b32", "0x00800000")                       # the values' power of two (its f32 bits)
         j = o("mov.u32", 0)
-        entries(j, pgs)
-        sc_ok = oks[0]
-        data(j, pgs, bufs[0], scs[0])
-        entries(o("mov.u32", 1), pgs)
-        l_top, l_done = e.L("ld"), e.L("ldd")
-        p_l0 = e.cond("eq.u32", lane, 0)
-        zero_ = o("mov.u32", 0)
-        swz = o("and.b32", rsub, 7)
+        l_top, l_done = e.L("cv"), e.L("cvd")
         e.label(l_top)
-        for u in range(2):
-            e(f"@{e.cond('ge.u32', j, nb)} bra {l_done};")
-            ph = o("and.b32", o("shr.u32", j, 1), 1)
-            j1 = o("add.u32", j, 1)
-            sc_ok = oks[1 - u]
-            data(j1, pgs, bufs[1 - u], scs[1 - u])             # the next tile's loads in flight,
-            entries(o("add.u32", j, 2), pgs)                   # and the pages of the one after it
-            fb = o("mad.lo.u32", isv, 8, bars)
-            wait_bar_warp(e, f"{fb}+{EMPTY + 16 * u}", o("xor.b32", ph, 1), err, ERR_LOAD, l_done)
-            stage = o("mad.lo.u32", isv, kv_bytes, sKV)
-            # K in the type of Q; V in bf16
-            l_v, l_cv = e.L("asbf"), e.L("cvd")
-
-            def convert(as_half):
-                for h in range(boxes):
-                    for k in range(4):
-                        out = []
-                        for x in bufs[u][h * 4 + k]:
-                            for sel in ("0x4140", "0x4342"):
-                                if as_half:
-                                    t_ = o("prmt.b32", x, c64, sel)
-                                    out.append(o("sub.rn.f16x2", t_, c1152))
-                                else:
-                                    t_ = o("prmt.b32", x, zero_, sel)
-                                    m_ = o("lop3.b32", t_, "0x007F007F", c4300, "0xEA")     # (t & 7F) | 4300
-                                    c_ = o("lop3.b32", t_, "0x00800080", c4380, "0x6A")     # (t & 80) ^ 4380
-                                    out.append(o("sub.rn.bf16x2", m_, c_))
-                        # bytes 16 c.. of half h are columns 16 c..: two 16-byte chunks of the row's 128
-                        ra = o("mad.lo.u32", rsub, 128, o("add.u32", stage, 2 * u * kv_bytes + h * kv_box + k * 2048))
-                        for i in range(2):
-                            ch = o("xor.b32", o("mad.lo.u32", chunk16, 2, i), swz)
-                            sa = o("mad.lo.u32", ch, 16, ra)
-                            e(f"st.shared.v4.b32 [{sa}], {{{', '.join(out[4 * i:4 * i + 4])}}};")
-
-            if half:
-                c64, c1152 = o("mov.b32", "0x64646464"), o("mov.b32", "0x64806480")
-            c4300, c4380 = o("mov.b32", "0x43004300"), o("mov.b32", "0x43804380")
-            if half:
-                e(f"@{p_v} bra {l_v};")
-                convert(True)
-                e(f"bra {l_cv};")
-                e.label(l_v)
-            convert(False)
-            e.label(l_cv)
-            # K's warps: the scales of 64 keys and the mask words (a key has a page and lies below the end)
-            l_ns = e.L("nosc")
-            e(f"@{p_v} bra {l_ns};")
-            sa = o("mad.lo.u32", o("and.b32", j, 3), BKV * 4, bars)
-            sa = o("mad.lo.u32", t64, 4, sa)
-            e(f"st.shared.f32 [{sa}+{KSC}], {scs[u][0]};")
-            e(f"st.shared.f32 [{sa}+{VSC}], {scs[u][1]};")
-            mw_ = o("vote.sync.ballot.b32", e.cond("ne.u32", oks[u], 0), -1)
-            ma = o("mad.lo.u32", o("and.b32", j, 3), 8, bars)
-            ma = o("mad.lo.u32", warp, 4, ma)
-            e(f"@{p_l0} st.shared.b32 [{ma}+{KMASK}], {mw_};")
-            e.label(l_ns)
+        e(f"@{e.cond('ge.u32', j, nb)} bra {l_done};")
+        u_, ph, ph1 = o("and.b32", j, 1), o("and.b32", o("shr.u32", j, 1), 1), o("and.b32", j, 1)
+        rb = o("mad.lo.u32", u_, 8, bars)
+        wait_bar_warp(e, f"{rb}+{FULL}", ph, err, ERR_LOAD, l_done)
+        slot_c = o("and.b32", j, 3)
+        l_nosc = e.L("nosc")
+        e(f"@!{p_w2} bra {l_nosc};")
+        # warp 2: the tile's scales, two a lane; those of V over the power, which grows when one reaches twice it
+        rs = o("mad.lo.u32", lane, 8, o("mad.lo.u32", u_, 2 * BKV * 4, bars))
+        ksv, vsv = [e.r("f"), e.r("f")], [e.r("f"), e.r("f")]
+        e(f"ld.shared.v2.f32 {{{ksv[0]}, {ksv[1]}}}, [{rs}+{RAWSC}];")
+        e(f"ld.shared.v2.f32 {{{vsv[0]}, {vsv[1]}}}, [{rs}+{RAWSC + BKV * 4}];")
+        key0c = o("mad.lo.u32", lane, 2, o("shl.b32", tile_of(j), 6))
+        mw = o("mad.lo.u32", slot_c, 8, bars)
+        mw = o("ld.shared.b32", f"[{o('mad.lo.u32', o('shr.u32', lane, 4), 4, mw)}+{KMASK}]")
+        big = o("mov.b32", "0f00000000", cls="f")
+        for i in range(2):
+            bit = o("and.b32", o("shr.u32", mw, o("add.u32", o("shl.b32", o("and.b32", lane, 15), 1), i)), 1)
+            kk = o("add.u32", key0c, i) if i else key0c
+            pk2 = e.cond("lt.u32", kk, w["end"])
+            pk1 = e.cond("ne.u32", bit, 0)
+            e(f"and.pred {pk1}, {pk1}, {pk2};")
+            if window is not None:                              # nor those that no row sees
+                p1, p2 = e.cond("ge.u32", kk, w["lo"]), e.cond("lt.u32", kk, sinks)
+                e(f"or.pred {p1}, {p1}, {p2};")
+                e(f"and.pred {pk1}, {pk1}, {p1};")
+            e(f"@{pk1} max.f32 {big}, {big}, {vsv[i]};")        # a NaN drops out
+        bigb = o("redux.sync.max.u32", o("mov.b32", big), -1)
+        bigb = o("min.u32", o("and.b32", bigb, "0x7F800000"), "0x7E000000")
+        grow = e.cond("gt.u32", bigb, vpow)
+        e(f"@{grow} mov.u32 {vpow}, {bigb};")
+        vinv = o("mov.b32", o("sub.u32", "0x7F000000", vpow), cls="f")
+        sd = o("mad.lo.u32", lane, 8, o("mad.lo.u32", slot_c, BKV * 4, bars))
+        e(f"st.shared.v2.f32 [{sd}+{KSC}], {{{ksv[0]}, {ksv[1]}}};")
+        v0, v1 = (o("mul.f32", x, vinv, cls="f") for x in vsv)
+        e(f"st.shared.v2.f32 [{sd}+{VSC}], {{{v0}, {v1}}};")
+        e(f"@{p_l0c} st.shared.b32 [{o('mad.lo.u32', slot_c, 4, bars)}+{VREF}], {vpow};")
+        e.label(l_nosc)
+        for kv in range(2):
+            src = o("mad.lo.u32", u_, 2 * raw_b, o("add.u32", sRaw, kv * raw_b))
+            words = []
+            for h in range(boxes):
+                for k in range(4):
+                    d_ = [e.r() for _ in range(4)]
+                    e(f"ld.shared.v4.b32 {{{', '.join(d_)}}}, [{o('add.u32', src, raw_at[h])}+{16 * k * D}];")
+                    words.append(d_)
+            wait_bar_warp(e, f"{bars}+{EMPTY + 8 * (2 + kv)}", o("xor.b32", ph1, 1), err, ERR_LOAD, l_done)
+            dsts = [o("add.u32", o("add.u32", sKV, kv * kv_bytes), x) for x in out_at]
+            for h in range(boxes):
+                for k in range(4):
+                    out = [o("sub.rn.f16x2", o("prmt.b32", x, c64, sel), c1152)
+                           for x in words[4 * h + k] for sel in ("0x4140", "0x4342")]
+                    for i in range(2):
+                        e(f"st.shared.v4.b32 [{dsts[i]}+{h * kv_box + 16 * k * 128}], "
+                          f"{{{', '.join(out[4 * i:4 * i + 4])}}};")
             e("fence.proxy.async.shared::cta;")
             e("bar.warp.sync -1;")
-            e(f"@{p_l0} mbarrier.arrive.shared::cta.b64 _, [{fb}+{FULL + 16 * u}];")
-            e(f"mov.u32 {j}, {j1};")
+            if kv:
+                e(f"@{p_l0c} mbarrier.arrive.shared::cta.b64 _, [{rb}+{EMPTY}];")
+            e(f"@{p_l0c} mbarrier.arrive.shared::cta.b64 _, [{bars}+{FULL + 8 * (2 + kv)}];")
+        e(f"add.u32 {j}, {j}, 1;")
         e(f"bra {l_top};")
         e.label(l_done)
         e(f"bra {l_end};")
@@ -531,8 +508,10 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
 
     q0 = desc(sQ, khi)
     qd = [plus(q0, (k // 4) * q_box + (k % 4) * 32) for k in range(D // 16)]
-    stg = [o("add.u32", sKV, s * kv_bytes) for s in range(STAGES)]
-    kd, vd = [desc(stg[2 * u], khi) for u in range(2)], [desc(stg[2 * u + 1], vhi) for u in range(2)]
+    ring_k, ring_v = ([2, 2], [3, 3]) if quant else ([0, 2], [1, 3])         # barriers of a tile's K and V by its parity
+    stg = [o("add.u32", sKV, s * kv_bytes) for s in range(2 if quant else STAGES)]
+    kd = [desc(stg[0 if quant else 2 * u], khi) for u in range(2)]
+    vd = [desc(stg[1 if quant else 2 * u + 1], vhi) for u in range(2)]
     scol = [o("add.u32", taddr, S0 + BKV * u) for u in range(2)]
 
     def commit(off):
@@ -546,11 +525,11 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         for k in range(D // 16):
             e(f"tcgen05.mma.cta_group::1.kind::f16 [{scol[u]}], {qd[k]}, {plus(kd[u], (k // 4) * kv_box + (k % 4) * 32)}, "
               f"{iqk}, {ptrue if k else pfalse};")
-        commit(EMPTY + 8 * (2 * u))
+        commit(EMPTY + 8 * ring_k[u])
         commit(SFULL + 8 * u)
 
     j = o("mov.u32", 0)
-    ring(0, zero2)
+    ring(ring_k[0], zero2)
     qk(0)
     l_mg = e.L("mg")
     e.label(l_mg)
@@ -560,10 +539,10 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         have = e.cond("lt.u32", jn, nb)
         l_nok = e.L("nok")
         e(f"@!{have} bra {l_nok};")
-        ring(2 * (1 - u), ph if u == 0 else o("xor.b32", ph, 1))
+        ring(ring_k[1 - u], str(1 - u) if quant else ph if u == 0 else o("xor.b32", ph, 1))
         qk(1 - u)
         e.label(l_nok)
-        ring(2 * u + 1, ph)
+        ring(ring_v[u], str(u) if quant else ph)
         wait_bar(e, f"{bars}+{PFULL + 8 * u}", ph, err, ERR_MMA, l_mdone)
         e("tcgen05.fence::after_thread_sync;")
         pacc = e.cond("ne.u32", j, 0)
@@ -571,7 +550,7 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
             for k in range(BKV // 16):
                 e(f"tcgen05.mma.cta_group::1.kind::f16 [{taddr}], [{scol[u]}+{BKV // 2 * part + 8 * k}], "
                   f"{plus(vd[u], 2048 * k)}, {ipv}, {pacc if k == 0 and part == 0 else ptrue};")
-        commit(EMPTY + 8 * (2 * u + 1))
+        commit(EMPTY + 8 * ring_v[u])
         commit(PFREE + 8 * u)
         e(f"@!{have} bra {l_mdone};")
         e(f"mov.u32 {j}, {jn};")
@@ -589,6 +568,7 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     per_row = row_b // 16                                      # lanes a row takes
     qsub, qch = o("div.u32", lane, per_row), o("rem.u32", lane, per_row)
     passes = 32 * per_row // 32
+    recast = quant and dtype == "bf16"
     for p0 in range(0, passes, 8):
         ws, rr_ = [], []
         for p_ in range(p0, min(passes, p0 + 8)):
@@ -600,6 +580,24 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
             ws.append(d_)
             rr_.append(r_)
         for d_, r_ in zip(ws, rr_):
+            if recast:
+                # the row's largest number to 2^14 by a power of two (at most 2^40), then f16: see above
+                big = None
+                for x in d_:
+                    a_ = o("and.b32", x, "0x7FFF7FFF")
+                    big = a_ if big is None else o("max.u16x2", big, a_)
+                big = o("max.u32", o("and.b32", big, 65535), o("shr.u32", big, 16))
+                k_ = 1
+                while k_ < per_row:
+                    big = o("max.u32", big, o("shfl.sync.bfly.b32", big, k_, 31, -1))
+                    k_ *= 2
+                ex = o("min.s32", o("sub.s32", 127 + 14, o("shr.u32", big, 7)), 40)
+                up = o("shl.b32", o("add.s32", ex, 127), 23, cls="f")
+                down = o("shl.b32", o("sub.s32", 127, ex), 23, cls="f")
+                qsa = o("mad.lo.u32", r_, 4, bars)
+                e(f"@{e.cond('eq.u32', qch, 0)} st.shared.f32 [{qsa}+{QSC}], {o('mul.f32', down, cscale, cls='f')};")
+                d_ = [o("cvt.rn.f16x2.f32", o("mul.f32", o("and.b32", x, -65536, cls="f"), up, cls="f"),
+                        o("mul.f32", o("shl.b32", x, 16, cls="f"), up, cls="f")) for x in d_]
             box = o("shr.u32", qch, 3)
             ch = o("xor.b32", o("and.b32", qch, 7), o("and.b32", r_, 7))
             sa = o("mad.lo.u32", box, q_box, sQ)
@@ -613,6 +611,10 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     lanebase = o("add.u32", o("shl.b32", quad, 21), taddr)
     tok = o("div.u32", rowl, group) if group > 1 else rowl
     pos = o("min.s32", o("add.s32", pos0, tok), pos1)          # rows without a token: the last one's
+    cf = o("mov.b32", cscale, cls="f")                          # scale * log2(e) for this row's scores
+    if recast:
+        e(f"ld.shared.f32 {cf}, [{o('mad.lo.u32', rowl, 4, bars)}+{QSC}];")
+    vref = o("mov.b32", "0f00800000", cls="f") if quant else None
     s_ = [e.r("f") for _ in range(BKV)]
     mref, lsum = o("mov.b32", "0fFF800000", cls="f"), o("mov.b32", "0f00000000", cls="f")
     j = o("mov.u32", 0)
@@ -636,11 +638,20 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     sca = None
     if quant:
         sca = o("mad.lo.u32", slot_a, BKV * 4, bars)
-        for c in range(0, BKV, 4):
-            kf = [e.r("f") for _ in range(4)]
-            e(f"ld.shared.v4.f32 {{{', '.join(kf)}}}, [{sca}+{KSC + 4 * c}];")
-            for i in range(4):
-                e(f"mul.f32 {s_[c + i]}, {s_[c + i]}, {kf[i]};")
+        vnew = o("ld.shared.f32", f"[{o('mad.lo.u32', slot_a, 4, bars)}+{VREF}]", cls="f")
+
+        def times(off):
+            """The row times 64 numbers in shared memory, two at a time."""
+            for c in range(0, BKV, 4):
+                kp = [e.r("rd"), e.r("rd")]
+                e(f"ld.shared.v2.b64 {{{kp[0]}, {kp[1]}}}, [{sca}+{off + 4 * c}];")
+                for i in range(2):
+                    x0, x1 = s_[c + 2 * i], s_[c + 2 * i + 1]
+                    xp = e.r("rd")
+                    e(f"mov.b64 {xp}, {{{x0}, {x1}}};")
+                    e(f"mul.rn.f32x2 {xp}, {xp}, {kp[i]};")
+                    e(f"mov.b64 {{{x0}, {x1}}}, {xp};")
+        times(KSC)
     # the keys of the tile this row sees, as 64 bits: up to its own position, inside the window or among
     # the sinks, on a page.  Tiles that every row of the warp sees whole skip all of it.
     lim = o("sub.s32", pos, key0)
@@ -719,25 +730,31 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     e(f"max.f32 {lvl[3]}, {lvl[3]}, {lvl[4]}, {lvl[5]};")
     e(f"max.f32 {lvl[6]}, {lvl[6]}, {lvl[7]};")
     e(f"max.f32 {lvl[0]}, {lvl[0]}, {lvl[3]}, {lvl[6]};")
-    mnew = o("max.f32", mref, o("mul.f32", lvl[0], cscale, cls="f"), cls="f")
+    mnew = o("max.f32", mref, o("mul.f32", lvl[0], cf, cls="f"), cls="f")
     alpha = o("mov.b32", "0f3F800000", cls="f")
     l_first, l_after = e.L("first"), e.L("after")
     anyneed = e.cond("ne.u32", lane, lane)
     e(f"@{e.cond('eq.u32', j, 0)} bra {l_first};")
     need = e.cond("gt.f32", mnew, o("add.f32", mref, _f32(RESCALE), cls="f"))
+    if quant:
+        e(f"or.pred {need}, {need}, {e.cond('ne.f32', vnew, vref)};")           # the same for every row
     e(f"vote.sync.any.pred {anyneed}, {need}, -1;")
     e(f"@!{anyneed} bra {l_after};")
     e(f"ex2.approx.ftz.f32 {alpha}, {o('sub.f32', mref, mnew, cls='f')};")
     # a row that has seen nothing yet while another of the warp rescales: -inf - -inf must not make a NaN
     e(f"@{e.cond('eq.f32', mnew, '0fFF800000')} mov.b32 {alpha}, 0f3F800000;")
     e(f"mul.f32 {lsum}, {lsum}, {alpha};")
+    if quant:
+        inv_ = o("mov.b32", o("sub.u32", "0x7F000000", o("mov.b32", vnew)), cls="f")
+        e(f"mul.f32 {alpha}, {alpha}, {o('mul.f32', vref, inv_, cls='f')};")
     e.label(l_first)
     e(f"mov.b32 {mref}, {mnew};")
+    if quant:
+        e(f"mov.b32 {vref}, {vnew};")
     e.label(l_after)
-    lift = F16_LIFT if p_f16 else 0.0
+    lift = 0.0 if not p_f16 else QUANT_LIFT if quant else F16_LIFT
     negm = o("sub.f32", o("mov.b32", _f32(lift), cls="f"), mref, cls="f")
     e(f"@{e.cond('eq.f32', mref, '0fFF800000')} mov.b32 {negm}, 0f00000000;")
-    cf = o("mov.b32", cscale, cls="f")
     cp2, np2 = e.r("rd"), e.r("rd")
     e(f"mov.b64 {cp2}, {{{cf}, {cf}}};")
     e(f"mov.b64 {np2}, {{{negm}, {negm}}};")
@@ -756,19 +773,12 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
             e(f"add.rn.f32x2 {acc[k & 1]}, {acc[k & 1]}, {ep};")
 
     if p_f16:
-        for h in range(2):
-            cols = list(range(32 * h, 32 * h + 32))
-            exps(cols)
+        def pack(cols):
             hw = [o("cvt.rn.f16x2.f32", s_[c + 1], s_[c]) for c in cols[::2]]
-            e(f"tcgen05.st.sync.aligned.32x32b.x16.b32 [{sc_col}+{16 * h}], {{{', '.join(hw)}}};")
-    else:
-        exps(list(range(BKV)))
+            e(f"tcgen05.st.sync.aligned.32x32b.x16.b32 [{sc_col}+{cols[0] // 2}], {{{', '.join(hw)}}};")
         if quant:
-            for c in range(0, BKV, 4):
-                vf = [e.r("f") for _ in range(4)]
-                e(f"ld.shared.v4.f32 {{{', '.join(vf)}}}, [{sca}+{VSC + 4 * c}];")
-                for i in range(4):
-                    e(f"mul.f32 {s_[c + i]}, {s_[c + i]}, {vf[i]};")
+            exps(list(range(BKV)))
+            times(VSC)
             # a masked key's scale may be NaN: its weight is 0 whatever it was multiplied by
             l_nz = e.L("nz")
             e(f"@{v_all} bra {l_nz};")
@@ -776,6 +786,13 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
                 t_ = o("and.b32", (m0, m1)[c // 32], 1 << (c % 32) if c % 32 < 31 else -(1 << 31))
                 e(f"@{e.cond('eq.u32', t_, 0)} mov.b32 {s_[c]}, 0f00000000;")
             e.label(l_nz)
+        for h in range(2):
+            cols = list(range(32 * h, 32 * h + 32))
+            if not quant:
+                exps(cols)
+            pack(cols)
+    else:
+        exps(list(range(BKV)))
         for h in range(2):
             hi, lo = [], []
             for c in range(32 * h, 32 * h + 32, 2):
@@ -825,8 +842,10 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         e(f"@{e.cond('gt.u32', total, per)} bra {l_part};")
     p_zero = e.cond("eq.f32", lsum, "0f00000000")
     inv = o("rcp.rn.f32", o("selp.f32", "0f3F800000", lsum, p_zero, cls="f"), cls="f")
+    if quant:
+        e(f"mul.f32 {inv}, {inv}, {vref};")
     oa = at(o_ptr, wide(row_index(rowl), row_b))
-    pack = "cvt.rn.f16x2.f32" if half else "cvt.rn.bf16x2.f32"
+    out_cvt = "cvt.rn.f16x2.f32" if dtype == "f16" else "cvt.rn.bf16x2.f32"
     for c in range(D // 32):
         regs = s_[:32]
         e(f"tcgen05.ld.sync.aligned.32x32b.x32.b32 {{{', '.join(regs)}}}, [{lanebase}+{32 * c}];")
@@ -835,7 +854,7 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         for k in range(16):
             x0 = o("mul.f32", regs[2 * k], inv, cls="f")
             x1 = o("mul.f32", regs[2 * k + 1], inv, cls="f")
-            words.append(o("selp.b32", 0, o(pack, x1, x0), p_zero))
+            words.append(o("selp.b32", 0, o(out_cvt, x1, x0), p_zero))
         for i in range(2):
             e(f"@{p_row} st.global.v8.b32 [{oa}+{64 * c + 32 * i}], {{{', '.join(words[8 * i:8 * i + 8])}}};")
     if splits > 1:
@@ -847,6 +866,9 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
             regs = s_[:32]
             e(f"tcgen05.ld.sync.aligned.32x32b.x32.b32 {{{', '.join(regs)}}}, [{lanebase}+{32 * c}];")
             e("tcgen05.wait::ld.sync.aligned;")
+            if quant:
+                for x in regs:
+                    e(f"mul.f32 {x}, {x}, {vref};")
             for i in range(4):
                 e(f"@{p_row} st.global.v8.f32 [{pa}+{128 * c + 32 * i}], {{{', '.join(regs[8 * i:8 * i + 8])}}};")
         mla = at(at(gptr("p_part"), grid * rows * D * 4), wide(pi, 8))
@@ -866,7 +888,7 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
 
     if quant:
         qn, kn, vn, ksn, vsn, tn, ln, fn, on = names
-        params = [("Q", qn, 16), ("KC", kn, 16), ("VC", vn, 16), ("KS", ksn, 4), ("VS", vsn, 4)]
+        params = [("Q", qn, 16), ("KC", kn, 16), ("VC", vn, 16), ("KS", ksn, 16), ("VS", vsn, 16)]
     else:
         qn, kn, vn, tn, ln, fn, on = names
         params = [("Q", qn, 16), ("KC", kn, 16), ("VC", vn, 16)]
@@ -875,12 +897,11 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     if splits > 1:
         params += [("part", scratch, 32)]
         sc_spec = [{"name": scratch, "dtype": "f32", "shape": [grid * rows, D + 2], "per_call": True}]
-    tmaps = []
-    if not quant:
-        es = 2
-        tmaps = [{"name": f"tm{x}", "tensor": nm, "dtype": dtype, "dims": [D, page, kv_heads, pages],
-                  "strides": [D * es, page * D * es, kv_heads * page * D * es], "box": [64, box_rows, 1, 1],
-                  "swizzle": "128B"} for x, nm in (("K", kn), ("V", vn))]
+    es = 1 if quant else 2
+    span = min(128, D * es)                                     # a box row, and the swizzle
+    tmaps = [{"name": f"tm{x}", "tensor": nm, "dtype": "u8" if quant else dtype, "dims": [D, page, kv_heads, pages],
+              "strides": [D * es, page * D * es, kv_heads * page * D * es], "box": [span // es, box_rows, 1, 1],
+              "swizzle": f"{span}B"} for x, nm in (("K", kn), ("V", vn))]
     plist = [f"\t.param .u64 p_{p}" for p, _, _ in params]
     plist += [f"\t.param .align 64 .b8 p_{t['name']}[128]" for t in tmaps] + ["\t.param .u64 p_err"]
     text = [f".visible .entry {name}(", ",\n".join(plist), ")", f".reqntid {threads}, 1, 1",
@@ -890,7 +911,7 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         "name": name, "kind": "tcgen05_paged_attention", "params": [n for _, n, _ in params],
         "raw_entry": text, "raw_decls": [f".extern .shared .align 1024 .b8 {smem_sym}[];"],
         "grid": [grid, 1, 1], "block": [threads, 1, 1],
-        "dyn_smem": q_bytes + STAGES * kv_bytes + (AUX_BYTES if quant else KSC) + 1024,
+        "dyn_smem": q_bytes + (2 * kv_bytes + 4 * raw_b + AUX_BYTES if quant else STAGES * kv_bytes + KSC) + 1024,
         "align": {n: a_ for _, n, a_ in params}, "zero_outputs": [], "tmaps": tmaps,
         "extra": [{"name": "__err", "kind": "errword"}], "scratch": sc_spec,
     }
