@@ -33,7 +33,7 @@ from __future__ import annotations
 import math
 
 from .ptxasm import wait_bar_warp
-from .tc_paged_attention import F16_LIFT, LOG2E, RESCALE, _E, _f32, _unit, join_entry
+from .tc_paged_attention import F16_LIFT, LOG2E, RESCALE, _E, _f32, _unit
 
 MAX_ROWS = 64
 QUANT_LIFT = 6.0                 # bytes: P's exponent is lifted by one less, since its scale may be twice vref
@@ -95,7 +95,7 @@ def _tiles_of(e, at, lens_ptr, fresh_ptr, b, ok, chunk, cap, window, sinks):
     n_, f_ = o("mov.u32", 0), o("mov.u32", 0)
     e(f"@{ok} ld.global.nc.u32 {n_}, [{at(lens_ptr, o('mul.wide.u32', b, 4, cls='rd'))}];")
     e(f"@{ok} ld.global.nc.u32 {f_}, [{at(fresh_ptr, o('mul.wide.u32', b, 4, cls='rd'))}];")
-    total = _unit(e, None, n_, f_, o("mov.u32", 0), 1, 1, chunk, chunk, cap, window, sinks)["total"]
+    total = _unit(e, n_, f_, o("mov.u32", 0), chunk, chunk, cap, window, sinks)["total"]
     return o("selp.u32", total, 0, e.cond("gt.s32", f_, 0))
 
 
@@ -225,7 +225,7 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
     b_new = o("ld.global.nc.u32", f"[{at(fresh_ptr, wide(b, 4))}]")
     if not ctas:
         e(f"@{e.cond('le.s32', b_new, 0)} ret;")              # nothing new in this sequence
-    w = _unit(e, None, b_len, b_new, o("mov.u32", 0), 1, 1, chunk, chunk, cap, window, sinks)
+    w = _unit(e, b_len, b_new, o("mov.u32", 0), chunk, chunk, cap, window, sinks)
     total, end, pos0, pos1 = w["total"], w["end"], w["pos0"], w["pos1"]
     i0, nb = None, total
     if ctas:
@@ -745,43 +745,141 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
     }
 
 
-def spread_join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype, window, sinks, names, scratch, ctas,
-                      min_tiles=MIN_TILES):
-    """The second entry of a spread module: rows whose unit has several runs (see
-    :func:`.tc_paged_attention.join_entry`); rows that see no key at all, which no run covers, become 0."""
-    rows = chunk * (heads // kv_heads)
+def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype, window, sinks, names, scratch, ctas,
+               min_tiles=MIN_TILES):
+    """The second entry: the rows of units of more than one run, o = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.  One
+    block a row, which finds its unit's runs by the same sums over the batch; its four warps take every fourth part,
+    so that a row of 100 parts is 25 loads deep.  Rows of units of one run are written already; rows that see no key
+    at all, which no run covers, become 0."""
+    D = dim
     group = heads // kv_heads
-    cap = max_pages * page
+    rows, cap = chunk * group, max_pages * page
+    per_lane = D // 32
+    e = _E()
+    o = e.o
 
-    def locate(e, at, gptr, lane, b, c, h, zero_row):
-        """(parts, function from a part's number to its row in the scratch) of row (b, c, h)."""
-        o = e.o
-        lens_ptr, fresh_ptr = gptr("p_lens"), gptr("p_fresh")
-        run, before, tb = o("mov.u32", 0), o("mov.u32", 0), o("mov.u32", 0)
-        for k in range(-(-batch // 32)):
-            bb = o("add.u32", lane, 32 * k) if k else lane
-            v = _tiles_of(e, at, lens_ptr, fresh_ptr, bb, e.cond("lt.u32", bb, batch), chunk, cap, window, sinks)
-            e(f"add.u32 {run}, {run}, {v};")
-            e(f"@{e.cond('lt.u32', bb, b)} add.u32 {before}, {before}, {v};")
-            e(f"@{e.cond('eq.u32', bb, b)} mov.u32 {tb}, {v};")
-        run, before, tb = (o("redux.sync.add.u32", x, -1) for x in (run, before, tb))
-        zero_row(e.cond("eq.u32", tb, 0))
-        per = o("div.u32", o("add.u32", o("mul.lo.u32", run, kv_heads), ctas - 1), ctas)
-        per = o("max.u32", per, min_tiles)
-        t0 = o("mad.lo.u32", before, kv_heads, o("mul.lo.u32", o("div.u32", h, group), tb))
-        first = o("div.u32", t0, per)
-        last = o("div.u32", o("sub.u32", o("add.u32", t0, tb), 1), per)
-        e(f"@{e.cond('eq.u32', first, last)} ret;")             # one run: written already
-        nact = o("add.u32", o("sub.u32", last, first), 1)
-        # the first run reaches the unit as a later segment unless it begins with it
-        late = o("selp.u32", 1, 0, e.cond("ne.u32", t0, o("mul.lo.u32", first, per)))
-        rowl = o("mad.lo.u32", c, group, o("rem.u32", h, group))
+    def gptr(pname):
+        return o("cvta.to.global.u64", o("ld.param.u64", f"[{pname}]", cls="rd"), cls="rd")
 
-        def part(s):
-            slot = o("shl.b32", o("add.u32", first, s), 1)
-            slot = o("add.u32", slot, o("selp.u32", late, 0, e.cond("eq.u32", s, 0)))
-            return o("mad.lo.u32", slot, rows, rowl)
-        return nact, part, 2 * ctas * rows
+    def at(base, x, n):
+        return o("add.s64", base, o("mul.wide.u32", x, n, cls="rd"), cls="rd")
 
-    return join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype, window, sinks, names, scratch,
-                      ctas, min_tiles, locate=locate)
+    tid = o("mov.u32", "%tid.x")
+    warp, lane = o("shr.u32", tid, 5), o("and.b32", tid, 31)
+    e("griddepcontrol.wait;")                                   # the parts are written
+    row = o("mov.u32", "%ctaid.x")
+    h, bc = o("rem.u32", row, heads), o("div.u32", row, heads)
+    c, b = o("rem.u32", bc, chunk), o("div.u32", bc, chunk)
+    b_new = o("ld.global.nc.u32", f"[{at(gptr('p_fresh'), b, 4)}]")
+    e(f"@{e.cond('ge.s32', c, b_new)} ret;")
+    lens_ptr, fresh_ptr = gptr("p_lens"), gptr("p_fresh")
+    run, before, tb = o("mov.u32", 0), o("mov.u32", 0), o("mov.u32", 0)
+    for k in range(-(-batch // 32)):
+        bb = o("add.u32", lane, 32 * k) if k else lane
+        v = _tiles_of(e, lambda x, y: o("add.s64", x, y, cls="rd"), lens_ptr, fresh_ptr, bb, e.cond("lt.u32", bb, batch),
+                      chunk, cap, window, sinks)
+        e(f"add.u32 {run}, {run}, {v};")
+        e(f"@{e.cond('lt.u32', bb, b)} add.u32 {before}, {before}, {v};")
+        e(f"@{e.cond('eq.u32', bb, b)} mov.u32 {tb}, {v};")
+    run, before, tb = (o("redux.sync.add.u32", x, -1) for x in (run, before, tb))
+    l_some = e.L("some")
+    e(f"@{e.cond('ne.u32', tb, 0)} bra {l_some};")             # a row that sees no key: 0
+    e(f"@{e.cond('ge.u32', tid, D // 2)} ret;")
+    e(f"st.global.b32 [{at(at(gptr('p_O'), row, D * 2), tid, 4)}], {o('mov.b32', 0)};")
+    e("ret;")
+    e.label(l_some)
+    per = o("div.u32", o("add.u32", o("mul.lo.u32", run, kv_heads), ctas - 1), ctas)
+    per = o("max.u32", per, min_tiles)
+    t0 = o("mad.lo.u32", before, kv_heads, o("mul.lo.u32", o("div.u32", h, group), tb))
+    first = o("div.u32", t0, per)
+    last = o("div.u32", o("sub.u32", o("add.u32", t0, tb), 1), per)
+    e(f"@{e.cond('eq.u32', first, last)} ret;")                # one run: written already
+    nact = o("add.u32", o("sub.u32", last, first), 1)
+    # the first run reaches the unit as a later segment unless it begins with it
+    late = o("selp.u32", 1, 0, e.cond("ne.u32", t0, o("mul.lo.u32", first, per)))
+    rowl = o("mad.lo.u32", c, group, o("rem.u32", h, group))
+
+    def part_row(s_):
+        slot = o("shl.b32", o("add.u32", first, s_), 1)
+        slot = o("add.u32", slot, o("selp.u32", late, 0, e.cond("eq.u32", s_, 0)))
+        return o("mad.lo.u32", slot, rows, rowl)
+
+    part_rows = 2 * ctas * rows
+    part = gptr("p_part")
+    ml = o("add.s64", part, part_rows * D * 4, cls="rd")
+    # the largest reference of the row's parts (every warp on its own)
+    m = o("mov.b32", "0fFF800000", cls="f")
+    s = o("mov.u32", lane)
+    l_m, l_md = e.L("m"), e.L("md")
+    e.label(l_m)
+    e(f"@{e.cond('ge.u32', o('and.b32', s, -32), nact)} bra {l_md};")           # the same for the warp
+    v = o("mov.b32", "0fFF800000", cls="f")
+    e(f"@{e.cond('lt.u32', s, nact)} ld.global.f32 {v}, [{at(ml, part_row(s), 8)}];")
+    e(f"max.f32 {m}, {m}, {v};")
+    e(f"add.u32 {s}, {s}, 32;")
+    e(f"bra {l_m};")
+    e.label(l_md)
+    for d in (16, 8, 4, 2, 1):
+        e(f"max.f32 {m}, {m}, {o('shfl.sync.bfly.b32', m, d, 31, -1, cls='f')};")
+    e(f"@{e.cond('eq.f32', m, '0fFF800000')} mov.b32 {m}, 0f00000000;")
+    acc = [o("mov.b32", "0f00000000", cls="f") for _ in range(per_lane)]
+    l = o("mov.b32", "0f00000000", cls="f")
+    s = o("mov.u32", warp)
+    l_top, l_done = e.L("p"), e.L("pd")
+    UN = 4
+    vec = f"v{per_lane}"
+    part_l = at(part, lane, per_lane * 4)
+    e.label(l_top)
+    e(f"@{e.cond('ge.u32', s, nact)} bra {l_done};")
+    loaded = []
+    for u in range(UN):
+        su = o("add.u32", s, 4 * u)
+        ok = e.cond("lt.u32", su, nact)
+        idx = part_row(su)
+        ms, ls = o("mov.b32", "0fFF800000", cls="f"), o("mov.b32", "0f00000000", cls="f")
+        e(f"@{ok} ld.global.v2.f32 {{{ms}, {ls}}}, [{at(ml, idx, 8)}];")
+        xs = [o("mov.b32", "0f00000000", cls="f") for _ in range(per_lane)]
+        e(f"@{ok} ld.global.{vec}.f32 {{{', '.join(xs)}}}, [{at(part_l, idx, D * 4)}];")
+        loaded.append((ms, ls, xs))
+    for ms, ls, xs in loaded:
+        f = o("ex2.approx.ftz.f32", o("sub.f32", ms, m, cls="f"), cls="f")
+        e(f"fma.rn.f32 {l}, {f}, {ls}, {l};")
+        for a_, x in zip(acc, xs):
+            e(f"fma.rn.f32 {a_}, {f}, {x}, {a_};")
+    e(f"add.u32 {s}, {s}, {4 * UN};")
+    e(f"bra {l_top};")
+    e.label(l_done)
+    sm = o("mov.u32", f"{name}_sum")
+    sl = o("mov.u32", f"{name}_l")
+    wa = o("mad.lo.u32", warp, D * 4, sm)
+    wa = o("mad.lo.u32", lane, per_lane * 4, wa)
+    e(f"st.shared.{vec}.f32 [{wa}], {{{', '.join(acc)}}};")
+    e(f"st.shared.f32 [{o('mad.lo.u32', warp, 4, sl)}], {l};")                 # every lane holds the same l
+    e("bar.sync 0;")
+    e(f"@{e.cond('ge.u32', tid, D // 2)} ret;")
+    ls = [e.r("f") for _ in range(4)]
+    e(f"ld.shared.v4.f32 {{{', '.join(ls)}}}, [{sl}];")
+    lt = o("add.f32", o("add.f32", ls[0], ls[1], cls="f"), o("add.f32", ls[2], ls[3], cls="f"), cls="f")
+    xs = [o("mov.b32", "0f00000000", cls="f") for _ in range(2)]
+    ra = o("mad.lo.u32", tid, 8, sm)
+    for k in range(4):
+        y = [e.r("f") for _ in range(2)]
+        e(f"ld.shared.v2.f32 {{{y[0]}, {y[1]}}}, [{ra}+{k * D * 4}];")
+        for i in range(2):
+            e(f"add.f32 {xs[i]}, {xs[i]}, {y[i]};")
+    p_zero = e.cond("eq.f32", lt, "0f00000000")
+    inv = o("rcp.rn.f32", o("selp.f32", "0f3F800000", lt, p_zero, cls="f"), cls="f")
+    x0, x1 = (o("mul.f32", x, inv, cls="f") for x in xs)
+    word = o("cvt.rn.f16x2.f32" if dtype == "f16" else "cvt.rn.bf16x2.f32", x1, x0)
+    word = o("selp.b32", 0, word, p_zero)
+    oa = at(at(gptr("p_O"), row, D * 2), tid, 4)
+    e(f"st.global.b32 [{oa}], {word};")
+    ln, fn, on = names
+    params = [("lens", ln, 4), ("fresh", fn, 4), ("O", on, 4), ("part", scratch, 32)]
+    text = [f".visible .entry {name}(", ",\n".join(f"\t.param .u64 p_{p}" for p, _, _ in params), ")",
+            ".reqntid 128, 1, 1", "{"]
+    text += e.decls() + e.lines + ["\tret;", "}"]
+    return {"name": name, "kind": "paged_attention_join", "params": [n for _, n, _ in params], "raw_entry": text,
+            "raw_decls": [f".shared .align 16 .b8 {name}_sum[{4 * D * 4}];", f".shared .align 16 .b8 {name}_l[16];"],
+            "grid": [batch * chunk * heads, 1, 1], "block": [128, 1, 1], "dyn_smem": 0,
+            "align": {n: a_ for _, n, a_ in params}, "zero_outputs": [], "pdl": True}

@@ -4,14 +4,15 @@ O = softmax(Q K^T * scale) V over the keys each token sees (:func:`..irgen.paged
 its own position, or a window of them and a few first ones, in pages that a table names.  The cache holds the
 activations' 16-bit type, or bytes with one f32 scale per token and head.
 
-**Work.**  A CTA owns up to 128 query rows of one sequence and one key head: as many tokens as fit with all
-their query heads (a row is token * group + head of the group), so one pass over a key head's keys serves its
-whole group.  It walks its keys in tiles of 64, the tiles of the first tokens and then those of the window
-when there is one.  When that makes too few CTAs for the GPU, or leaves it to one long sequence, the tiles
-of a unit are split over ``splits`` CTAs, each of at least ``min_tiles``; parts store O, the row's reference m and its sum
-l in f32 and a second entry joins them (o = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s).  A unit whose
-tiles fit one part writes O itself.  Two CTAs share an SM (half its TMEM columns and shared memory each), so
-one's loads and softmax run beside the other's products.
+**Work.**  A unit is up to 128 query rows of one sequence and one key head: as many tokens as fit with all their
+query heads (a row is token * group + head of the group), so one pass over a key head's keys serves its whole
+group.  It walks its keys in tiles of 64, the tiles of the first tokens and then those of the window when there is
+one.  The tiles of all units, in a row, are cut into equal runs, one for each CTA the GPU holds at a time (two an
+SM, half its TMEM columns and shared memory each, so that one's loads and softmax run beside the other's
+products): every CTA takes prefix sums over the units and so finds its own run, whatever the lengths are.  A unit of
+more than one run leaves parts in f32 (O, the row's reference m and its sum l) and a second entry joins them
+(o = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s).  Batches of very many units, and very short sequences, take one
+CTA a unit instead.
 
 **Roles.**  One thread issues the ``tcgen05.mma``: S(j+1) = Q K_(j+1)^T into one of two 64-column score buffers,
 then O += P(j) V_j.  Four softmax warps hold one row a thread; warps without a row take no part.  A warp loads by
@@ -32,6 +33,8 @@ largest still has 11 bits.  O is rescaled only when the row's maximum grew by mo
 name become -inf; a row that sees nothing ends as 0.  Rows of a V tile that no row of the CTA sees are zeroed in
 shared memory before the product (P is 0 there, but a stale row may hold NaN).
 
+The roles (loads, conversion, products, softmax) walk the run's segments on their own, each as far ahead as the
+barriers between them let it; barrier phases, ring stages and score buffers go by the tile's number in the run.
 Every wait is bounded and reports a code (71-76); TMEM is always freed.
 """
 from __future__ import annotations
@@ -102,24 +105,28 @@ def geometry(chunk, heads, kv_heads):
     return group, tq, -(-chunk // tq), min(tq, chunk) * group
 
 
-def plan_splits(batch, chunk, heads, kv_heads, page, max_pages, window, sinks, sms=148):
-    """(splits, least tiles of a part): one part where the units fill the GPU's two CTAs an SM, otherwise as many
-    parts as fill it, of at least 8 tiles.  Splitting more costs more than it evens out here: a part of 128 rows
-    writes and the join reads 64 KiB of f32, as much as two tiles of keys and values (a 2048-token chunk over
-    8192 keys ran at 876 TFLOP/s in one part and 647 in up to four)."""
+MAX_SPREAD_PAIRS = 256           # (sequence, token tile) pairs each CTA takes prefix sums of
+MIN_TILES = 8                    # a run's least tiles: a part of 128 rows is as many bytes as two of them
+
+
+def plan_ctas(batch, chunk, heads, kv_heads, page, max_pages, window, sinks, sms=148):
+    """CTAs to spread the tiles over, or 0 for one CTA a unit: for sequences of at most 8 tiles, and where the units
+    fill the GPU by themselves.  There the parts and the second launch cost more than equal runs give (a 2048-token
+    chunk over 8192 keys, 1024 units: 393 us against 412; a windowed chunk of 848 units 68 us against 90)."""
     group, tq, ntile, rows = geometry(chunk, heads, kv_heads)
     longest = -(-max_pages * page // BKV)
     if window is not None:
         longest = min(longest, -(-sinks // BKV) + (window + min(tq, chunk) - 1) // BKV + 2)
-    min_tiles = 8
-    units = batch * kv_heads * ntile
-    return max(1, min(longest // min_tiles, 2 * sms // units)), min_tiles
+    pairs = batch * ntile
+    if longest <= 8 or pairs > MAX_SPREAD_PAIRS or pairs * kv_heads >= 2 * sms:
+        return 0
+    return 2 * sms
 
 
-def _unit(e, k, b_len, b_new, c0, splits, min_tiles, tq, chunk, cap, window, sinks):
+def _unit(e, b_len, b_new, c0, tq, chunk, cap, window, sinks):
     """What a unit (a sequence's token tile) walks, from its length and new tokens: emitted alike by the attention
     and by the join.  Returns registers: the last token c1, first and last position, the first window key
-    ``lo``, sink tiles ``st``, ``gap`` (tile = i + gap from sink tile st on), tiles ``total`` and tiles per part."""
+    ``lo``, sink tiles ``st``, ``gap`` (tile = i + gap from sink tile st on) and the number of tiles ``total``."""
     n = e.o("min.s32", b_new, chunk)
     c1 = e.o("min.s32", e.o("add.s32", c0, tq), n)
     c1 = e.o("sub.s32", c1, 1)
@@ -136,21 +143,66 @@ def _unit(e, k, b_len, b_new, c0, splits, min_tiles, tq, chunk, cap, window, sin
         st = e.o("min.u32", wt0, -(-sinks // BKV))
         gap = e.o("sub.u32", wt0, st)
         total = e.o("sub.u32", tend, gap)
-    per = total
-    if splits > 1:
-        per = e.o("div.u32", e.o("add.u32", total, splits - 1), splits)
-        per = e.o("max.u32", per, min_tiles)
-    return dict(n=n, c1=c1, pos0=pos0, pos1=pos1, end=end, lo=lo, st=st, gap=gap, total=total, per=per)
+    return dict(n=n, c1=c1, pos0=pos0, pos1=pos1, end=end, lo=lo, st=st, gap=gap, total=total)
+
+
+class _Place:
+    """A (sequence, token tile) pair's registers: sequence ``b``, its length and new tokens, the tile's first token,
+    what :func:`_unit` gives, whether it has a token (``live``), its tiles (0 without one) and its rows."""
+
+    def __init__(self, e, pair, ok, lens, fresh, batch, chunk, group, tq, ntile, cap, window, sinks):
+        o = e.o
+        self.b = o("rem.u32", pair, batch)
+        tile = o("sub.u32", ntile - 1, o("div.u32", pair, batch))               # the longest rows of a sequence first
+        off = o("mul.wide.u32", self.b, 4, cls="rd")
+        n, f = o("mov.u32", 0), o("mov.u32", 0)
+        g = f"@{ok} " if ok else ""
+        e(f"{g}ld.global.nc.u32 {n}, [{o('add.s64', lens, off, cls='rd')}];")
+        e(f"{g}ld.global.nc.u32 {f}, [{o('add.s64', fresh, off, cls='rd')}];")
+        self.c0 = o("mul.lo.u32", tile, tq)
+        self.w = _unit(e, n, f, self.c0, tq, chunk, cap, window, sinks)
+        self.live = e.cond("lt.s32", self.c0, f)
+        self.tiles = o("selp.u32", self.w["total"], 0, self.live)
+        self.vrows = o("mul.lo.u32", o("add.u32", o("sub.u32", self.w["c1"], self.c0), 1), group)
+
+
+def _prefix(e, lane, pairs, tiles_of, run_heads):
+    """Inclusive prefix sums of ``tiles_of(pair, ok)`` times ``run_heads`` over the pairs, 32 to a register (lane l of
+    register k holds pair 32 k + l), and the total."""
+    o = e.o
+    sums, run = [], None
+    for k in range(-(-pairs // 32)):
+        q = o("add.u32", lane, 32 * k) if k else lane
+        sums.append(o("mul.lo.u32", tiles_of(q, e.cond("lt.u32", q, pairs)), run_heads))
+    for v in sums:
+        for d in (1, 2, 4, 8, 16):
+            up = o("shfl.sync.up.b32", v, d, 0, -1)
+            e(f"@{e.cond('ge.u32', lane, d)} add.u32 {v}, {v}, {up};")
+        if run is not None:
+            e(f"add.u32 {v}, {v}, {run};")
+        run = o("shfl.sync.idx.b32", v, 31, 31, -1)
+    return sums, run
+
+
+def _first_behind(e, sums, start):
+    """The first pair whose inclusive sum lies behind ``start``, and the sum before it."""
+    o = e.o
+    pair, before = o("mov.u32", 0), o("mov.u32", 0)
+    for v in sums:
+        past = e.cond("le.u32", v, start)
+        e(f"add.u32 {pair}, {pair}, {o('popc.b32', o('vote.sync.ballot.b32', past, -1))};")
+        e(f"max.u32 {before}, {before}, {o('redux.sync.max.u32', o('selp.u32', v, 0, past), -1)};")
+    return pair, before
 
 
 def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_pages, dtype, quant, window, sinks,
-                          scale, names, scratch, splits, min_tiles, prefix=""):
+                          scale, names, scratch, ctas, min_tiles=MIN_TILES, prefix=""):
     """The launch record and PTX; ``names``: Q, KC, VC, (KS, VS,) table, lens, fresh, O; ``scratch``: the parts'
     buffer, all their O rows and then their m and l."""
     D = dim
     group, tq, ntile, rows = geometry(chunk, heads, kv_heads)
-    units = batch * kv_heads * ntile
-    grid = units * splits
+    pairs = batch * ntile
+    grid = ctas or pairs * kv_heads
     half = dtype == "f16" or quant           # the operands' type; in bf16 P comes in two parts
     p_f16 = half
     raw_b = BKV * D if quant else 0          # raw bytes of a K or V tile
@@ -170,7 +222,7 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     kdesc_hi = smem_desc_hi(16, 1024)
     vdesc_hi = smem_desc_hi(kv_box, 1024)
     cscale = _f32(scale * LOG2E)
-    S0 = D                                   # score buffers behind O's columns
+    SCOL = D                                 # score buffers behind O's columns
     e = _E()
     o = e.o
 
@@ -191,57 +243,91 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     lane = o("and.b32", tid, 31)
     cta = o("mov.u32", "%ctaid.x")
     err, o_ptr = gptr("p_err"), gptr("p_O")
-    if splits > 1:
+    lens, fresh = gptr("p_lens"), gptr("p_fresh")
+
+    def place(pair, ok=None):
+        return _Place(e, pair, ok, lens, fresh, batch, chunk, group, tq, ntile, cap, window, sinks)
+
+    if ctas:
         e("griddepcontrol.launch_dependents;")                  # the join's blocks may come up and wait
-        unit, sp = o("div.u32", cta, splits), o("rem.u32", cta, splits)
+        sums, run = _prefix(e, lane, pairs, lambda q, ok: place(q, ok).tiles, kv_heads)
+        per = o("max.u32", o("div.u32", o("add.u32", run, ctas - 1), ctas), min_tiles)
+        start = o("mul.lo.u32", cta, per)
+        e(f"@{e.cond('ge.u32', start, run)} ret;")              # no tiles for this CTA
+        stop = o("min.u32", o("add.u32", start, per), run)
+        pair0, before0 = _first_behind(e, sums, start)
     else:
-        unit, sp = cta, None
-    kvh = o("rem.u32", unit, kv_heads)
-    ub = o("div.u32", unit, kv_heads)
-    b = o("rem.u32", ub, batch)
-    tile = o("sub.u32", ntile - 1, o("div.u32", ub, batch))     # the longest rows of a sequence first
-    b_len = ldg(at(gptr("p_lens"), wide(b, 4)))
-    b_new = ldg(at(gptr("p_fresh"), wide(b, 4)))
-    c0 = o("mul.lo.u32", tile, tq)
-    e(f"@{e.cond('ge.s32', c0, b_new)} ret;")                   # a tile of padding
-    w = _unit(e, None, b_len, b_new, c0, splits, min_tiles, tq, chunk, cap, window, sinks)
-    c1, pos0, pos1, total, per = w["c1"], w["pos0"], w["pos1"], w["total"], w["per"]
-    ntok = o("add.u32", o("sub.u32", c1, c0), 1)
-    vrows = o("mul.lo.u32", ntok, group)
-    # first row of Q and O in [batch * chunk * heads, dim], and row r's index from it
-    base_row = o("mad.lo.u32", b, chunk, c0)
-    base_row = o("mad.lo.u32", base_row, heads, o("mul.lo.u32", kvh, group))
+        kvh0 = o("rem.u32", cta, kv_heads)
+        S0 = place(o("div.u32", cta, kv_heads))
+        e(f"@!{S0.live} ret;")                                  # a tile of padding
 
-    def row_index(r):
-        """Row r of the CTA's tile as a row of Q and O: token r / group, head r % group."""
-        if group == 1:
-            return o("mad.lo.u32", r, heads, base_row)
-        t_ = o("div.u32", r, group)
-        return o("add.u32", o("mad.lo.u32", t_, heads, base_row), o("sub.u32", r, o("mul.lo.u32", t_, group)))
+    class Segment:
+        """One unit's share of the run, as a role sees it."""
 
-    i0, nb = None, total
-    if splits > 1:
-        i0 = o("mul.lo.u32", sp, per)
-        p_none = e.cond("ge.u32", i0, total)
-        p_later = e.cond("ne.u32", sp, 0)
-        e(f"and.pred {p_none}, {p_none}, {p_later};")
-        e(f"@{p_none} ret;")                                    # no tiles for this part
-        nb = o("min.u32", o("sub.u32", total, i0), per)
-    # a unit that sees no key at all: its rows are 0
-    l_some = e.L("some")
-    e(f"@{e.cond('ne.u32', total, 0)} bra {l_some};")
-    zr, zero = o("mov.u32", tid), o("mov.u32", 0)
-    l_z, l_zd = e.L("zero"), e.L("zerod")
-    e.label(l_z)
-    e(f"@{e.cond('ge.u32', zr, vrows)} bra {l_zd};")
-    za = at(o_ptr, wide(row_index(zr), row_b))
-    for c in range(row_b // 32):
-        e(f"st.global.v8.b32 [{za}+{32 * c}], {{{', '.join([zero] * 8)}}};")
-    e(f"add.u32 {zr}, {zr}, {threads};")
-    e(f"bra {l_z};")
-    e.label(l_zd)
-    e("ret;")
-    e.label(l_some)
+        def __init__(self, P, kvh, i0, nb):
+            self.P, self.w, self.kvh, self.i0, self.nb, self.b = P, P.w, kvh, i0, nb, P.b
+            # first row of Q and O in [batch * chunk * heads, dim]
+            r = o("mad.lo.u32", P.b, chunk, P.c0)
+            self.base_row = o("mad.lo.u32", r, heads, o("mul.lo.u32", kvh, group))
+
+        def row_index(self, r):
+            """Row r of the unit as a row of Q and O: token r / group, head r % group."""
+            if group == 1:
+                return o("mad.lo.u32", r, heads, self.base_row)
+            t_ = o("div.u32", r, group)
+            return o("add.u32", o("mad.lo.u32", t_, heads, self.base_row), o("sub.u32", r, o("mul.lo.u32", t_, group)))
+
+        def tile_of(self, j):
+            """The key tile of the segment's tile number j."""
+            i = o("add.u32", j, self.i0) if self.i0 is not None else j
+            if window is None:
+                return i
+            past = e.cond("ge.u32", i, self.w["st"])
+            return o("selp.u32", o("add.u32", i, self.w["gap"]), i, past)
+
+    def each_segment(tag, body, out):
+        """Emits ``body(segment)`` once, in a loop over the run's segments, and then a branch to ``out``."""
+        if not ctas:
+            body(Segment(S0, kvh0, None, S0.w["total"]))
+            e(f"bra {out};")
+            return
+        pair, before, now = o("mov.u32", pair0), o("mov.u32", before0), o("mov.u32", start)
+        l_find, l_seg = e.L(f"{tag}find"), e.L(f"{tag}seg")
+        e.label(l_find)
+        P = place(pair)
+        behind = o("mad.lo.u32", P.tiles, kv_heads, before)
+        e(f"@{e.cond('lt.u32', now, behind)} bra {l_seg};")
+        e(f"mov.u32 {before}, {behind};")
+        e(f"add.u32 {pair}, {pair}, 1;")
+        e(f"bra {l_find};")
+        e.label(l_seg)
+        off = o("sub.u32", now, before)
+        kvh = o("div.u32", off, P.tiles)
+        i0 = o("sub.u32", off, o("mul.lo.u32", kvh, P.tiles))
+        seg = Segment(P, kvh, i0, o("min.u32", o("sub.u32", P.tiles, i0), o("sub.u32", stop, now)))
+        seg.now = now
+        body(seg)
+        e(f"add.u32 {now}, {now}, {seg.nb};")
+        e(f"@{e.cond('lt.u32', now, stop)} bra {l_find};")
+        e(f"bra {out};")
+
+    if not ctas:
+        # a unit that sees no key at all: its rows are 0
+        l_some = e.L("some")
+        e(f"@{e.cond('ne.u32', S0.w['total'], 0)} bra {l_some};")
+        zs = Segment(S0, kvh0, None, None)
+        zr, zero = o("mov.u32", tid), o("mov.u32", 0)
+        l_z, l_zd = e.L("zero"), e.L("zerod")
+        e.label(l_z)
+        e(f"@{e.cond('ge.u32', zr, S0.vrows)} bra {l_zd};")
+        za = at(o_ptr, wide(zs.row_index(zr), row_b))
+        for c in range(row_b // 32):
+            e(f"st.global.v8.b32 [{za}+{32 * c}], {{{', '.join([zero] * 8)}}};")
+        e(f"add.u32 {zr}, {zr}, {threads};")
+        e(f"bra {l_z};")
+        e.label(l_zd)
+        e("ret;")
+        e.label(l_some)
 
     smem_sym = f"{prefix}paged_smem"
     raw = o("mov.u32", smem_sym)
@@ -250,16 +336,15 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     # bytes: two raw tiles, then one converted K and V
     sRaw = o("add.u32", sKV, 2 * kv_bytes) if quant else None
     bars = o("add.u32", sKV, 2 * kv_bytes + 4 * raw_b if quant else STAGES * kv_bytes)
-    nwarps = o("shr.u32", o("add.u32", vrows, 31), 5)          # softmax warps that have a row
     l_init = e.L("noinit")
     e(f"@{e.cond('ne.u32', tid, 0)} bra {l_init};")
-    e(f"mbarrier.init.shared::cta.b64 [{bars}+{QFULL}], {nwarps};")
+    e(f"mbarrier.init.shared::cta.b64 [{bars}+{QFULL}], 4;")
     for s in range(STAGES):
-        e(f"mbarrier.init.shared::cta.b64 [{bars}+{FULL + 8 * s}], {2 if quant and s >= 2 else 1};")
+        e(f"mbarrier.init.shared::cta.b64 [{bars}+{FULL + 8 * s}], 1;")
         e(f"mbarrier.init.shared::cta.b64 [{bars}+{EMPTY + 8 * s}], {2 if quant and s < 2 else 1};")
     for u in range(2):
         e(f"mbarrier.init.shared::cta.b64 [{bars}+{SFULL + 8 * u}], 1;")
-        e(f"mbarrier.init.shared::cta.b64 [{bars}+{PFULL + 8 * u}], {nwarps};")
+        e(f"mbarrier.init.shared::cta.b64 [{bars}+{PFULL + 8 * u}], 4;")
         e(f"mbarrier.init.shared::cta.b64 [{bars}+{PFREE + 8 * u}], 1;")
     e("fence.mbarrier_init.release.cluster;")
     e("fence.proxy.async.shared::cta;")
@@ -277,24 +362,6 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     l_end, l_mma, l_soft = e.L("end"), e.L("mma"), e.L("soft")
     e(f"@{p_mma} bra {l_mma};")
     e(f"@{e.cond('ge.u32', warp, soft0)} bra {l_soft};")
-    table = gptr("p_table")
-    trow = at(table, wide(b, 4 * max_pages))                   # this sequence's row of the table
-
-    def tile_of(j):
-        """The key tile of the part's tile number j."""
-        i = o("add.u32", j, i0) if i0 is not None else j
-        if window is None:
-            return i
-        past = e.cond("ge.u32", i, w["st"])
-        return o("selp.u32", o("add.u32", i, w["gap"]), i, past)
-
-    def entry(dst, slot, ok):
-        """dst = the page of table slot ``slot`` where ``ok``, or -1 (also for a number outside the pool)."""
-        a_ = at(trow, wide(slot, 4))
-        e(f"mov.u32 {dst}, -1;")
-        e(f"@{ok} ld.global.nc.u32 {dst}, [{a_}];")
-        return dst
-
     def valid(pg):
         return e.cond("lt.u32", pg, pages)
 
@@ -302,17 +369,27 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     l_conv = e.L("conv")
     if quant:
         e(f"@{e.cond('ge.u32', warp, 2)} bra {l_conv};")
-    if True:
-        tk, tv = [o("cvta.param.u64", o("mov.u64", f"p_tm{x}", cls="rd"), cls="rd") for x in "KV"]
-        per_batch = 32 // pieces                               # tiles whose pages one lane-load fetches
-        sub = o("div.u32", lane, pieces) if pieces > 1 else lane
-        piece = o("rem.u32", lane, pieces) if pieces > 1 else None
+    tk, tv = [o("cvta.param.u64", o("mov.u64", f"p_tm{x}", cls="rd"), cls="rd") for x in "KV"]
+    table = gptr("p_table")
+    if quant:
+        ks_ptr, vs_ptr = gptr("p_KS"), gptr("p_VS")
+    per_batch = 32 // pieces                                   # tiles whose pages one lane-load fetches
+    sub = o("div.u32", lane, pieces) if pieces > 1 else lane
+    piece = o("rem.u32", lane, pieces) if pieces > 1 else None
+    cur, nxt = e.r(), e.r()
+    p_l0, p_pc = e.cond("eq.u32", lane, 0), e.cond("lt.u32", lane, pieces)
+    nfull = [o("mov.u32", 0) for _ in range(1 if quant else 2)]       # tiles loaded (16 bits: of K, of V)
+    l_ldone = e.L("ldd")
+    jj_ld = o("mov.u32", 0)                                    # the tile's number in the run
+
+    def loads(S):
+        trow = at(table, wide(S.b, 4 * max_pages))             # this sequence's row of the table
 
         def fetch(dst, j0):
-            """Lane l: the page of piece l % pieces of tile j0 + l / pieces."""
+            """Lane l: the page of piece l % pieces of tile j0 + l / pieces, or -1."""
             j = o("add.u32", j0, sub)
-            ok = e.cond("lt.u32", j, nb)
-            vt = tile_of(j)
+            ok = e.cond("lt.u32", j, S.nb)
+            vt = S.tile_of(j)
             if pieces > 1:
                 slot = o("mad.lo.u32", vt, pieces, piece)
             elif page == BKV:
@@ -321,19 +398,19 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
                 slot = o("div.u32", vt, page // BKV)
             okm = e.cond("lt.u32", slot, max_pages)
             e(f"and.pred {ok}, {ok}, {okm};")
-            return entry(dst, slot, ok)
+            a_ = at(trow, wide(slot, 4))
+            e(f"mov.u32 {dst}, -1;")
+            e(f"@{ok} ld.global.nc.u32 {dst}, [{a_}];")
 
-        cur, nxt = e.r(), e.r()
-        j = o("mov.u32", 0)
+        j, jj = o("mov.u32", 0), jj_ld
         fetch(cur, j)
         fetch(nxt, o("mov.u32", per_batch))
-        armed = [o("mov.u32", 2) for _ in range(STAGES)]
-        l_top, l_done = e.L("ld"), e.L("ldd")
-        p_l0, p_pc = e.cond("eq.u32", lane, 0), e.cond("lt.u32", lane, pieces)
-        e.label(l_top)
-        for u in range(2):
-            e(f"@{e.cond('ge.u32', j, nb)} bra {l_done};")
-            ph = o("and.b32", o("shr.u32", j, 1), 1)
+        l_u, l_seg = [e.L("ld0"), e.L("ld1")], e.L("ldseg")
+        e(f"@{e.cond('ne.u32', o('and.b32', jj, 1), 0)} bra {l_u[1]};")
+        for u in range(2):                                     # ring stages by the tile's parity
+            e.label(l_u[u])
+            e(f"@{e.cond('ge.u32', j, S.nb)} bra {l_seg};")
+            ph = o("and.b32", o("shr.u32", jj, 1), 1)
             at_ = o("and.b32", j, per_batch - 1)
             l_same = e.L("same")
             p_new = e.cond("eq.u32", at_, 0)
@@ -354,34 +431,34 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
                     k_ = o("div.u32", o("add.u32", lane, 32 * h), page)
                     src = o("shfl.sync.idx.b32", cur, o("add.u32", l0, k_), 31, -1)
                 words.append(o("vote.sync.ballot.b32", valid(src), -1))
-            vt = tile_of(j)
+            vt = S.tile_of(j)
             pgc = o("selp.b32", mine, -1, valid(mine))         # outside the pool: the box reads zeros
             roff = o("mul.lo.u32", o("rem.u32", vt, page // BKV), BKV) if page > BKV else 0
-            ma = o("mad.lo.u32", o("and.b32", j, 3), 8, bars)
+            ma = o("mad.lo.u32", o("and.b32", jj, 3), 8, bars)
 
-            def arm(st_, nbytes, first):
+            def arm(st_, nbytes, first, count):
                 """Waits for ring stage st_, notes the mask words with a tile's first box, expects the bytes."""
-                wait_bar_warp(e, f"{bars}+{EMPTY + 8 * st_}", o("xor.b32", ph, 1), err, ERR_LOAD, l_done)
+                wait_bar_warp(e, f"{bars}+{EMPTY + 8 * st_}", o("xor.b32", ph, 1), err, ERR_LOAD, l_ldone)
                 if first:
                     e(f"@{p_l0} st.shared.v2.b32 [{ma}+{KMASK}], {{{words[0]}, {words[1]}}};")
                 e(f"@{p_l0} mbarrier.arrive.expect_tx.shared::cta.b64 _, [{bars}+{FULL + 8 * st_}], {nbytes};")
-                e(f"mov.u32 {armed[st_]}, {ph};")
+                e(f"add.u32 {count}, {count}, 1;")
                 e("bar.warp.sync -1;")
 
             def box(tm, x, dst, st_):
                 if pieces > 1:
-                    dst = o("mad.lo.u32", piece, page * min(128, row_b if not quant else D), dst)
+                    dst = o("mad.lo.u32", piece, page * min(128, D if quant else row_b), dst)
                 e(f"@{p_pc} cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-                  f"[{dst}], [{tm}, {{{x}, {roff}, {kvh}, {pgc}}}], [{bars}+{FULL + 8 * st_}];")
+                  f"[{dst}], [{tm}, {{{x}, {roff}, {S.kvh}, {pgc}}}], [{bars}+{FULL + 8 * st_}];")
 
             if quant:
                 ok_ = valid(mine)
                 here = o("and.b32", o("vote.sync.ballot.b32", ok_, -1), (1 << pieces) - 1)
-                arm(u, o("mad.lo.u32", o("popc.b32", here), 2 * box_rows * 4, 2 * raw_b), True)
+                arm(u, o("mad.lo.u32", o("popc.b32", here), 2 * box_rows * 4, 2 * raw_b), True, nfull[0])
                 e(f"and.pred {ok_}, {ok_}, {p_pc};")
-                for kv, (tm, scp) in enumerate(((tk, gptr("p_KS")), (tv, gptr("p_VS")))):
+                for kv, (tm, scp) in enumerate(((tk, ks_ptr), (tv, vs_ptr))):
                     box(tm, 0, o("add.u32", sRaw, (2 * u + kv) * raw_b), u)
-                    first = o("mad.lo.u32", kvh, page, roff)
+                    first = o("mad.lo.u32", S.kvh, page, roff)
                     off = o("mad.wide.u32", mine, kv_heads * page * 4, wide(first, 4), cls="rd")
                     sd = o("add.u32", bars, RAWSC + (2 * u + kv) * BKV * 4)
                     if pieces > 1:
@@ -390,112 +467,122 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
                       f"{box_rows * 4}, [{bars}+{FULL + 8 * u}];")
             else:
                 for kv, tm in enumerate((tk, tv)):
-                    arm(2 * u + kv, kv_bytes, kv == 0)
+                    arm(2 * u + kv, kv_bytes, kv == 0, nfull[kv])
                     for h in range(boxes):
                         box(tm, 64 * h, o("add.u32", sKV, (2 * u + kv) * kv_bytes + h * kv_box), 2 * u + kv)
             e(f"add.u32 {j}, {j}, 1;")
-        e(f"bra {l_top};")
-        e.label(l_done)
-        for s in range(2 if quant else STAGES):
+            e(f"add.u32 {jj}, {jj}, 1;")
+        e(f"bra {l_u[0]};")
+        e.label(l_seg)
+
+    each_segment("ld", loads, l_ldone)
+    e.label(l_ldone)
+    # wait for what is in flight: use k of a stage completes phase k - 1 (stage u has seen half the tiles)
+    for kv in range(1 if quant else 2):
+        for u in range(2):
             skip = e.L("nodrain")
-            e(f"@{e.cond('eq.u32', armed[s], 2)} bra {skip};")
-            wait_bar_warp(e, f"{bars}+{FULL + 8 * s}", armed[s], err, ERR_DRAIN, skip)
+            uses = o("shr.u32", o("add.u32", nfull[kv], 1 - u), 1)
+            e(f"@{e.cond('eq.u32', uses, 0)} bra {skip};")
+            wait_bar_warp(e, f"{bars}+{FULL + 8 * (u if quant else 2 * u + kv)}", o("and.b32", o("sub.u32", uses, 1), 1), err,
+                          ERR_DRAIN, skip)
             e.label(skip)
-        e(f"bra {l_end};")
+    e(f"bra {l_end};")
     if quant:
         # ---------------------------------------------------------------- bytes to f16 (warps 2 and 3)
         e.label(l_conv)
-        t64 = o("and.b32", tid, 63)
-        quarter, u8_ = o("shr.u32", t64, 3), o("and.b32", t64, 7)
-        piece4, odd = o("and.b32", u8_, 3), o("shr.u32", u8_, 2)
-        rlow = o("xor.b32", o("shl.b32", quarter, 1), o("mul.lo.u32", odd, 5))       # row within 16
+        piece4, odd = o("and.b32", lane, 3), o("and.b32", o("shr.u32", lane, 2), 1)
+        rlow = o("xor.b32", o("shl.b32", o("shr.u32", lane, 3), 1), o("mul.lo.u32", odd, 5))      # row within 8
         c64, c1152 = o("mov.b32", "0x64646464"), o("mov.b32", "0x64806480")
         if D == 128:                                            # 16-byte pieces by the row's low three bits
-            raw_at = [o("mad.lo.u32", o("xor.b32", o("add.u32", piece4, 4 * h), o("and.b32", rlow, 7)), 16,
-                        o("shl.b32", rlow, 7)) for h in range(2)]
+            raw_at = [o("mad.lo.u32", o("xor.b32", o("add.u32", piece4, 4 * h), rlow), 16, o("shl.b32", rlow, 7))
+                      for h in range(2)]
         else:                                                   # 64-byte rows: by bits 1 and 2
             raw_at = [o("mad.lo.u32", o("xor.b32", piece4, o("and.b32", o("shr.u32", rlow, 1), 3)), 16,
                         o("shl.b32", rlow, 6))]
-        out_at = [o("mad.lo.u32", o("xor.b32", o("mad.lo.u32", piece4, 2, i), o("and.b32", rlow, 7)), 16,
-                    o("shl.b32", rlow, 7)) for i in range(2)]
+        out_at = [o("mad.lo.u32", o("xor.b32", o("mad.lo.u32", piece4, 2, i), rlow), 16, o("shl.b32", rlow, 7))
+                  for i in range(2)]
+        # warp 2 converts K, warp 3 V, each as far ahead as the products let it
+        isv = o("sub.u32", warp, 2)
+        raw_kv = o("mad.lo.u32", isv, raw_b, sRaw)
+        out_kv = [o("mad.lo.u32", isv, kv_bytes, o("add.u32", sKV, x)) for x in out_at]
+        kvb = o("mad.lo.u32", isv, 8, o("add.u32", bars, 16))   # K's and V's barriers behind the raw stages'
         p_l0c = e.cond("eq.u32", lane, 0)
         p_w2 = e.cond("eq.u32", warp, 2)
-        vpow = o("mov.b32", "0x00800000")                       # the values' power of two (its f32 bits)
-        j = o("mov.u32", 0)
-        l_top, l_done = e.L("cv"), e.L("cvd")
-        e.label(l_top)
-        e(f"@{e.cond('ge.u32', j, nb)} bra {l_done};")
-        u_, ph, ph1 = o("and.b32", j, 1), o("and.b32", o("shr.u32", j, 1), 1), o("and.b32", j, 1)
-        rb = o("mad.lo.u32", u_, 8, bars)
-        wait_bar_warp(e, f"{rb}+{FULL}", ph, err, ERR_LOAD, l_done)
-        slot_c = o("and.b32", j, 3)
-        l_nosc = e.L("nosc")
-        e(f"@!{p_w2} bra {l_nosc};")
-        # warp 2: the tile's scales, two a lane; those of V over the power, which grows when one reaches twice it
-        rs = o("mad.lo.u32", lane, 8, o("mad.lo.u32", u_, 2 * BKV * 4, bars))
-        ksv, vsv = [e.r("f"), e.r("f")], [e.r("f"), e.r("f")]
-        e(f"ld.shared.v2.f32 {{{ksv[0]}, {ksv[1]}}}, [{rs}+{RAWSC}];")
-        e(f"ld.shared.v2.f32 {{{vsv[0]}, {vsv[1]}}}, [{rs}+{RAWSC + BKV * 4}];")
-        key0c = o("mad.lo.u32", lane, 2, o("shl.b32", tile_of(j), 6))
-        mw = o("mad.lo.u32", slot_c, 8, bars)
-        mw = o("ld.shared.b32", f"[{o('mad.lo.u32', o('shr.u32', lane, 4), 4, mw)}+{KMASK}]")
-        big = o("mov.b32", "0f00000000", cls="f")
-        for i in range(2):
-            bit = o("and.b32", o("shr.u32", mw, o("add.u32", o("shl.b32", o("and.b32", lane, 15), 1), i)), 1)
-            kk = o("add.u32", key0c, i) if i else key0c
-            pk2 = e.cond("lt.u32", kk, w["end"])
-            pk1 = e.cond("ne.u32", bit, 0)
-            e(f"and.pred {pk1}, {pk1}, {pk2};")
-            if window is not None:                              # nor those that no row sees
-                p1, p2 = e.cond("ge.u32", kk, w["lo"]), e.cond("lt.u32", kk, sinks)
-                e(f"or.pred {p1}, {p1}, {p2};")
-                e(f"and.pred {pk1}, {pk1}, {p1};")
-            e(f"@{pk1} max.f32 {big}, {big}, {vsv[i]};")        # a NaN drops out
-        bigb = o("redux.sync.max.u32", o("mov.b32", big), -1)
-        bigb = o("min.u32", o("and.b32", bigb, "0x7F800000"), "0x7E000000")
-        grow = e.cond("gt.u32", bigb, vpow)
-        e(f"@{grow} mov.u32 {vpow}, {bigb};")
-        vinv = o("mov.b32", o("sub.u32", "0x7F000000", vpow), cls="f")
-        sd = o("mad.lo.u32", lane, 8, o("mad.lo.u32", slot_c, BKV * 4, bars))
-        e(f"st.shared.v2.f32 [{sd}+{KSC}], {{{ksv[0]}, {ksv[1]}}};")
-        v0, v1 = (o("mul.f32", x, vinv, cls="f") for x in vsv)
-        e(f"st.shared.v2.f32 [{sd}+{VSC}], {{{v0}, {v1}}};")
-        e(f"@{p_l0c} st.shared.b32 [{o('mad.lo.u32', slot_c, 4, bars)}+{VREF}], {vpow};")
-        e.label(l_nosc)
-        for kv in range(2):
-            src = o("mad.lo.u32", u_, 2 * raw_b, o("add.u32", sRaw, kv * raw_b))
-            words = []
+        jj_cv = o("mov.u32", 0)
+
+        def convert(S):
+            w = S.w
+            vpow = o("mov.b32", "0x00800000")                      # the values' power of two (its f32 bits)
+            j, jj = o("mov.u32", 0), jj_cv
+            l_top, l_seg = e.L("cv"), e.L("cvseg")
+            e.label(l_top)
+            e(f"@{e.cond('ge.u32', j, S.nb)} bra {l_seg};")
+            u_, ph, ph1 = o("and.b32", jj, 1), o("and.b32", o("shr.u32", jj, 1), 1), o("and.b32", jj, 1)
+            rb = o("mad.lo.u32", u_, 8, bars)
+            wait_bar_warp(e, f"{rb}+{FULL}", ph, err, ERR_LOAD, l_end)
+            slot_c = o("and.b32", jj, 3)
+            l_nosc = e.L("nosc")
+            e(f"@!{p_w2} bra {l_nosc};")
+            # warp 2: the tile's scales, two a lane; those of V over the power, which grows when one reaches twice it
+            rs = o("mad.lo.u32", lane, 8, o("mad.lo.u32", u_, 2 * BKV * 4, bars))
+            ksv, vsv = [e.r("f"), e.r("f")], [e.r("f"), e.r("f")]
+            e(f"ld.shared.v2.f32 {{{ksv[0]}, {ksv[1]}}}, [{rs}+{RAWSC}];")
+            e(f"ld.shared.v2.f32 {{{vsv[0]}, {vsv[1]}}}, [{rs}+{RAWSC + BKV * 4}];")
+            key0c = o("mad.lo.u32", lane, 2, o("shl.b32", S.tile_of(j), 6))
+            mw = o("mad.lo.u32", slot_c, 8, bars)
+            mw = o("ld.shared.b32", f"[{o('mad.lo.u32', o('shr.u32', lane, 4), 4, mw)}+{KMASK}]")
+            big = o("mov.b32", "0f00000000", cls="f")
+            for i in range(2):
+                bit = o("and.b32", o("shr.u32", mw, o("add.u32", o("shl.b32", o("and.b32", lane, 15), 1), i)), 1)
+                kk = o("add.u32", key0c, i) if i else key0c
+                pk2 = e.cond("lt.u32", kk, w["end"])
+                pk1 = e.cond("ne.u32", bit, 0)
+                e(f"and.pred {pk1}, {pk1}, {pk2};")
+                if window is not None:                              # nor those that no row sees
+                    p1, p2 = e.cond("ge.u32", kk, w["lo"]), e.cond("lt.u32", kk, sinks)
+                    e(f"or.pred {p1}, {p1}, {p2};")
+                    e(f"and.pred {pk1}, {pk1}, {p1};")
+                e(f"@{pk1} max.f32 {big}, {big}, {vsv[i]};")        # a NaN drops out
+            bigb = o("redux.sync.max.u32", o("mov.b32", big), -1)
+            bigb = o("min.u32", o("and.b32", bigb, "0x7F800000"), "0x7E000000")
+            grow = e.cond("gt.u32", bigb, vpow)
+            e(f"@{grow} mov.u32 {vpow}, {bigb};")
+            vinv = o("mov.b32", o("sub.u32", "0x7F000000", vpow), cls="f")
+            sd = o("mad.lo.u32", lane, 8, o("mad.lo.u32", slot_c, BKV * 4, bars))
+            e(f"st.shared.v2.f32 [{sd}+{KSC}], {{{ksv[0]}, {ksv[1]}}};")
+            v0, v1 = (o("mul.f32", x, vinv, cls="f") for x in vsv)
+            e(f"st.shared.v2.f32 [{sd}+{VSC}], {{{v0}, {v1}}};")
+            e(f"@{p_l0c} st.shared.b32 [{o('mad.lo.u32', slot_c, 4, bars)}+{VREF}], {vpow};")
+            e.label(l_nosc)
+            src = o("mad.lo.u32", u_, 2 * raw_b, raw_kv)
             for h in range(boxes):
-                for k in range(4):
+                words = []
+                for k in range(8):
                     d_ = [e.r() for _ in range(4)]
-                    e(f"ld.shared.v4.b32 {{{', '.join(d_)}}}, [{o('add.u32', src, raw_at[h])}+{16 * k * D}];")
+                    e(f"ld.shared.v4.b32 {{{', '.join(d_)}}}, [{o('add.u32', src, raw_at[h])}+{8 * k * D}];")
                     words.append(d_)
-            wait_bar_warp(e, f"{bars}+{EMPTY + 8 * (2 + kv)}", o("xor.b32", ph1, 1), err, ERR_LOAD, l_done)
-            dsts = [o("add.u32", o("add.u32", sKV, kv * kv_bytes), x) for x in out_at]
-            for h in range(boxes):
-                for k in range(4):
+                if h == 0:
+                    wait_bar_warp(e, f"{kvb}+{EMPTY}", o("xor.b32", ph1, 1), err, ERR_LOAD, l_end)
+                for k in range(8):
                     out = [o("sub.rn.f16x2", o("prmt.b32", x, c64, sel), c1152)
-                           for x in words[4 * h + k] for sel in ("0x4140", "0x4342")]
+                           for x in words[k] for sel in ("0x4140", "0x4342")]
                     for i in range(2):
-                        e(f"st.shared.v4.b32 [{dsts[i]}+{h * kv_box + 16 * k * 128}], "
+                        e(f"st.shared.v4.b32 [{out_kv[i]}+{h * kv_box + 8 * k * 128}], "
                           f"{{{', '.join(out[4 * i:4 * i + 4])}}};")
             e("fence.proxy.async.shared::cta;")
             e("bar.warp.sync -1;")
-            if kv:
-                e(f"@{p_l0c} mbarrier.arrive.shared::cta.b64 _, [{rb}+{EMPTY}];")
-            e(f"@{p_l0c} mbarrier.arrive.shared::cta.b64 _, [{bars}+{FULL + 8 * (2 + kv)}];")
-        e(f"add.u32 {j}, {j}, 1;")
-        e(f"bra {l_top};")
-        e.label(l_done)
-        e(f"bra {l_end};")
+            e(f"@{p_l0c} mbarrier.arrive.shared::cta.b64 _, [{rb}+{EMPTY}];")
+            e(f"@{p_l0c} mbarrier.arrive.shared::cta.b64 _, [{kvb}+{FULL}];")
+            e(f"add.u32 {j}, {j}, 1;")
+            e(f"add.u32 {jj}, {jj}, 1;")
+            e(f"bra {l_top};")
+            e.label(l_seg)
+
+        each_segment("cv", convert, l_end)
 
     # ------------------------------------------------------------------ MMA issue (one thread)
     e.label(l_mma)
     e(f"@{e.cond('ne.u32', lane, 0)} bra {l_end};")
-    l_mdone = e.L("mdone")
-    zero2 = o("mov.u32", 0)
-    wait_bar(e, f"{bars}+{QFULL}", zero2, err, ERR_MMA, l_mdone)
-    e("tcgen05.fence::after_thread_sync;")
     iqk, ipv = o("mov.u32", idesc_qk), o("mov.u32", idesc_pv)
     ptrue, pfalse = e.cond("eq.u32", lane, lane), e.cond("ne.u32", lane, lane)
     khi, vhi = o("mov.b64", kdesc_hi, cls="rd"), o("mov.b64", vdesc_hi, cls="rd")
@@ -512,13 +599,13 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     stg = [o("add.u32", sKV, s * kv_bytes) for s in range(2 if quant else STAGES)]
     kd = [desc(stg[0 if quant else 2 * u], khi) for u in range(2)]
     vd = [desc(stg[1 if quant else 2 * u + 1], vhi) for u in range(2)]
-    scol = [o("add.u32", taddr, S0 + BKV * u) for u in range(2)]
+    scol = [o("add.u32", taddr, SCOL + BKV * u) for u in range(2)]
 
     def commit(off):
         e(f"tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [{bars}+{off}];")
 
     def ring(st_, ph):
-        wait_bar(e, f"{bars}+{FULL + 8 * st_}", ph, err, ERR_MMA, l_mdone)
+        wait_bar(e, f"{bars}+{FULL + 8 * st_}", ph, err, ERR_MMA, l_end)
         e("tcgen05.fence::after_thread_sync;")
 
     def qk(u):
@@ -528,354 +615,377 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         commit(EMPTY + 8 * ring_k[u])
         commit(SFULL + 8 * u)
 
-    j = o("mov.u32", 0)
-    ring(ring_k[0], zero2)
-    qk(0)
-    l_mg = e.L("mg")
-    e.label(l_mg)
-    for u in range(2):                                         # tile j = 2 g + u
-        ph = o("and.b32", o("shr.u32", j, 1), 1)
-        jn = o("add.u32", j, 1)
-        have = e.cond("lt.u32", jn, nb)
-        l_nok = e.L("nok")
-        e(f"@!{have} bra {l_nok};")
-        ring(ring_k[1 - u], str(1 - u) if quant else ph if u == 0 else o("xor.b32", ph, 1))
-        qk(1 - u)
-        e.label(l_nok)
-        ring(ring_v[u], str(u) if quant else ph)
-        wait_bar(e, f"{bars}+{PFULL + 8 * u}", ph, err, ERR_MMA, l_mdone)
+    jj_m, segs = o("mov.u32", 0), o("mov.u32", 0)
+
+    def phase_of(x):
+        """The phase of a ring barrier at tile x of the run: of two stages, or of one (bytes: the tile's parity)."""
+        return o("and.b32", x if quant else o("shr.u32", x, 1), 1)
+
+    def issue(S):
+        j, jj = o("mov.u32", 0), jj_m
+        wait_bar(e, f"{bars}+{QFULL}", o("and.b32", segs, 1), err, ERR_MMA, l_end)
         e("tcgen05.fence::after_thread_sync;")
-        pacc = e.cond("ne.u32", j, 0)
-        for part in range(1 if p_f16 else 2):
-            for k in range(BKV // 16):
-                e(f"tcgen05.mma.cta_group::1.kind::f16 [{taddr}], [{scol[u]}+{BKV // 2 * part + 8 * k}], "
-                  f"{plus(vd[u], 2048 * k)}, {ipv}, {pacc if k == 0 and part == 0 else ptrue};")
-        commit(EMPTY + 8 * ring_v[u])
-        commit(PFREE + 8 * u)
-        e(f"@!{have} bra {l_mdone};")
-        e(f"mov.u32 {j}, {jn};")
-    e(f"bra {l_mg};")
-    e.label(l_mdone)
-    e(f"bra {l_end};")
+        e(f"add.u32 {segs}, {segs}, 1;")
+        l_in, l_u, l_seg = [e.L("in0"), e.L("in1")], [e.L("mg0"), e.L("mg1")], e.L("mseg")
+        e(f"@{e.cond('ne.u32', o('and.b32', jj, 1), 0)} bra {l_in[1]};")
+        for u in range(2):
+            e.label(l_in[u])
+            ring(ring_k[u], phase_of(jj))
+            qk(u)
+            e(f"bra {l_u[u]};")
+        for u in range(2):                                     # a tile of parity u
+            e.label(l_u[u])
+            jn, jjn = o("add.u32", j, 1), o("add.u32", jj, 1)
+            have = e.cond("lt.u32", jn, S.nb)
+            l_nok = e.L("nok")
+            e(f"@!{have} bra {l_nok};")
+            ring(ring_k[1 - u], phase_of(jjn))
+            qk(1 - u)
+            e.label(l_nok)
+            ring(ring_v[u], phase_of(jj))
+            wait_bar(e, f"{bars}+{PFULL + 8 * u}", o("and.b32", o("shr.u32", jj, 1), 1), err, ERR_MMA, l_end)
+            e("tcgen05.fence::after_thread_sync;")
+            pacc = e.cond("ne.u32", j, 0)
+            for part in range(1 if p_f16 else 2):
+                for k in range(BKV // 16):
+                    e(f"tcgen05.mma.cta_group::1.kind::f16 [{taddr}], [{scol[u]}+{BKV // 2 * part + 8 * k}], "
+                      f"{plus(vd[u], 2048 * k)}, {ipv}, {pacc if k == 0 and part == 0 else ptrue};")
+            commit(EMPTY + 8 * ring_v[u])
+            commit(PFREE + 8 * u)
+            e(f"mov.u32 {j}, {jn};")
+            e(f"mov.u32 {jj}, {jjn};")
+            e(f"@!{have} bra {l_seg};")
+        e(f"bra {l_u[0]};")
+        e.label(l_seg)
+
+    each_segment("m", issue, l_end)
 
     # ------------------------------------------------------------------ softmax (one row a thread)
     e.label(l_soft)
     quad = o("and.b32", warp, 3)                               # the TMEM lanes a warp reaches
-    e(f"@{e.cond('ge.u32', quad, nwarps)} bra {l_end};")
     rowl = o("mad.lo.u32", quad, 32, lane)
-    # Q: each warp its own 32 rows, 16 bytes a lane, into the swizzled K-major tile
     q_ptr = gptr("p_Q")
     per_row = row_b // 16                                      # lanes a row takes
     qsub, qch = o("div.u32", lane, per_row), o("rem.u32", lane, per_row)
     passes = 32 * per_row // 32
     recast = quant and dtype == "bf16"
-    for p0 in range(0, passes, 8):
-        ws, rr_ = [], []
-        for p_ in range(p0, min(passes, p0 + 8)):
-            r_ = o("mad.lo.u32", quad, 32, o("add.u32", qsub, p_ * (32 // per_row)))
-            ok = e.cond("lt.u32", r_, vrows)
-            qa = at(at(q_ptr, wide(row_index(r_), row_b)), wide(qch, 16))
-            d_ = [o("mov.b32", 0) for _ in range(4)]
-            e(f"@{ok} ld.global.nc.v4.b32 {{{', '.join(d_)}}}, [{qa}];")
-            ws.append(d_)
-            rr_.append(r_)
-        for d_, r_ in zip(ws, rr_):
-            if recast:
-                # the row's largest number to 2^14 by a power of two (at most 2^40), then f16: see above
-                big = None
-                for x in d_:
-                    a_ = o("and.b32", x, "0x7FFF7FFF")
-                    big = a_ if big is None else o("max.u16x2", big, a_)
-                big = o("max.u32", o("and.b32", big, 65535), o("shr.u32", big, 16))
-                k_ = 1
-                while k_ < per_row:
-                    big = o("max.u32", big, o("shfl.sync.bfly.b32", big, k_, 31, -1))
-                    k_ *= 2
-                ex = o("min.s32", o("sub.s32", 127 + 14, o("shr.u32", big, 7)), 40)
-                up = o("shl.b32", o("add.s32", ex, 127), 23, cls="f")
-                down = o("shl.b32", o("sub.s32", 127, ex), 23, cls="f")
-                qsa = o("mad.lo.u32", r_, 4, bars)
-                e(f"@{e.cond('eq.u32', qch, 0)} st.shared.f32 [{qsa}+{QSC}], {o('mul.f32', down, cscale, cls='f')};")
-                d_ = [o("cvt.rn.f16x2.f32", o("mul.f32", o("and.b32", x, -65536, cls="f"), up, cls="f"),
-                        o("mul.f32", o("shl.b32", x, 16, cls="f"), up, cls="f")) for x in d_]
-            box = o("shr.u32", qch, 3)
-            ch = o("xor.b32", o("and.b32", qch, 7), o("and.b32", r_, 7))
-            sa = o("mad.lo.u32", box, q_box, sQ)
-            sa = o("mad.lo.u32", r_, 128, sa)
-            sa = o("mad.lo.u32", ch, 16, sa)
-            e(f"st.shared.v4.b32 [{sa}], {{{', '.join(d_)}}};")
-    e("fence.proxy.async.shared::cta;")
-    e("bar.warp.sync -1;")
     p_l0s = e.cond("eq.u32", lane, 0)
-    e(f"@{p_l0s} mbarrier.arrive.shared::cta.b64 _, [{bars}+{QFULL}];")
     lanebase = o("add.u32", o("shl.b32", quad, 21), taddr)
-    tok = o("div.u32", rowl, group) if group > 1 else rowl
-    pos = o("min.s32", o("add.s32", pos0, tok), pos1)          # rows without a token: the last one's
-    cf = o("mov.b32", cscale, cls="f")                          # scale * log2(e) for this row's scores
-    if recast:
-        e(f"ld.shared.f32 {cf}, [{o('mad.lo.u32', rowl, 4, bars)}+{QSC}];")
-    vref = o("mov.b32", "0f00800000", cls="f") if quant else None
     s_ = [e.r("f") for _ in range(BKV)]
-    mref, lsum = o("mov.b32", "0fFF800000", cls="f"), o("mov.b32", "0f00000000", cls="f")
-    j = o("mov.u32", 0)
-    l_sj, l_sdone, l_noepi = e.L("sj"), e.L("sdone"), e.L("noepi")
-    e.label(l_sj)
-    e(f"@{e.cond('ge.u32', j, nb)} bra {l_sdone};")
-    buf = o("and.b32", j, 1)
-    ph = o("and.b32", o("shr.u32", j, 1), 1)
-    bb = o("mad.lo.u32", buf, 8, bars)
-    sc_col = o("add.u32", o("mad.lo.u32", buf, BKV, lanebase), S0)
-    key0 = o("shl.b32", tile_of(j), 6)
-    wait_bar_warp(e, f"{bb}+{SFULL}", ph, err, ERR_SOFTMAX, l_noepi)
-    e("tcgen05.fence::after_thread_sync;")
-    for c in range(BKV // 32):
-        e(f"tcgen05.ld.sync.aligned.32x32b.x32.b32 {{{', '.join(s_[32 * c:32 * c + 32])}}}, [{sc_col}+{32 * c}];")
-    slot_a = o("and.b32", j, 3)
-    ma = o("mad.lo.u32", slot_a, 8, bars)
-    km = [e.r(), e.r()]
-    e(f"ld.shared.v2.b32 {{{km[0]}, {km[1]}}}, [{ma}+{KMASK}];")
-    e("tcgen05.wait::ld.sync.aligned;")
-    sca = None
-    if quant:
-        sca = o("mad.lo.u32", slot_a, BKV * 4, bars)
-        vnew = o("ld.shared.f32", f"[{o('mad.lo.u32', slot_a, 4, bars)}+{VREF}]", cls="f")
-
-        def times(off):
-            """The row times 64 numbers in shared memory, two at a time."""
-            for c in range(0, BKV, 4):
-                kp = [e.r("rd"), e.r("rd")]
-                e(f"ld.shared.v2.b64 {{{kp[0]}, {kp[1]}}}, [{sca}+{off + 4 * c}];")
-                for i in range(2):
-                    x0, x1 = s_[c + 2 * i], s_[c + 2 * i + 1]
-                    xp = e.r("rd")
-                    e(f"mov.b64 {xp}, {{{x0}, {x1}}};")
-                    e(f"mul.rn.f32x2 {xp}, {xp}, {kp[i]};")
-                    e(f"mov.b64 {{{x0}, {x1}}}, {xp};")
-        times(KSC)
-    # the keys of the tile this row sees, as 64 bits: up to its own position, inside the window or among
-    # the sinks, on a page.  Tiles that every row of the warp sees whole skip all of it.
-    lim = o("sub.s32", pos, key0)
-    p_all = e.cond("ge.s32", lim, BKV - 1)
-    kand = o("and.b32", km[0], km[1])
-    pk_ = e.cond("eq.s32", kand, -1)
-    e(f"and.pred {p_all}, {p_all}, {pk_};")
-    wl = sk = None
-    if window is not None:
-        wl = o("sub.s32", o("sub.s32", pos, window), key0)      # keys up to here lie before the window
-        sk = o("sub.s32", sinks, key0)                          # keys below here are sinks
-        pw_ = e.cond("lt.s32", wl, 0)
-        ps_ = e.cond("ge.s32", sk, BKV)
-        e(f"or.pred {pw_}, {pw_}, {ps_};")
-        e(f"and.pred {p_all}, {p_all}, {pw_};")
-    v_all = o("vote.sync.all.pred", p_all, -1, cls="p")
-    l_seen = e.L("seen")
-    m0, m1 = o("mov.b32", -1), o("mov.b32", -1)
-    e(f"@{v_all} bra {l_seen};")
-
-    def below(n, cls="rd"):
-        """The bits below n (clamped to 0..64)."""
-        k_ = o("sub.s32", 64, o("min.s32", o("max.s32", n, 0), 64))
-        return o("shr.u64", o("mov.b64", -1, cls="rd"), k_, cls="rd")        # a shift by 64 leaves 0
-
-    bits = below(o("add.s32", o("min.s32", lim, BKV), 1))
-    if window is not None:
-        inside = o("not.b64", below(o("add.s32", wl, 1)), cls="rd")
-        inside = o("or.b64", inside, below(sk), cls="rd")
-        bits = o("and.b64", bits, inside, cls="rd")
-    pages_ = e.r("rd")
-    e(f"mov.b64 {pages_}, {{{km[0]}, {km[1]}}};")
-    bits = o("and.b64", bits, pages_, cls="rd")
-    e(f"mov.b64 {{{m0}, {m1}}}, {bits};")
-    for c in range(BKV):
-        t_ = o("and.b32", (m0, m1)[c // 32], 1 << (c % 32) if c % 32 < 31 else -(1 << 31))
-        e(f"@{e.cond('eq.u32', t_, 0)} mov.b32 {s_[c]}, 0fFF800000;")
-    e.label(l_seen)
-    if not quant:
-        # rows of V that no row of this CTA sees (past its last token, or between sinks and window) may
-        # hold anything: zero them before the product multiplies them by P = 0
-        l_vok = e.L("vok")
-        vlim = o("sub.s32", pos1, key0)
-        pv_ = e.cond("ge.s32", vlim, BKV - 1)
-        if window is not None:
-            lo_k = o("sub.s32", w["lo"], key0)
-            p1_, p2_ = e.cond("le.s32", lo_k, 0), e.cond("ge.s32", sk, BKV)
-            e(f"or.pred {p1_}, {p1_}, {p2_};")
-            e(f"and.pred {pv_}, {pv_}, {p1_};")
-        e(f"@{pv_} bra {l_vok};")                               # the same for every thread
-        wait_bar_warp(e, f"{o('mad.lo.u32', buf, 16, bars)}+{FULL + 8}", ph, err, ERR_SOFTMAX, l_noepi)
-        va = o("mad.lo.u32", buf, 2 * kv_bytes, o("add.u32", sKV, kv_bytes))
-        z_ = o("mov.b32", 0)
-        for h in range(2):
-            r_ = o("add.u32", lane, 32 * h)
-            pz = e.cond("gt.s32", r_, vlim)
-            if window is not None:
-                pa, pb = e.cond("lt.s32", r_, lo_k), e.cond("ge.s32", r_, sk)
-                e(f"and.pred {pa}, {pa}, {pb};")
-                e(f"or.pred {pz}, {pz}, {pa};")
-            ra = o("mad.lo.u32", r_, 128, va)
-            for box in range(boxes):
-                for i in range(8):
-                    e(f"@{pz} st.shared.v4.b32 [{ra}+{box * kv_box + 16 * i}], {{{z_}, {z_}, {z_}, {z_}}};")
-        e("fence.proxy.async.shared::cta;")
-        e.label(l_vok)
-    # the row's maximum: 8 chains of three-input maxima
-    lvl = [e.r("f") for _ in range(8)]
-    for k in range(8):
-        col = list(range(k, BKV, 8))
-        e(f"max.f32 {lvl[k]}, {s_[col[0]]}, {s_[col[1]]}, {s_[col[2]]};")
-        e(f"max.f32 {lvl[k]}, {lvl[k]}, {s_[col[3]]}, {s_[col[4]]};")
-        e(f"max.f32 {lvl[k]}, {lvl[k]}, {s_[col[5]]}, {s_[col[6]]};")
-        e(f"max.f32 {lvl[k]}, {lvl[k]}, {s_[col[7]]};")
-    e(f"max.f32 {lvl[0]}, {lvl[0]}, {lvl[1]}, {lvl[2]};")
-    e(f"max.f32 {lvl[3]}, {lvl[3]}, {lvl[4]}, {lvl[5]};")
-    e(f"max.f32 {lvl[6]}, {lvl[6]}, {lvl[7]};")
-    e(f"max.f32 {lvl[0]}, {lvl[0]}, {lvl[3]}, {lvl[6]};")
-    mnew = o("max.f32", mref, o("mul.f32", lvl[0], cf, cls="f"), cls="f")
-    alpha = o("mov.b32", "0f3F800000", cls="f")
-    l_first, l_after = e.L("first"), e.L("after")
-    anyneed = e.cond("ne.u32", lane, lane)
-    e(f"@{e.cond('eq.u32', j, 0)} bra {l_first};")
-    need = e.cond("gt.f32", mnew, o("add.f32", mref, _f32(RESCALE), cls="f"))
-    if quant:
-        e(f"or.pred {need}, {need}, {e.cond('ne.f32', vnew, vref)};")           # the same for every row
-    e(f"vote.sync.any.pred {anyneed}, {need}, -1;")
-    e(f"@!{anyneed} bra {l_after};")
-    e(f"ex2.approx.ftz.f32 {alpha}, {o('sub.f32', mref, mnew, cls='f')};")
-    # a row that has seen nothing yet while another of the warp rescales: -inf - -inf must not make a NaN
-    e(f"@{e.cond('eq.f32', mnew, '0fFF800000')} mov.b32 {alpha}, 0f3F800000;")
-    e(f"mul.f32 {lsum}, {lsum}, {alpha};")
-    if quant:
-        inv_ = o("mov.b32", o("sub.u32", "0x7F000000", o("mov.b32", vnew)), cls="f")
-        e(f"mul.f32 {alpha}, {alpha}, {o('mul.f32', vref, inv_, cls='f')};")
-    e.label(l_first)
-    e(f"mov.b32 {mref}, {mnew};")
-    if quant:
-        e(f"mov.b32 {vref}, {vnew};")
-    e.label(l_after)
-    lift = 0.0 if not p_f16 else QUANT_LIFT if quant else F16_LIFT
-    negm = o("sub.f32", o("mov.b32", _f32(lift), cls="f"), mref, cls="f")
-    e(f"@{e.cond('eq.f32', mref, '0fFF800000')} mov.b32 {negm}, 0f00000000;")
-    cp2, np2 = e.r("rd"), e.r("rd")
-    e(f"mov.b64 {cp2}, {{{cf}, {cf}}};")
-    e(f"mov.b64 {np2}, {{{negm}, {negm}}};")
-    acc = [o("mov.b64", 0, cls="rd") for _ in range(2)]
-
-    def exps(cols):
-        for k, idx in enumerate(cols[::2]):
-            x0, x1 = s_[idx], s_[idx + 1]
-            xp, ep = e.r("rd"), e.r("rd")
-            e(f"mov.b64 {xp}, {{{x0}, {x1}}};")
-            e(f"fma.rn.f32x2 {xp}, {xp}, {cp2}, {np2};")
-            e(f"mov.b64 {{{x0}, {x1}}}, {xp};")
-            e(f"ex2.approx.ftz.f32 {x0}, {x0};")
-            e(f"ex2.approx.ftz.f32 {x1}, {x1};")
-            e(f"mov.b64 {ep}, {{{x0}, {x1}}};")
-            e(f"add.rn.f32x2 {acc[k & 1]}, {acc[k & 1]}, {ep};")
-
-    if p_f16:
-        def pack(cols):
-            hw = [o("cvt.rn.f16x2.f32", s_[c + 1], s_[c]) for c in cols[::2]]
-            e(f"tcgen05.st.sync.aligned.32x32b.x16.b32 [{sc_col}+{cols[0] // 2}], {{{', '.join(hw)}}};")
-        if quant:
-            exps(list(range(BKV)))
-            times(VSC)
-            # a masked key's scale may be NaN: its weight is 0 whatever it was multiplied by
-            l_nz = e.L("nz")
-            e(f"@{v_all} bra {l_nz};")
-            for c in range(BKV):
-                t_ = o("and.b32", (m0, m1)[c // 32], 1 << (c % 32) if c % 32 < 31 else -(1 << 31))
-                e(f"@{e.cond('eq.u32', t_, 0)} mov.b32 {s_[c]}, 0f00000000;")
-            e.label(l_nz)
-        for h in range(2):
-            cols = list(range(32 * h, 32 * h + 32))
-            if not quant:
-                exps(cols)
-            pack(cols)
-    else:
-        exps(list(range(BKV)))
-        for h in range(2):
-            hi, lo = [], []
-            for c in range(32 * h, 32 * h + 32, 2):
-                hi.append(o("prmt.b32", s_[c], s_[c + 1], "0x7632"))
-                d0 = o("sub.f32", s_[c], o("and.b32", s_[c], -65536, cls="f"), cls="f")
-                d1 = o("sub.f32", s_[c + 1], o("and.b32", s_[c + 1], -65536, cls="f"), cls="f")
-                lo.append(o("prmt.b32", d0, d1, "0x7632"))
-            e(f"tcgen05.st.sync.aligned.32x32b.x16.b32 [{sc_col}+{16 * h}], {{{', '.join(hi)}}};")
-            e(f"tcgen05.st.sync.aligned.32x32b.x16.b32 [{sc_col}+{32 + 16 * h}], {{{', '.join(lo)}}};")
-    parts = [e.r("f") for _ in range(4)]
-    e(f"mov.b64 {{{parts[0]}, {parts[1]}}}, {acc[0]};")
-    e(f"mov.b64 {{{parts[2]}, {parts[3]}}}, {acc[1]};")
-    psum = o("add.f32", o("add.f32", parts[0], parts[1], cls="f"), o("add.f32", parts[2], parts[3], cls="f"), cls="f")
-    e(f"add.f32 {lsum}, {lsum}, {psum};")
-    # the lazy rescale of O, once the previous product has completed
-    l_nore = e.L("norescale")
-    e(f"@!{anyneed} bra {l_nore};")
-
-    def pv_done(k, code, bail):
-        br = o("mad.lo.u32", o("and.b32", k, 1), 8, bars)
-        wait_bar_warp(e, f"{br}+{PFREE}", o("and.b32", o("shr.u32", k, 1), 1), err, code, bail)
-
-    pv_done(o("sub.u32", j, 1), ERR_SOFTMAX, l_noepi)
-    e("tcgen05.fence::after_thread_sync;")
-    for c in range(D // 32):
-        regs = s_[:32]
-        e(f"tcgen05.ld.sync.aligned.32x32b.x32.b32 {{{', '.join(regs)}}}, [{lanebase}+{32 * c}];")
-        e("tcgen05.wait::ld.sync.aligned;")
-        for r_ in regs:
-            e(f"mul.f32 {r_}, {r_}, {alpha};")
-        e(f"tcgen05.st.sync.aligned.32x32b.x32.b32 [{lanebase}+{32 * c}], {{{', '.join(regs)}}};")
-    e.label(l_nore)
-    e("tcgen05.wait::st.sync.aligned;")
-    e("tcgen05.fence::before_thread_sync;")
-    e("bar.warp.sync -1;")
-    e(f"@{p_l0s} mbarrier.arrive.shared::cta.b64 _, [{bb}+{PFULL}];")
-    e(f"add.u32 {j}, {j}, 1;")
-    e(f"bra {l_sj};")
-
-    # epilogue: after the last product, O / l as the output type, or the part's O, m and l in f32
-    e.label(l_sdone)
-    pv_done(o("sub.u32", nb, 1), ERR_EPILOGUE, l_noepi)
-    e("tcgen05.fence::after_thread_sync;")
-    p_row = e.cond("lt.u32", rowl, vrows)
-    l_part = e.L("part")
-    if splits > 1:
-        e(f"@{e.cond('gt.u32', total, per)} bra {l_part};")
-    p_zero = e.cond("eq.f32", lsum, "0f00000000")
-    inv = o("rcp.rn.f32", o("selp.f32", "0f3F800000", lsum, p_zero, cls="f"), cls="f")
-    if quant:
-        e(f"mul.f32 {inv}, {inv}, {vref};")
-    oa = at(o_ptr, wide(row_index(rowl), row_b))
+    jj_s = o("mov.u32", 0)
     out_cvt = "cvt.rn.f16x2.f32" if dtype == "f16" else "cvt.rn.bf16x2.f32"
-    for c in range(D // 32):
-        regs = s_[:32]
-        e(f"tcgen05.ld.sync.aligned.32x32b.x32.b32 {{{', '.join(regs)}}}, [{lanebase}+{32 * c}];")
+    lift = 0.0 if not p_f16 else QUANT_LIFT if quant else F16_LIFT
+
+    def softmax(S):
+        w, pos0, pos1, vrows = S.w, S.w["pos0"], S.w["pos1"], S.P.vrows
+        # Q: each warp its own 32 rows, 16 bytes a lane, into the swizzled K-major tile
+        for p0 in range(0, passes, 8):
+            ws, rr_ = [], []
+            for p_ in range(p0, min(passes, p0 + 8)):
+                r_ = o("mad.lo.u32", quad, 32, o("add.u32", qsub, p_ * (32 // per_row)))
+                ok = e.cond("lt.u32", r_, vrows)
+                qa = at(at(q_ptr, wide(S.row_index(r_), row_b)), wide(qch, 16))
+                d_ = [o("mov.b32", 0) for _ in range(4)]
+                e(f"@{ok} ld.global.nc.v4.b32 {{{', '.join(d_)}}}, [{qa}];")
+                ws.append(d_)
+                rr_.append(r_)
+            for d_, r_ in zip(ws, rr_):
+                if recast:
+                    # the row's largest number to 2^14 by a power of two (at most 2^40), then f16: see above
+                    big = None
+                    for x in d_:
+                        a_ = o("and.b32", x, "0x7FFF7FFF")
+                        big = a_ if big is None else o("max.u16x2", big, a_)
+                    big = o("max.u32", o("and.b32", big, 65535), o("shr.u32", big, 16))
+                    k_ = 1
+                    while k_ < per_row:
+                        big = o("max.u32", big, o("shfl.sync.bfly.b32", big, k_, 31, -1))
+                        k_ *= 2
+                    ex = o("min.s32", o("sub.s32", 127 + 14, o("shr.u32", big, 7)), 40)
+                    up = o("shl.b32", o("add.s32", ex, 127), 23, cls="f")
+                    down = o("shl.b32", o("sub.s32", 127, ex), 23, cls="f")
+                    qsa = o("mad.lo.u32", r_, 4, bars)
+                    e(f"@{e.cond('eq.u32', qch, 0)} st.shared.f32 [{qsa}+{QSC}], {o('mul.f32', down, cscale, cls='f')};")
+                    d_ = [o("cvt.rn.f16x2.f32", o("mul.f32", o("and.b32", x, -65536, cls="f"), up, cls="f"),
+                            o("mul.f32", o("shl.b32", x, 16, cls="f"), up, cls="f")) for x in d_]
+                box = o("shr.u32", qch, 3)
+                ch = o("xor.b32", o("and.b32", qch, 7), o("and.b32", r_, 7))
+                sa = o("mad.lo.u32", box, q_box, sQ)
+                sa = o("mad.lo.u32", r_, 128, sa)
+                sa = o("mad.lo.u32", ch, 16, sa)
+                e(f"st.shared.v4.b32 [{sa}], {{{', '.join(d_)}}};")
+        e("fence.proxy.async.shared::cta;")
+        e("bar.warp.sync -1;")
+        e(f"@{p_l0s} mbarrier.arrive.shared::cta.b64 _, [{bars}+{QFULL}];")
+        tok = o("div.u32", rowl, group) if group > 1 else rowl
+        pos = o("min.s32", o("add.s32", pos0, tok), pos1)          # rows without a token: the last one's
+        cf = o("mov.b32", cscale, cls="f")                          # scale * log2(e) for this row's scores
+        if recast:
+            e(f"ld.shared.f32 {cf}, [{o('mad.lo.u32', rowl, 4, bars)}+{QSC}];")
+        vref = o("mov.b32", "0f00800000", cls="f") if quant else None
+        mref, lsum = o("mov.b32", "0fFF800000", cls="f"), o("mov.b32", "0f00000000", cls="f")
+        j, jj = o("mov.u32", 0), jj_s
+        l_sj, l_sdone, l_noepi = e.L("sj"), e.L("sdone"), e.L("noepi")
+        e.label(l_sj)
+        e(f"@{e.cond('ge.u32', j, S.nb)} bra {l_sdone};")
+        buf = o("and.b32", jj, 1)
+        ph = o("and.b32", o("shr.u32", jj, 1), 1)
+        bb = o("mad.lo.u32", buf, 8, bars)
+        sc_col = o("add.u32", o("mad.lo.u32", buf, BKV, lanebase), SCOL)
+        key0 = o("shl.b32", S.tile_of(j), 6)
+        wait_bar_warp(e, f"{bb}+{SFULL}", ph, err, ERR_SOFTMAX, l_end)
+        e("tcgen05.fence::after_thread_sync;")
+        for c in range(BKV // 32):
+            e(f"tcgen05.ld.sync.aligned.32x32b.x32.b32 {{{', '.join(s_[32 * c:32 * c + 32])}}}, [{sc_col}+{32 * c}];")
+        slot_a = o("and.b32", jj, 3)
+        ma = o("mad.lo.u32", slot_a, 8, bars)
+        km = [e.r(), e.r()]
+        e(f"ld.shared.v2.b32 {{{km[0]}, {km[1]}}}, [{ma}+{KMASK}];")
         e("tcgen05.wait::ld.sync.aligned;")
-        words = []
-        for k in range(16):
-            x0 = o("mul.f32", regs[2 * k], inv, cls="f")
-            x1 = o("mul.f32", regs[2 * k + 1], inv, cls="f")
-            words.append(o("selp.b32", 0, o(out_cvt, x1, x0), p_zero))
-        for i in range(2):
-            e(f"@{p_row} st.global.v8.b32 [{oa}+{64 * c + 32 * i}], {{{', '.join(words[8 * i:8 * i + 8])}}};")
-    if splits > 1:
-        e(f"bra {l_noepi};")
-        e.label(l_part)
-        pi = o("mad.lo.u32", cta, rows, rowl)
-        pa = at(gptr("p_part"), wide(pi, D * 4))
+        sca = None
+        if quant:
+            sca = o("mad.lo.u32", slot_a, BKV * 4, bars)
+            vnew = o("ld.shared.f32", f"[{o('mad.lo.u32', slot_a, 4, bars)}+{VREF}]", cls="f")
+
+            def times(off):
+                """The row times 64 numbers in shared memory, two at a time."""
+                for c in range(0, BKV, 4):
+                    kp = [e.r("rd"), e.r("rd")]
+                    e(f"ld.shared.v2.b64 {{{kp[0]}, {kp[1]}}}, [{sca}+{off + 4 * c}];")
+                    for i in range(2):
+                        x0, x1 = s_[c + 2 * i], s_[c + 2 * i + 1]
+                        xp = e.r("rd")
+                        e(f"mov.b64 {xp}, {{{x0}, {x1}}};")
+                        e(f"mul.rn.f32x2 {xp}, {xp}, {kp[i]};")
+                        e(f"mov.b64 {{{x0}, {x1}}}, {xp};")
+            times(KSC)
+        # the keys of the tile this row sees, as 64 bits: up to its own position, inside the window or among
+        # the sinks, on a page.  Tiles that every row of the warp sees whole skip all of it.
+        lim = o("sub.s32", pos, key0)
+        p_all = e.cond("ge.s32", lim, BKV - 1)
+        kand = o("and.b32", km[0], km[1])
+        pk_ = e.cond("eq.s32", kand, -1)
+        e(f"and.pred {p_all}, {p_all}, {pk_};")
+        wl = sk = None
+        if window is not None:
+            wl = o("sub.s32", o("sub.s32", pos, window), key0)      # keys up to here lie before the window
+            sk = o("sub.s32", sinks, key0)                          # keys below here are sinks
+            pw_ = e.cond("lt.s32", wl, 0)
+            ps_ = e.cond("ge.s32", sk, BKV)
+            e(f"or.pred {pw_}, {pw_}, {ps_};")
+            e(f"and.pred {p_all}, {p_all}, {pw_};")
+        v_all = o("vote.sync.all.pred", p_all, -1, cls="p")
+        l_seen = e.L("seen")
+        m0, m1 = o("mov.b32", -1), o("mov.b32", -1)
+        e(f"@{v_all} bra {l_seen};")
+
+        def below(n, cls="rd"):
+            """The bits below n (clamped to 0..64)."""
+            k_ = o("sub.s32", 64, o("min.s32", o("max.s32", n, 0), 64))
+            return o("shr.u64", o("mov.b64", -1, cls="rd"), k_, cls="rd")        # a shift by 64 leaves 0
+
+        bits = below(o("add.s32", o("min.s32", lim, BKV), 1))
+        if window is not None:
+            inside = o("not.b64", below(o("add.s32", wl, 1)), cls="rd")
+            inside = o("or.b64", inside, below(sk), cls="rd")
+            bits = o("and.b64", bits, inside, cls="rd")
+        pages_ = e.r("rd")
+        e(f"mov.b64 {pages_}, {{{km[0]}, {km[1]}}};")
+        bits = o("and.b64", bits, pages_, cls="rd")
+        e(f"mov.b64 {{{m0}, {m1}}}, {bits};")
+        for c in range(BKV):
+            t_ = o("and.b32", (m0, m1)[c // 32], 1 << (c % 32) if c % 32 < 31 else -(1 << 31))
+            e(f"@{e.cond('eq.u32', t_, 0)} mov.b32 {s_[c]}, 0fFF800000;")
+        e.label(l_seen)
+        if not quant:
+            # rows of V that no row of this CTA sees (past its last token, or between sinks and window) may
+            # hold anything: zero them before the product multiplies them by P = 0
+            l_vok = e.L("vok")
+            vlim = o("sub.s32", pos1, key0)
+            pv_ = e.cond("ge.s32", vlim, BKV - 1)
+            if window is not None:
+                lo_k = o("sub.s32", w["lo"], key0)
+                p1_, p2_ = e.cond("le.s32", lo_k, 0), e.cond("ge.s32", sk, BKV)
+                e(f"or.pred {p1_}, {p1_}, {p2_};")
+                e(f"and.pred {pv_}, {pv_}, {p1_};")
+            e(f"@{pv_} bra {l_vok};")                               # the same for every thread
+            wait_bar_warp(e, f"{o('mad.lo.u32', buf, 16, bars)}+{FULL + 8}", ph, err, ERR_SOFTMAX, l_end)
+            va = o("mad.lo.u32", buf, 2 * kv_bytes, o("add.u32", sKV, kv_bytes))
+            z_ = o("mov.b32", 0)
+            for h in range(2):
+                r_ = o("add.u32", lane, 32 * h)
+                pz = e.cond("gt.s32", r_, vlim)
+                if window is not None:
+                    pa, pb = e.cond("lt.s32", r_, lo_k), e.cond("ge.s32", r_, sk)
+                    e(f"and.pred {pa}, {pa}, {pb};")
+                    e(f"or.pred {pz}, {pz}, {pa};")
+                ra = o("mad.lo.u32", r_, 128, va)
+                for box in range(boxes):
+                    for i in range(8):
+                        e(f"@{pz} st.shared.v4.b32 [{ra}+{box * kv_box + 16 * i}], {{{z_}, {z_}, {z_}, {z_}}};")
+            e("fence.proxy.async.shared::cta;")
+            e.label(l_vok)
+        # the row's maximum: 8 chains of three-input maxima
+        lvl = [e.r("f") for _ in range(8)]
+        for k in range(8):
+            col = list(range(k, BKV, 8))
+            e(f"max.f32 {lvl[k]}, {s_[col[0]]}, {s_[col[1]]}, {s_[col[2]]};")
+            e(f"max.f32 {lvl[k]}, {lvl[k]}, {s_[col[3]]}, {s_[col[4]]};")
+            e(f"max.f32 {lvl[k]}, {lvl[k]}, {s_[col[5]]}, {s_[col[6]]};")
+            e(f"max.f32 {lvl[k]}, {lvl[k]}, {s_[col[7]]};")
+        e(f"max.f32 {lvl[0]}, {lvl[0]}, {lvl[1]}, {lvl[2]};")
+        e(f"max.f32 {lvl[3]}, {lvl[3]}, {lvl[4]}, {lvl[5]};")
+        e(f"max.f32 {lvl[6]}, {lvl[6]}, {lvl[7]};")
+        e(f"max.f32 {lvl[0]}, {lvl[0]}, {lvl[3]}, {lvl[6]};")
+        mnew = o("max.f32", mref, o("mul.f32", lvl[0], cf, cls="f"), cls="f")
+        alpha = o("mov.b32", "0f3F800000", cls="f")
+        l_first, l_after = e.L("first"), e.L("after")
+        anyneed = e.cond("ne.u32", lane, lane)
+        e(f"@{e.cond('eq.u32', j, 0)} bra {l_first};")
+        need = e.cond("gt.f32", mnew, o("add.f32", mref, _f32(RESCALE), cls="f"))
+        if quant:
+            e(f"or.pred {need}, {need}, {e.cond('ne.f32', vnew, vref)};")           # the same for every row
+        e(f"vote.sync.any.pred {anyneed}, {need}, -1;")
+        e(f"@!{anyneed} bra {l_after};")
+        e(f"ex2.approx.ftz.f32 {alpha}, {o('sub.f32', mref, mnew, cls='f')};")
+        # a row that has seen nothing yet while another of the warp rescales: -inf - -inf must not make a NaN
+        e(f"@{e.cond('eq.f32', mnew, '0fFF800000')} mov.b32 {alpha}, 0f3F800000;")
+        e(f"mul.f32 {lsum}, {lsum}, {alpha};")
+        if quant:
+            inv_ = o("mov.b32", o("sub.u32", "0x7F000000", o("mov.b32", vnew)), cls="f")
+            e(f"mul.f32 {alpha}, {alpha}, {o('mul.f32', vref, inv_, cls='f')};")
+        e.label(l_first)
+        e(f"mov.b32 {mref}, {mnew};")
+        if quant:
+            e(f"mov.b32 {vref}, {vnew};")
+        e.label(l_after)
+        negm = o("sub.f32", o("mov.b32", _f32(lift), cls="f"), mref, cls="f")
+        e(f"@{e.cond('eq.f32', mref, '0fFF800000')} mov.b32 {negm}, 0f00000000;")
+        cp2, np2 = e.r("rd"), e.r("rd")
+        e(f"mov.b64 {cp2}, {{{cf}, {cf}}};")
+        e(f"mov.b64 {np2}, {{{negm}, {negm}}};")
+        acc = [o("mov.b64", 0, cls="rd") for _ in range(2)]
+
+        def exps(cols):
+            for k, idx in enumerate(cols[::2]):
+                x0, x1 = s_[idx], s_[idx + 1]
+                xp, ep = e.r("rd"), e.r("rd")
+                e(f"mov.b64 {xp}, {{{x0}, {x1}}};")
+                e(f"fma.rn.f32x2 {xp}, {xp}, {cp2}, {np2};")
+                e(f"mov.b64 {{{x0}, {x1}}}, {xp};")
+                e(f"ex2.approx.ftz.f32 {x0}, {x0};")
+                e(f"ex2.approx.ftz.f32 {x1}, {x1};")
+                e(f"mov.b64 {ep}, {{{x0}, {x1}}};")
+                e(f"add.rn.f32x2 {acc[k & 1]}, {acc[k & 1]}, {ep};")
+
+        if p_f16:
+            def pack(cols):
+                hw = [o("cvt.rn.f16x2.f32", s_[c + 1], s_[c]) for c in cols[::2]]
+                e(f"tcgen05.st.sync.aligned.32x32b.x16.b32 [{sc_col}+{cols[0] // 2}], {{{', '.join(hw)}}};")
+            if quant:
+                exps(list(range(BKV)))
+                times(VSC)
+                # a masked key's scale may be NaN: its weight is 0 whatever it was multiplied by
+                l_nz = e.L("nz")
+                e(f"@{v_all} bra {l_nz};")
+                for c in range(BKV):
+                    t_ = o("and.b32", (m0, m1)[c // 32], 1 << (c % 32) if c % 32 < 31 else -(1 << 31))
+                    e(f"@{e.cond('eq.u32', t_, 0)} mov.b32 {s_[c]}, 0f00000000;")
+                e.label(l_nz)
+            for h in range(2):
+                cols = list(range(32 * h, 32 * h + 32))
+                if not quant:
+                    exps(cols)
+                pack(cols)
+        else:
+            exps(list(range(BKV)))
+            for h in range(2):
+                hi, lo = [], []
+                for c in range(32 * h, 32 * h + 32, 2):
+                    hi.append(o("prmt.b32", s_[c], s_[c + 1], "0x7632"))
+                    d0 = o("sub.f32", s_[c], o("and.b32", s_[c], -65536, cls="f"), cls="f")
+                    d1 = o("sub.f32", s_[c + 1], o("and.b32", s_[c + 1], -65536, cls="f"), cls="f")
+                    lo.append(o("prmt.b32", d0, d1, "0x7632"))
+                e(f"tcgen05.st.sync.aligned.32x32b.x16.b32 [{sc_col}+{16 * h}], {{{', '.join(hi)}}};")
+                e(f"tcgen05.st.sync.aligned.32x32b.x16.b32 [{sc_col}+{32 + 16 * h}], {{{', '.join(lo)}}};")
+        parts = [e.r("f") for _ in range(4)]
+        e(f"mov.b64 {{{parts[0]}, {parts[1]}}}, {acc[0]};")
+        e(f"mov.b64 {{{parts[2]}, {parts[3]}}}, {acc[1]};")
+        psum = o("add.f32", o("add.f32", parts[0], parts[1], cls="f"), o("add.f32", parts[2], parts[3], cls="f"), cls="f")
+        e(f"add.f32 {lsum}, {lsum}, {psum};")
+        # the lazy rescale of O, once the previous product has completed
+        l_nore = e.L("norescale")
+        e(f"@!{anyneed} bra {l_nore};")
+
+        def pv_done(k, code, bail):
+            br = o("mad.lo.u32", o("and.b32", k, 1), 8, bars)
+            wait_bar_warp(e, f"{br}+{PFREE}", o("and.b32", o("shr.u32", k, 1), 1), err, code, bail)
+
+        pv_done(o("sub.u32", jj, 1), ERR_SOFTMAX, l_end)
+        e("tcgen05.fence::after_thread_sync;")
         for c in range(D // 32):
             regs = s_[:32]
             e(f"tcgen05.ld.sync.aligned.32x32b.x32.b32 {{{', '.join(regs)}}}, [{lanebase}+{32 * c}];")
             e("tcgen05.wait::ld.sync.aligned;")
-            if quant:
-                for x in regs:
-                    e(f"mul.f32 {x}, {x}, {vref};")
-            for i in range(4):
-                e(f"@{p_row} st.global.v8.f32 [{pa}+{128 * c + 32 * i}], {{{', '.join(regs[8 * i:8 * i + 8])}}};")
-        mla = at(at(gptr("p_part"), grid * rows * D * 4), wide(pi, 8))
-        # the parts' O and l stand for 2^-negm; a part that saw nothing has m = -inf
-        meff = o("sub.f32", mref, _f32(lift), cls="f")
-        e(f"@{p_row} st.global.v2.f32 [{mla}], {{{meff}, {lsum}}};")
-    e.label(l_noepi)
+            for r_ in regs:
+                e(f"mul.f32 {r_}, {r_}, {alpha};")
+            e(f"tcgen05.st.sync.aligned.32x32b.x32.b32 [{lanebase}+{32 * c}], {{{', '.join(regs)}}};")
+        e.label(l_nore)
+        e("tcgen05.wait::st.sync.aligned;")
+        e("tcgen05.fence::before_thread_sync;")
+        e("bar.warp.sync -1;")
+        e(f"@{p_l0s} mbarrier.arrive.shared::cta.b64 _, [{bb}+{PFULL}];")
+        e(f"add.u32 {j}, {j}, 1;")
+        e(f"add.u32 {jj}, {jj}, 1;")
+        e(f"bra {l_sj};")
+
+        # epilogue: after the last product, O / l as the output type, or the part's O, m and l in f32
+        e.label(l_sdone)
+        pv_done(o("sub.u32", jj, 1), ERR_EPILOGUE, l_end)
+        e("tcgen05.fence::after_thread_sync;")
+        p_row = e.cond("lt.u32", rowl, vrows)
+        l_part = e.L("part")
+        if ctas:
+            e(f"@{e.cond('ne.u32', S.nb, S.P.tiles)} bra {l_part};")            # the unit has other runs too
+        p_zero = e.cond("eq.f32", lsum, "0f00000000")
+        inv = o("rcp.rn.f32", o("selp.f32", "0f3F800000", lsum, p_zero, cls="f"), cls="f")
+        if quant:
+            e(f"mul.f32 {inv}, {inv}, {vref};")
+        oa = at(o_ptr, wide(S.row_index(rowl), row_b))
+        for c in range(D // 32):
+            regs = s_[:32]
+            e(f"tcgen05.ld.sync.aligned.32x32b.x32.b32 {{{', '.join(regs)}}}, [{lanebase}+{32 * c}];")
+            e("tcgen05.wait::ld.sync.aligned;")
+            words = []
+            for k in range(16):
+                x0 = o("mul.f32", regs[2 * k], inv, cls="f")
+                x1 = o("mul.f32", regs[2 * k + 1], inv, cls="f")
+                words.append(o("selp.b32", 0, o(out_cvt, x1, x0), p_zero))
+            for i in range(2):
+                e(f"@{p_row} st.global.v8.b32 [{oa}+{64 * c + 32 * i}], {{{', '.join(words[8 * i:8 * i + 8])}}};")
+        if ctas:
+            e(f"bra {l_noepi};")
+            e.label(l_part)
+            # a CTA's first segment leaves part 2 c, a later one 2 c + 1
+            part = o("add.u32", o("shl.b32", cta, 1), o("selp.u32", 1, 0, e.cond("ne.u32", S.now, start)))
+            pi = o("mad.lo.u32", part, rows, rowl)
+            pa = at(gptr("p_part"), wide(pi, D * 4))
+            for c in range(D // 32):
+                regs = s_[:32]
+                e(f"tcgen05.ld.sync.aligned.32x32b.x32.b32 {{{', '.join(regs)}}}, [{lanebase}+{32 * c}];")
+                e("tcgen05.wait::ld.sync.aligned;")
+                if quant:
+                    for x in regs:
+                        e(f"mul.f32 {x}, {x}, {vref};")
+                for i in range(4):
+                    e(f"@{p_row} st.global.v8.f32 [{pa}+{128 * c + 32 * i}], {{{', '.join(regs[8 * i:8 * i + 8])}}};")
+            mla = at(at(gptr("p_part"), 2 * ctas * rows * D * 4), wide(pi, 8))
+            # the parts' O and l stand for 2^-negm; a part that saw nothing has m = -inf
+            meff = o("sub.f32", mref, _f32(lift), cls="f")
+            e(f"@{p_row} st.global.v2.f32 [{mla}], {{{meff}, {lsum}}};")
+        e.label(l_noepi)
+
+    each_segment("s", softmax, l_end)
 
     e.label(l_end)
     e("barrier.sync 0;")
@@ -894,9 +1004,9 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         params = [("Q", qn, 16), ("KC", kn, 16), ("VC", vn, 16)]
     params += [("table", tn, 4), ("lens", ln, 4), ("fresh", fn, 4), ("O", on, 32)]
     sc_spec = []
-    if splits > 1:
+    if ctas:
         params += [("part", scratch, 32)]
-        sc_spec = [{"name": scratch, "dtype": "f32", "shape": [grid * rows, D + 2], "per_call": True}]
+        sc_spec = [{"name": scratch, "dtype": "f32", "shape": [2 * ctas * rows, D + 2], "per_call": True}]
     es = 1 if quant else 2
     span = min(128, D * es)                                     # a box row, and the swizzle
     tmaps = [{"name": f"tm{x}", "tensor": nm, "dtype": "u8" if quant else dtype, "dims": [D, page, kv_heads, pages],
@@ -917,15 +1027,16 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     }
 
 
-def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype, window, sinks, names, scratch, splits,
-               min_tiles, locate=None):
-    """The second entry: rows whose unit was split, o = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.  One block a row;
-    its four warps take every fourth part, so that a row of 100 parts is 25 loads deep.  Rows of units that
-    fit one part are written already and return at once.  ``locate`` finds a row's parts (the default: ``splits`` parts
-    a unit, of at least ``min_tiles`` tiles each)."""
+def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype, window, sinks, names, scratch, ctas,
+               min_tiles=MIN_TILES):
+    """The second entry: the rows of units of more than one run, o = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.  One
+    block a unit, which finds the unit's runs by the same prefix sums; a warp a row.  Units of one run are written
+    already; rows of units that see no key at all, which no run covers, become 0."""
     D = dim
     group, tq, ntile, rows = geometry(chunk, heads, kv_heads)
+    pairs = batch * ntile
     per_lane = D // 32
+    threads = 256
     e = _E()
     o = e.o
 
@@ -938,44 +1049,57 @@ def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype,
     tid = o("mov.u32", "%tid.x")
     warp, lane = o("shr.u32", tid, 5), o("and.b32", tid, 31)
     e("griddepcontrol.wait;")                                   # the parts are written
-    row = o("mov.u32", "%ctaid.x")
-    h, bc = o("rem.u32", row, heads), o("div.u32", row, heads)
-    c, b = o("rem.u32", bc, chunk), o("div.u32", bc, chunk)
-    b_len = o("ld.global.nc.u32", f"[{at(gptr('p_lens'), b, 4)}]")
-    b_new = o("ld.global.nc.u32", f"[{at(gptr('p_fresh'), b, 4)}]")
-    e(f"@{e.cond('ge.s32', c, b_new)} ret;")
-    if locate is None:
-        tile = o("div.u32", c, tq)
-        c0 = o("mul.lo.u32", tile, tq)
-        w = _unit(e, None, b_len, b_new, c0, splits, min_tiles, tq, chunk, max_pages * page, window, sinks)
-        e(f"@{e.cond('le.u32', w['total'], w['per'])} ret;")
-        nact = o("div.u32", o("sub.u32", o("add.u32", w["total"], w["per"]), 1), w["per"])
-        unit = o("mad.lo.u32", o("sub.u32", ntile - 1, tile), batch, b)
-        unit = o("mad.lo.u32", unit, kv_heads, o("div.u32", h, group))
-        rowl = o("mad.lo.u32", o("sub.u32", c, c0), group, o("rem.u32", h, group))
-        base = o("mad.lo.u32", o("mul.lo.u32", unit, splits), rows, rowl)     # part 0's row; parts are ``rows`` apart
-        part_rows = batch * kv_heads * ntile * splits * rows
+    cta = o("mov.u32", "%ctaid.x")
+    lens, fresh = gptr("p_lens"), gptr("p_fresh")
 
-        def part_row(s_):
-            return o("mad.lo.u32", s_, rows, base)
-    else:
-        def zero_row(p_none):
-            """A row that sees no key, where ``p_none``: 0."""
-            l_ = e.L("nz")
-            e(f"@!{p_none} bra {l_};")
-            e(f"@{e.cond('ge.u32', tid, D // 2)} ret;")
-            e(f"st.global.b32 [{at(at(gptr('p_O'), row, D * 2), tid, 4)}], {o('mov.b32', 0)};")
-            e("ret;")
-            e.label(l_)
-        nact, part_row, part_rows = locate(e, lambda x, y: o("add.s64", x, y, cls="rd"), gptr, lane, b, c, h, zero_row)
+    def place(pair, ok=None):
+        return _Place(e, pair, ok, lens, fresh, batch, chunk, group, tq, ntile, max_pages * page, window, sinks)
+
+    kvh, pair = o("rem.u32", cta, kv_heads), o("div.u32", cta, kv_heads)
+    P = place(pair)
+    e(f"@!{P.live} ret;")                                       # a tile of padding
+    run, before = o("mov.u32", 0), o("mov.u32", 0)
+    for k in range(-(-pairs // 32)):
+        q = o("add.u32", lane, 32 * k) if k else lane
+        v = place(q, e.cond("lt.u32", q, pairs)).tiles
+        e(f"add.u32 {run}, {run}, {v};")
+        e(f"@{e.cond('lt.u32', q, pair)} add.u32 {before}, {before}, {v};")
+    run, before = (o("mul.lo.u32", o("redux.sync.add.u32", x, -1), kv_heads) for x in (run, before))
+    per = o("max.u32", o("div.u32", o("add.u32", run, ctas - 1), ctas), min_tiles)
+    t0 = o("mad.lo.u32", kvh, P.tiles, before)
+    first = o("div.u32", t0, per)
+    last = o("div.u32", o("sub.u32", o("add.u32", t0, P.tiles), 1), per)
+    none = e.cond("eq.u32", P.tiles, 0)
+    p_one = e.cond("eq.u32", first, last)
+    some = e.cond("ne.u32", P.tiles, 0)
+    e(f"and.pred {p_one}, {p_one}, {some};")
+    e(f"@{p_one} ret;")                                         # one run: written already
+    nact = o("selp.u32", 0, o("add.u32", o("sub.u32", last, first), 1), none)
+    # the first run reaches the unit as a later segment (part 2 c + 1) unless it begins with it
+    late = o("selp.u32", 1, 0, e.cond("ne.u32", t0, o("mul.lo.u32", first, per)))
+    r0 = o("mad.lo.u32", o("mul.lo.u32", first, 2), rows, 0)
+    r_late = o("mad.lo.u32", late, rows, r0)
+    base_row = o("mad.lo.u32", P.b, chunk, P.c0)
+    base_row = o("mad.lo.u32", base_row, heads, o("mul.lo.u32", kvh, group))
     part = gptr("p_part")
-    ml = o("add.s64", part, part_rows * D * 4, cls="rd")
-    # the largest reference of the row's parts (every warp on its own)
+    ml = o("add.s64", part, 2 * ctas * rows * D * 4, cls="rd")
+    part_l = at(part, lane, per_lane * 4)
+    o_l = at(gptr("p_O"), lane, per_lane * 2)
+    vec = f"v{per_lane}"
+    row = o("mov.u32", warp)
+    l_row, l_out = e.L("row"), e.L("out")
+    e.label(l_row)
+    e(f"@{e.cond('ge.u32', row, P.vrows)} bra {l_out};")
+
+    def part_row(s_):
+        base = o("selp.u32", r_late, o("mad.lo.u32", s_, 2 * rows, r0), e.cond("eq.u32", s_, 0))
+        return o("add.u32", base, row)
+
     m = o("mov.b32", "0fFF800000", cls="f")
     s = o("mov.u32", lane)
     l_m, l_md = e.L("m"), e.L("md")
     e.label(l_m)
-    e(f"@{e.cond('ge.u32', o('and.b32', s, -32), nact)} bra {l_md};")           # the same for the warp
+    e(f"@{e.cond('ge.u32', o('and.b32', s, -32), nact)} bra {l_md};")            # the same for the warp
     v = o("mov.b32", "0fFF800000", cls="f")
     e(f"@{e.cond('lt.u32', s, nact)} ld.global.f32 {v}, [{at(ml, part_row(s), 8)}];")
     e(f"max.f32 {m}, {m}, {v};")
@@ -987,16 +1111,13 @@ def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype,
     e(f"@{e.cond('eq.f32', m, '0fFF800000')} mov.b32 {m}, 0f00000000;")
     acc = [o("mov.b32", "0f00000000", cls="f") for _ in range(per_lane)]
     l = o("mov.b32", "0f00000000", cls="f")
-    s = o("mov.u32", warp)
+    s = o("mov.u32", 0)
     l_top, l_done = e.L("p"), e.L("pd")
-    UN = 4
-    vec = f"v{per_lane}"
-    part_l = at(part, lane, per_lane * 4)
     e.label(l_top)
     e(f"@{e.cond('ge.u32', s, nact)} bra {l_done};")
     loaded = []
-    for u in range(UN):
-        su = o("add.u32", s, 4 * u)
+    for u in range(4):
+        su = o("add.u32", s, u)
         ok = e.cond("lt.u32", su, nact)
         idx = part_row(su)
         ms, ls = o("mov.b32", "0fFF800000", cls="f"), o("mov.b32", "0f00000000", cls="f")
@@ -1009,40 +1130,31 @@ def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype,
         e(f"fma.rn.f32 {l}, {f}, {ls}, {l};")
         for a_, x in zip(acc, xs):
             e(f"fma.rn.f32 {a_}, {f}, {x}, {a_};")
-    e(f"add.u32 {s}, {s}, {4 * UN};")
+    e(f"add.u32 {s}, {s}, 4;")
     e(f"bra {l_top};")
     e.label(l_done)
-    sm = o("mov.u32", f"{name}_sum")
-    sl = o("mov.u32", f"{name}_l")
-    wa = o("mad.lo.u32", warp, D * 4, sm)
-    wa = o("mad.lo.u32", lane, per_lane * 4, wa)
-    e(f"st.shared.{vec}.f32 [{wa}], {{{', '.join(acc)}}};")
-    e(f"st.shared.f32 [{o('mad.lo.u32', warp, 4, sl)}], {l};")                 # every lane holds the same l
-    e("bar.sync 0;")
-    e(f"@{e.cond('ge.u32', tid, D // 2)} ret;")
-    ls = [e.r("f") for _ in range(4)]
-    e(f"ld.shared.v4.f32 {{{', '.join(ls)}}}, [{sl}];")
-    lt = o("add.f32", o("add.f32", ls[0], ls[1], cls="f"), o("add.f32", ls[2], ls[3], cls="f"), cls="f")
-    xs = [o("mov.b32", "0f00000000", cls="f") for _ in range(2)]
-    ra = o("mad.lo.u32", tid, 8, sm)
-    for k in range(4):
-        y = [e.r("f") for _ in range(2)]
-        e(f"ld.shared.v2.f32 {{{y[0]}, {y[1]}}}, [{ra}+{k * D * 4}];")
-        for i in range(2):
-            e(f"add.f32 {xs[i]}, {xs[i]}, {y[i]};")
-    p_zero = e.cond("eq.f32", lt, "0f00000000")
-    inv = o("rcp.rn.f32", o("selp.f32", "0f3F800000", lt, p_zero, cls="f"), cls="f")
-    x0, x1 = (o("mul.f32", x, inv, cls="f") for x in xs)
-    word = o("cvt.rn.f16x2.f32" if dtype == "f16" else "cvt.rn.bf16x2.f32", x1, x0)
-    word = o("selp.b32", 0, word, p_zero)
-    oa = at(at(gptr("p_O"), row, D * 2), tid, 4)
-    e(f"st.global.b32 [{oa}], {word};")
+    p_zero = e.cond("eq.f32", l, "0f00000000")
+    inv = o("rcp.rn.f32", o("selp.f32", "0f3F800000", l, p_zero, cls="f"), cls="f")
+    words = []
+    for x in range(0, per_lane, 2):
+        x0, x1 = (o("mul.f32", acc[x + k], inv, cls="f") for k in range(2))
+        word = o("cvt.rn.f16x2.f32" if dtype == "f16" else "cvt.rn.bf16x2.f32", x1, x0)
+        words.append(o("selp.b32", 0, word, p_zero))
+    t_ = o("div.u32", row, group)
+    ro = o("add.u32", o("mad.lo.u32", t_, heads, base_row), o("sub.u32", row, o("mul.lo.u32", t_, group)))
+    oa = at(o_l, ro, D * 2)
+    if per_lane == 2:
+        e(f"st.global.b32 [{oa}], {words[0]};")
+    else:
+        e(f"st.global.v2.b32 [{oa}], {{{', '.join(words)}}};")
+    e(f"add.u32 {row}, {row}, {threads // 32};")
+    e(f"bra {l_row};")
+    e.label(l_out)
     ln, fn, on = names
-    params = [("lens", ln, 4), ("fresh", fn, 4), ("O", on, 4), ("part", scratch, 32)]
+    params = [("lens", ln, 4), ("fresh", fn, 4), ("O", on, 8), ("part", scratch, 32)]
     text = [f".visible .entry {name}(", ",\n".join(f"\t.param .u64 p_{p}" for p, _, _ in params), ")",
-            ".reqntid 128, 1, 1", "{"]
+            f".reqntid {threads}, 1, 1", "{"]
     text += e.decls() + e.lines + ["\tret;", "}"]
     return {"name": name, "kind": "paged_attention_join", "params": [n for _, n, _ in params], "raw_entry": text,
-            "raw_decls": [f".shared .align 16 .b8 {name}_sum[{4 * D * 4}];", f".shared .align 16 .b8 {name}_l[16];"],
-            "grid": [batch * chunk * heads, 1, 1], "block": [128, 1, 1], "dyn_smem": 0,
+            "grid": [pairs * kv_heads, 1, 1], "block": [threads, 1, 1], "dyn_smem": 0,
             "align": {n: a_ for _, n, a_ in params}, "zero_outputs": [], "pdl": True}

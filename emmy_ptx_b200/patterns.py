@@ -520,7 +520,7 @@ def _args_of(graph, node) -> list:
 
 
 def _lower_paged_attention(graph, node, kw, prefix, options):
-    """The tensor-core entries of a paged attention: one, or two when its units are split.  Units of few rows
+    """The tensor-core entries of a paged attention: one, or two when its tiles are spread over CTAs.  Units of few rows
     (a decode step, a short draft) are bound by the cache's bytes and take the register form."""
     from .kernels import paged_rows as pr, tc_paged_attention as tpa
     geo = {k: kw[k] for k in ("batch", "chunk", "heads", "kv_heads", "page", "max_pages", "window", "sinks")}
@@ -531,23 +531,21 @@ def _lower_paged_attention(graph, node, kw, prefix, options):
     name = node.op.name
     names = [*node.inputs, node.outputs[0].name]
     scratch = f"{prefix}{name}__part"
-    jkw = dict(**geo, dim=kw["dim"], dtype=kw["dtype"], names=names[-3:], scratch=scratch)
     if few:
+        form, build = pr, pr.paged_rows_entry
         ctas = pr.plan_ctas(**geo, dim=kw["dim"], quant=kw["quant"], sms=sms)
-        if "paged_splits" in options:
-            n = int(options["paged_splits"])
-            ctas = n * kw["batch"] * kw["kv_heads"] if n > 1 and kw["batch"] <= pr.MAX_SPREAD_BATCH else 0
-        least = int(options.get("paged_min_tiles", pr.MIN_TILES))
-        main = pr.paged_rows_entry(name, **kw, names=names, scratch=scratch, ctas=ctas, min_tiles=least, prefix=prefix)
-        join = pr.spread_join_entry(f"{name}_join", **jkw, ctas=ctas, min_tiles=least) if ctas else None
     elif tpa.supported(kw["dim"], kw["heads"], kw["kv_heads"], kw["page"]):
-        splits, least = tpa.plan_splits(**geo, sms=sms)
-        splits, least = int(options.get("paged_splits", splits)), int(options.get("paged_min_tiles", least))
-        main = tpa.paged_attention_entry(name, **kw, names=names, scratch=scratch, splits=splits, min_tiles=least,
-                                         prefix=prefix)
-        join = tpa.join_entry(f"{name}_join", **jkw, splits=splits, min_tiles=least) if splits > 1 else None
+        form, build = tpa, tpa.paged_attention_entry
+        ctas = tpa.plan_ctas(**geo, sms=sms)
     else:
         return None
+    ctas = int(options.get("paged_ctas", ctas))
+    least = int(options.get("paged_min_tiles", form.MIN_TILES))
+    main = build(name, **kw, names=names, scratch=scratch, ctas=ctas, min_tiles=least, prefix=prefix)
+    join = None
+    if ctas:
+        join = form.join_entry(f"{name}_join", **geo, dim=kw["dim"], dtype=kw["dtype"], names=names[-3:], scratch=scratch,
+                               ctas=ctas, min_tiles=least)
     main["args"] = _args_of(graph, node)
     return [main, join] if join else main
 

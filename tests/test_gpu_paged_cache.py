@@ -9,7 +9,7 @@ from emmy_ptx_b200.compiler import compile_graph
 from emmy_ptx_b200.ir import Graph
 from emmy_ptx_b200.runtime import Executable
 from tests import pagedref as R
-from tests.test_paged_cache import ATTENDS, FORMS, READS, TENSOR, WRITES, awkward_rows, broken_table, form_opts, same
+from tests.test_paged_cache import ATTENDS, FORMS, READS, SPREAD, TENSOR, WRITES, awkward_rows, broken_table, form_opts, same
 
 pytestmark = pytest.mark.gpu
 
@@ -44,6 +44,19 @@ def test_paged_attention(form, case, dtype, quant):
     assert kinds[0] == FORMS[form]
     ref, bound, _ = R.attention_ref(t, page, window, sinks)
     R.check(got["O"], ref, bound, form)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("form,case", [(f, c) for f in FORMS for c in SPREAD if f == "tiles" or c[1] <= 32],
+                         ids=lambda c: c if isinstance(c, str) else "x".join(map(str, c[:7])))
+def test_paged_attention_runs_over_many_units(form, case, quant):
+    B, C, H, hk, d, page, mp, lens, fresh, window, sinks = case
+    t, pages = R.make("attend", B, hk, d, page, mp, lens, fresh, chunk=C, heads=H, quant=quant, seed=B)
+    p = irgen.paged_attention_ir(B, C, H, hk, d, pages, page, mp, "bf16", quant, window, sinks)
+    ref, bound, _ = R.attention_ref(t, page, window, sinks)
+    for ctas in (1, 2, 3, 4, 5, 7, 11, 40):
+        got, _ = go(p, t, {"paged_rows": 64 if form == "rows" else 0, "paged_ctas": ctas, "paged_min_tiles": 1})
+        R.check(got["O"], ref, bound, f"{form} {ctas}")
 
 
 @pytest.mark.parametrize("dtype,quant", [("bf16", False), ("f16", True)])
@@ -90,7 +103,7 @@ def test_paged_attention_missing_pages(page, quant):
     p = irgen.paged_attention_ir(2, 3, 2, 1, 64, pages, page, mp, "bf16", quant)
     ref, bound, _ = R.attention_ref(t, page)
     for rows in (0, 64):
-        for opts in ({}, {"paged_splits": 2, "paged_min_tiles": 2}):
+        for opts in ({}, {"paged_ctas": 3, "paged_min_tiles": 2}):
             got, _ = go(p, t, {**opts, "paged_rows": rows})
             R.check(got["O"], ref, bound, "missing pages")
     t["table"].fill_(-1)
@@ -158,7 +171,7 @@ def test_a_serving_step_captured_and_replayed(quant):
     t = {**r, **a, **t}
     common = (hk, d, pages, page, mp, "bf16", quant)
     steps = [build(irgen.cache_write_ir(B, 1, *common)), build(irgen.paged_attention_ir(B, 1, H, *common),
-             {"paged_splits": 2, "paged_min_tiles": 1}), build(irgen.cache_read_ir(B, mp * page, *common))]
+             {"paged_ctas": 3, "paged_min_tiles": 1}), build(irgen.cache_read_ir(B, mp * page, *common))]
     g = on_gpu(t)
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())

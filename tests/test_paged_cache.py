@@ -180,16 +180,16 @@ TENSOR = [
     # batch, chunk, heads, kv_heads, dim, page, max_pages, lens, fresh, window, sinks, options
     (2, 1, 2, 1, 64, 16, 8, [1, 128], [1, 1], None, 0, {}),
     (3, 1, 4, 2, 128, 32, 6, [190, 0, 64], [1, 0, 1], None, 0, {}),
-    (1, 1, 6, 2, 64, 64, 5, [300], [1], None, 0, {"paged_splits": 3, "paged_min_tiles": 1}),
-    (2, 5, 3, 1, 64, 8, 20, [77, 160], [5, 3], None, 0, {"paged_splits": 2, "paged_min_tiles": 1}),
+    (1, 1, 6, 2, 64, 64, 5, [300], [1], None, 0, {"paged_ctas": 5, "paged_min_tiles": 1}),
+    (2, 5, 3, 1, 64, 8, 20, [77, 160], [5, 3], None, 0, {"paged_ctas": 3, "paged_min_tiles": 1}),
     (1, 70, 5, 1, 64, 128, 2, [150], [70], None, 0, {}),                     # 25 tokens a tile, 125 rows
     (1, 130, 1, 1, 128, 64, 3, [140], [130], None, 0, {}),                   # a tile of 128 tokens and one of 2
     (2, 1, 2, 2, 64, 16, 20, [320, 40], [1, 1], 70, 3, {}),                  # sink tile, then the window's
-    (1, 40, 2, 1, 64, 32, 12, [380], [40], 100, 5, {"paged_splits": 2, "paged_min_tiles": 1}),
+    (1, 40, 2, 1, 64, 32, 12, [380], [40], 100, 5, {"paged_ctas": 3, "paged_min_tiles": 1}),
     (1, 9, 2, 1, 64, 64, 4, [256], [9], 1, 0, {}),
     (1, 9, 2, 1, 64, 64, 4, [200], [9], 3, 150, {}),                         # more sinks than a tile
     (2, 6, 2, 1, 64, 16, 2, [4, 40], [6, 6], None, 0, {}),                   # positions below 0, past the table
-    (2, 5, 7, 1, 128, 8, 20, [77, 160], [5, 3], 40, 3, {"paged_splits": 2, "paged_min_tiles": 1}),   # 35 rows
+    (2, 5, 7, 1, 128, 8, 20, [77, 160], [5, 3], 40, 3, {"paged_ctas": 3, "paged_min_tiles": 1}),   # 35 rows
     (1, 8, 8, 1, 64, 16, 9, [131], [8], None, 0, {}),                         # 64 rows
 ]
 FORMS = {"rows": "paged_attention_rows", "tiles": "tcgen05_paged_attention"}
@@ -213,7 +213,7 @@ def test_paged_attention_tensor_cores_emulated(form, case, dtype, quant):
     got, code, mod = PE.run(p, t, opts)
     assert code == 0
     kinds = [k["kind"] for k in mod.kernels]
-    assert kinds == [FORMS[form]] + ["paged_attention_join"] * (opts.get("paged_splits", 1) > 1)
+    assert kinds == [FORMS[form]] + ["paged_attention_join"] * (opts.get("paged_ctas", 0) > 0)
     ref, bound, _ = R.attention_ref(t, page, window, sinks)
     R.check(got["O"], ref, bound, form)
 
@@ -229,10 +229,34 @@ def test_paged_attention_late_completions_and_missing_pages(page, quant, rows):
     t["table"][0, mp - 2] = pages
     t["table"][1, 0] = 2 ** 31 - 1
     p = irgen.paged_attention_ir(2, 3, 2, 1, 64, pages, page, mp, "bf16", quant)
-    got, code, _ = PE.run(p, t, {"paged_splits": 2, "paged_min_tiles": 2, "paged_rows": rows}, defer=True)
+    got, code, _ = PE.run(p, t, {"paged_ctas": 3, "paged_min_tiles": 2, "paged_rows": rows}, defer=True)
     assert code == 0
     ref, bound, _ = R.attention_ref(t, page)
     R.check(got["O"], ref, bound, "late completions")
+
+
+SPREAD = [
+    # batch, chunk, heads, kv_heads, dim, page, max_pages, lens, fresh, window, sinks
+    (5, 2, 4, 2, 64, 16, 13, [70, 0, 200, 1, 65], [2, 0, 1, 2, 2], None, 0),       # 4's first row sees no key
+    (3, 70, 2, 1, 64, 64, 4, [250, 69, 130], [70, 70, 3], None, 0),                 # two token tiles, one of padding
+    (3, 3, 2, 1, 64, 8, 25, [200, 5, 150], [3, 3, 3], 66, 4),
+]
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("ctas", [1, 2, 3, 7])
+@pytest.mark.parametrize("form,case", [(f, c) for f in FORMS for c in SPREAD if f == "tiles" or c[1] <= 32],
+                         ids=lambda c: c if isinstance(c, str) else "x".join(map(str, c[:7])))
+def test_paged_attention_runs_over_many_units(form, case, ctas, quant):
+    # runs that end in one unit, cover others and begin a third, at odd and even tiles; sequences without work
+    B, C, H, hk, d, page, mp, lens, fresh, window, sinks = case
+    t, pages = R.make("attend", B, hk, d, page, mp, lens, fresh, chunk=C, heads=H, quant=quant, seed=ctas)
+    p = irgen.paged_attention_ir(B, C, H, hk, d, pages, page, mp, "bf16", quant, window, sinks)
+    ref, bound, _ = R.attention_ref(t, page, window, sinks)
+    got, code, _ = PE.run(p, t, {"paged_rows": 64 if form == "rows" else 0, "paged_ctas": ctas, "paged_min_tiles": 1},
+                          defer=ctas == 2)
+    assert code == 0
+    R.check(got["O"], ref, bound, f"{form} {ctas}")
 
 
 @pytest.mark.parametrize("missing", range(0, 17, 2))
@@ -254,7 +278,7 @@ def test_paged_attention_all_pages_missing_is_zero(quant, rows):
     t, pages = R.make("attend", 1, 1, 64, 16, 8, [100], [2], chunk=2, heads=2, quant=quant)
     t["table"].fill_(-1)
     p = irgen.paged_attention_ir(1, 2, 2, 1, 64, pages, 16, 8, "bf16", quant)
-    for opts in ({}, {"paged_splits": 2, "paged_min_tiles": 1}):
+    for opts in ({}, {"paged_ctas": 3, "paged_min_tiles": 1}):
         got, code, _ = PE.run(p, t, {**opts, "paged_rows": rows})
         assert code == 0 and not got["O"].any()
 
