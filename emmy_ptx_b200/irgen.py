@@ -788,7 +788,8 @@ def paged_attention_ir(batch: int, chunk: int, heads: int, kv_heads: int, dim: i
     sees the keys 0..p, or with ``window`` those of p - window + 1..p and the first ``sinks`` ones.  One warp per
     query row and the online softmax of :func:`attention_ir` with its safe maximum; keys that are not
     seen are skipped, so whatever their rows hold cannot reach the result.  A row that sees no key (or
-    only keys whose score is -inf) ends as 0."""
+    only keys whose score is -inf) ends as 0.  (Lowered to the tensor cores, an infinity in the values of a key that a
+    row does see may come out as NaN there, since P is multiplied in parts one of which can be 0.)"""
     _cache_dims("paged_attention_ir", dtype, quant, batch=batch, chunk=chunk, heads=heads, kv_heads=kv_heads, dim=dim,
                 pages=pages, page=page, max_pages=max_pages)
     if heads % kv_heads:

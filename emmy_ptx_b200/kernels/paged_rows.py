@@ -25,6 +25,10 @@ meets the other warps once, at the end.
   f16 caches, in two bf16 parts (2^-14 together) for bf16 caches and bytes; bytes are converted exactly.
   The reference of a row is raised when a score exceeds it by 2^8, so most blocks need no maximum.
 
+* **What is masked** keeps its promise: V rows that no row of the unit sees become 0 in registers, and where some rows
+  see a key and others do not, an infinity or a NaN in its V row is taken out of the product and put back by two
+  products of indicators (which rows see the key, which elements are +inf or NaN, -inf or NaN).
+
 The tcgen05 form holds a row a thread: four rows keep 4 of its 128 softmax threads busy, and each tile passes
 through TMA, MMA, TMEM and back.
 """
@@ -123,6 +127,7 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
     bpt = 64 // BLK                          # blocks of a 64-key tile
     prow = math.gcd(page, BLK)               # rows of a block that lie on one page at least
     pieces = range(BLK // prow)
+    scan = not quant and chunk > 1           # rows of different positions share V rows that may hold anything
     sc_b = 2 * BLK * 4 if quant else 0       # bytes of a block's scales
     bw = min(row_b, 128)                     # bytes of a box row, and the swizzle's span
     boxes = row_b // bw
@@ -555,6 +560,65 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
         for (a, j, h), ps in sees.items():
             e(f"@!{ps} mov.b32 {sv[a][2 * h + j]}, 0f00000000;")
         e.label(l_ok)
+    exp_mask = 0x7C00 if half else 0x7F80
+    one = 0x3C00 if half else 0x3F80
+
+    def specials(vr, nt0, n_, a0):
+        """Blocks in which a key is seen by some rows only: takes infinities and NaNs out of the V rows ``vr`` and adds
+        them to O for the rows that see them, by their signs (a NaN counts as both)."""
+        l_out = e.L("clean")
+        e(f"@{whole} bra {l_out};")
+        m_ = None
+        for r_ in range(4):
+            for x in vr[r_]:
+                x = o("and.b32", x, "0x7FFF7FFF")
+                m_ = x if m_ is None else o("max.u16x2", m_, x)
+        m_ = o("max.u32", o("and.b32", m_, 65535), o("shr.u32", m_, 16))
+        e(f"@!{o('vote.sync.any.pred', e.cond('ge.u32', m_, exp_mask), -1, cls='p')} bra {l_out};")
+        va_ = []                                               # which rows see which key: A of the indicators' products
+        for a in range(2):
+            for h in (0, 1):
+                if h not in hs:
+                    va_.append(zero)
+                    continue
+                lo_ = o("selp.u32", one, 0, sees[a0 + a, 0, h])
+                va_.append(o("add.u32", lo_, o("selp.u32", one << 16, 0, sees[a0 + a, 1, h])))
+        for x in range(n_):
+            ind = [[], []]
+            for k in range(2):
+                sel = "0x7632" if x % 2 else "0x5410"
+                w_ = o("prmt.b32", vr[2 * k][x // 2], vr[2 * k + 1][x // 2], sel)
+                pos_w, neg_w = o("mov.u32", 0), o("mov.u32", 0)
+                for hf in range(2):
+                    mag = o("and.b32", w_, 0x7FFF << (16 * hf))
+                    sg = o("and.b32", w_, 0x8000 << (16 * hf))
+                    p_sp = e.cond("ge.u32", mag, exp_mask << (16 * hf))
+                    p_nan = e.cond("gt.u32", mag, exp_mask << (16 * hf))
+                    p_neg = e.cond("ne.u32", sg, 0)
+                    p_p, p_n = e.r("p"), e.r("p")
+                    e(f"not.pred {p_p}, {p_neg};")
+                    e(f"or.pred {p_p}, {p_p}, {p_nan};")
+                    e(f"and.pred {p_p}, {p_p}, {p_sp};")
+                    e(f"or.pred {p_n}, {p_neg}, {p_nan};")
+                    e(f"and.pred {p_n}, {p_n}, {p_sp};")
+                    e(f"@{p_p} or.b32 {pos_w}, {pos_w}, {one << (16 * hf)};")
+                    e(f"@{p_n} or.b32 {neg_w}, {neg_w}, {one << (16 * hf)};")
+                ind[0].append(pos_w)
+                ind[1].append(neg_w)
+            for sgn, big in ((0, "0f7F800000"), (1, "0fFF800000")):
+                cnt = [o("mov.b32", "0f00000000", cls="f") for _ in range(4)]
+                mma(pty, cnt, va_, ind[sgn], cnt)
+                for h in hs:
+                    for j in range(2):
+                        y = acc[nt0 + x][2 * h + j]
+                        e(f"@{e.cond('gt.f32', cnt[2 * h + j], '0f00000000')} add.f32 {y}, {y}, {big};")
+        for r_ in range(4):
+            for x in vr[r_]:
+                lo_, hi_ = o("and.b32", x, 0x7FFF), o("and.b32", x, 0x7FFF0000)
+                e(f"@{e.cond('ge.u32', lo_, exp_mask)} and.b32 {x}, {x}, -65536;")
+                e(f"@{e.cond('ge.u32', hi_, exp_mask << 16)} and.b32 {x}, {x}, 65535;")
+        e.label(l_out)
+
     for kb in range(KB):
         # P as the second product's A: rows g (and g + 8), keys 2t, 2t+1 and 8 further
         pa = [[None] * 4 for _ in range(1 if p_f16 else 2)]
@@ -588,6 +652,8 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
                         e(f"@!{live[r_]} mov.b32 {x}, 0;")
                 e.label(l_live)
             per_piece = v_ld // es
+            if scan:
+                specials(vr, i * per_piece, per_piece, 2 * kb)
             for x in range(per_piece):
                 nt = i * per_piece + x
                 bb = []

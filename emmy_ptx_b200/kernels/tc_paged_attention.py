@@ -31,7 +31,9 @@ largest still has 11 bits.  O is rescaled only when the row's maximum grew by mo
 
 **What is masked.**  Scores past the row's own position, outside its window or of a page that the table does not
 name become -inf; a row that sees nothing ends as 0.  Rows of a V tile that no row of the CTA sees are zeroed in
-shared memory before the product (P is 0 there, but a stale row may hold NaN).
+shared memory before the product (P is 0 there, but a stale row may hold NaN).  Where some rows see a key and others
+do not (the diagonal, a window's edge) the V tile is scanned: an infinity or a NaN must reach the rows that see it,
+and no other.  It is added to O by those rows, and the product gets 0 in its place.
 
 The roles (loads, conversion, products, softmax) walk the run's segments on their own, each as far ahead as the
 barriers between them let it; barrier phases, ring stages and score buffers go by the tile's number in the run.
@@ -69,6 +71,7 @@ KMASK = 192
 KSC = 256
 VSC = KSC + 4 * BKV * 4
 VREF = 224                       # 4 floats
+VBAD = 240                       # two words per score buffer: rows of the V tile that hold an infinity or a NaN
 QSC = VSC + 4 * BKV * 4
 RAWSC = QSC + 4 * ROWS
 AUX_BYTES = RAWSC + 2 * 2 * BKV * 4
@@ -206,6 +209,8 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     half = dtype == "f16" or quant           # the operands' type; in bf16 P comes in two parts
     p_f16 = half
     raw_b = BKV * D if quant else 0          # raw bytes of a K or V tile
+    scan = not quant and min(tq, chunk) > 1  # rows of different positions share a V tile that may hold anything
+    exp_mask = 0x7C00 if dtype == "f16" else 0x7F80
     row_b = D * 2
     q_bytes, q_box = ROWS * row_b, ROWS * 128
     kv_bytes, kv_box = BKV * row_b, BKV * 128
@@ -346,6 +351,8 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         e(f"mbarrier.init.shared::cta.b64 [{bars}+{SFULL + 8 * u}], 1;")
         e(f"mbarrier.init.shared::cta.b64 [{bars}+{PFULL + 8 * u}], 4;")
         e(f"mbarrier.init.shared::cta.b64 [{bars}+{PFREE + 8 * u}], 1;")
+    if scan:
+        e(f"st.shared.v4.b32 [{bars}+{VBAD}], {{{', '.join([o('mov.b32', 0)] * 4)}}};")
     e("fence.mbarrier_init.release.cluster;")
     e("fence.proxy.async.shared::cta;")
     e.label(l_init)
@@ -616,6 +623,33 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         commit(SFULL + 8 * u)
 
     jj_m, segs = o("mov.u32", 0), o("mov.u32", 0)
+    zero2 = o("mov.u32", 0)
+
+    def clear(tile_addr, bad):
+        """Writes 0 over the infinities and NaNs of the V tile's rows ``bad`` (two words; one thread, a rare path)."""
+        row, end_ = o("mov.u32", 0), o("mov.u32", BKV)
+        l_r, l_c, l_n, l_d = e.L("clr"), e.L("clrc"), e.L("clrn"), e.L("clrd")
+        e.label(l_r)
+        e(f"@{e.cond('ge.u32', row, end_)} bra {l_d};")
+        word = o("selp.b32", bad[0], bad[1], e.cond("lt.u32", row, 32))
+        bit = o("and.b32", o("shr.u32", word, o("and.b32", row, 31)), 1)
+        e(f"@{e.cond('eq.u32', bit, 0)} bra {l_n};")
+        a_ = o("mad.lo.u32", row, 128, tile_addr)
+        k_ = o("mov.u32", 0)
+        e.label(l_c)
+        for box in range(boxes):
+            x = o("ld.shared.b32", f"[{a_}+{box * kv_box}]")
+            lo_, hi_ = o("and.b32", x, 0x7FFF), o("and.b32", x, 0x7FFF0000)
+            e(f"@{e.cond('ge.u32', lo_, exp_mask)} and.b32 {x}, {x}, -65536;")
+            e(f"@{e.cond('ge.u32', hi_, exp_mask << 16)} and.b32 {x}, {x}, 65535;")
+            e(f"st.shared.b32 [{a_}+{box * kv_box}], {x};")
+        e(f"add.u32 {a_}, {a_}, 4;")
+        e(f"add.u32 {k_}, {k_}, 1;")
+        e(f"@{e.cond('lt.u32', k_, 32)} bra {l_c};")
+        e.label(l_n)
+        e(f"add.u32 {row}, {row}, 1;")
+        e(f"bra {l_r};")
+        e.label(l_d)
 
     def phase_of(x):
         """The phase of a ring barrier at tile x of the run: of two stages, or of one (bytes: the tile's parity)."""
@@ -646,6 +680,17 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
             wait_bar(e, f"{bars}+{PFULL + 8 * u}", o("and.b32", o("shr.u32", jj, 1), 1), err, ERR_MMA, l_end)
             e("tcgen05.fence::after_thread_sync;")
             pacc = e.cond("ne.u32", j, 0)
+            if scan:
+                bad = [e.r(), e.r()]
+                e(f"ld.shared.v2.b32 {{{bad[0]}, {bad[1]}}}, [{bars}+{VBAD + 8 * u}];")
+                l_fine = e.L("fine")
+                any_ = o("or.b32", bad[0], bad[1])
+                e(f"@{e.cond('eq.u32', any_, 0)} bra {l_fine};")
+                clear(stg[2 * u + 1], bad)
+                e(f"st.shared.v2.b32 [{bars}+{VBAD + 8 * u}], {{{zero2}, {zero2}}};")
+                e("fence.proxy.async.shared::cta;")
+                e(f"setp.eq.u32 {pacc}, {lane}, {lane};")       # O holds what the rows added, also before the first product
+                e.label(l_fine)
             for part in range(1 if p_f16 else 2):
                 for k in range(BKV // 16):
                     e(f"tcgen05.mma.cta_group::1.kind::f16 [{taddr}], [{scol[u]}+{BKV // 2 * part + 8 * k}], "
@@ -675,6 +720,93 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     jj_s = o("mov.u32", 0)
     out_cvt = "cvt.rn.f16x2.f32" if dtype == "f16" else "cvt.rn.bf16x2.f32"
     lift = 0.0 if not p_f16 else QUANT_LIFT if quant else F16_LIFT
+
+    def add_specials(S, j, jj, buf, ph, key0, sk, seen, pv_done):
+        """Tiles in which a key is seen by some rows only: finds the V rows that hold an infinity or a NaN (every warp
+        for itself), tells the issuing thread, and adds them to O for the rows that see them."""
+        l_out = e.L("clean")
+        part_ = e.cond("lt.s32", o("sub.s32", S.w["pos0"], key0), BKV - 1)       # some row's own position lies in it
+        if window is not None:
+            # or a row's window begins in it, and it is not all sinks
+            p1 = e.cond("ge.s32", o("sub.s32", o("sub.s32", S.w["pos1"], window), key0), 0)
+            p2 = e.cond("lt.s32", sk, BKV)
+            e(f"and.pred {p1}, {p1}, {p2};")
+            e(f"or.pred {part_}, {part_}, {p1};")
+        e(f"@!{part_} bra {l_out};")                            # the same for every thread
+        wait_bar_warp(e, f"{o('mad.lo.u32', buf, 16, bars)}+{FULL + 8}", ph, err, ERR_SOFTMAX, l_end)
+        va = o("mad.lo.u32", buf, 2 * kv_bytes, o("add.u32", sKV, kv_bytes))
+        bad = []
+        for h in range(2):
+            ra = o("mad.lo.u32", o("add.u32", lane, 32 * h), 128, va)
+            m_ = None
+            for box in range(boxes):
+                for i in range(8):
+                    d_ = [e.r() for _ in range(4)]
+                    e(f"ld.shared.v4.b32 {{{', '.join(d_)}}}, [{ra}+{box * kv_box + 16 * i}];")
+                    for x in d_:
+                        x = o("and.b32", x, "0x7FFF7FFF")
+                        m_ = x if m_ is None else o("max.u16x2", m_, x)
+            m_ = o("max.u32", o("and.b32", m_, 65535), o("shr.u32", m_, 16))
+            bad.append(o("vote.sync.ballot.b32", e.cond("ge.u32", m_, exp_mask), -1))
+        e(f"@{e.cond('eq.u32', o('or.b32', bad[0], bad[1]), 0)} bra {l_out};")
+        # O is this warp's to change between the previous product and this tile's; before the first it is 0
+        l_old, l_have = e.L("oldo"), e.L("haveo")
+        zf = o("mov.b32", 0)
+        e(f"@{e.cond('ne.u32', j, 0)} bra {l_old};")
+        for c in range(D // 32):
+            e(f"tcgen05.st.sync.aligned.32x32b.x32.b32 [{lanebase}+{32 * c}], {{{', '.join([zf] * 32)}}};")
+        e("tcgen05.wait::st.sync.aligned;")
+        e(f"bra {l_have};")
+        e.label(l_old)
+        pv_done(o("sub.u32", jj, 1), ERR_SOFTMAX, l_end)
+        e("tcgen05.fence::after_thread_sync;")
+        e.label(l_have)
+        p_w = e.cond("eq.u32", o("or.b32", quad, lane), 0)
+        e(f"@{p_w} st.shared.v2.b32 [{o('mad.lo.u32', buf, 8, bars)}+{VBAD}], {{{bad[0]}, {bad[1]}}};")
+        row = o("mov.u32", 0)
+        l_r, l_n = e.L("sp"), e.L("spn")
+        e.label(l_r)
+        low = e.cond("lt.u32", row, 32)
+        sh = o("and.b32", row, 31)
+        bit = o("and.b32", o("shr.u32", o("selp.b32", bad[0], bad[1], low), sh), 1)
+        e(f"@{e.cond('eq.u32', bit, 0)} bra {l_n};")            # the same for the warp
+        mine = e.cond("ne.u32", o("and.b32", o("shr.u32", o("selp.b32", seen[0], seen[1], low), sh), 1), 0)
+        col, sw = o("mov.u32", 0), o("and.b32", row, 7)
+        l_c = e.L("spc")
+        e.label(l_c)                                            # 32 columns at a time
+        oc = o("add.u32", lanebase, col)
+        regs = [e.r("f") for _ in range(32)]
+        e(f"tcgen05.ld.sync.aligned.32x32b.x32.b32 {{{', '.join(regs)}}}, [{oc}];")
+        e("tcgen05.wait::ld.sync.aligned;")
+        ra = o("mad.lo.u32", row, 128, va)
+        ra = o("mad.lo.u32", o("shr.u32", col, 6), kv_box, ra)
+        first = o("and.b32", o("shr.u32", col, 3), 7)           # 16-byte pieces of the 64-column box
+        for i in range(4):
+            d_ = [e.r() for _ in range(4)]
+            pa_ = o("mad.lo.u32", o("xor.b32", o("add.u32", first, i), sw), 16, ra)
+            e(f"ld.shared.v4.b32 {{{', '.join(d_)}}}, [{pa_}];")
+            for k, x in enumerate(d_):
+                for h in range(2):
+                    mag = o("and.b32", x, 0x7FFF << (16 * h))
+                    p_ = e.cond("ge.u32", mag, exp_mask << (16 * h))
+                    e(f"and.pred {p_}, {p_}, {mine};")
+                    # an infinity or a NaN as f32: the same sign and kind
+                    if dtype == "bf16":
+                        f_ = o("shl.b32", x, 16) if h == 0 else o("and.b32", x, -65536)
+                    else:
+                        sign = o("shl.b32", o("and.b32", x, 0x8000), 16) if h == 0 else o("and.b32", x, -(1 << 31))
+                        frac = o("shl.b32", o("and.b32", x, 0x3FF), 13) if h == 0 else o("shr.u32", o("and.b32", x,
+                                                                                                    0x3FF0000), 3)
+                        f_ = o("or.b32", o("or.b32", sign, 0x7F800000), frac)
+                    e(f"@{p_} add.f32 {regs[8 * i + 2 * k + h]}, {regs[8 * i + 2 * k + h]}, {o('mov.b32', f_, cls='f')};")
+        e(f"tcgen05.st.sync.aligned.32x32b.x32.b32 [{oc}], {{{', '.join(regs)}}};")
+        e("tcgen05.wait::st.sync.aligned;")
+        e(f"add.u32 {col}, {col}, 32;")
+        e(f"@{e.cond('lt.u32', col, D)} bra {l_c};")
+        e.label(l_n)
+        e(f"add.u32 {row}, {row}, 1;")
+        e(f"@{e.cond('lt.u32', row, BKV)} bra {l_r};")
+        e.label(l_out)
 
     def softmax(S):
         w, pos0, pos1, vrows = S.w, S.w["pos0"], S.w["pos1"], S.P.vrows
@@ -726,6 +858,11 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         mref, lsum = o("mov.b32", "0fFF800000", cls="f"), o("mov.b32", "0f00000000", cls="f")
         j, jj = o("mov.u32", 0), jj_s
         l_sj, l_sdone, l_noepi = e.L("sj"), e.L("sdone"), e.L("noepi")
+
+        def pv_done(k, code, bail):
+            br = o("mad.lo.u32", o("and.b32", k, 1), 8, bars)
+            wait_bar_warp(e, f"{br}+{PFREE}", o("and.b32", o("shr.u32", k, 1), 1), err, code, bail)
+
         e.label(l_sj)
         e(f"@{e.cond('ge.u32', j, S.nb)} bra {l_sdone};")
         buf = o("and.b32", jj, 1)
@@ -825,6 +962,8 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
                         e(f"@{pz} st.shared.v4.b32 [{ra}+{box * kv_box + 16 * i}], {{{z_}, {z_}, {z_}, {z_}}};")
             e("fence.proxy.async.shared::cta;")
             e.label(l_vok)
+        if scan:
+            add_specials(S, j, jj, buf, ph, key0, sk, (m0, m1), pv_done)
         # the row's maximum: 8 chains of three-input maxima
         lvl = [e.r("f") for _ in range(8)]
         for k in range(8):
@@ -916,10 +1055,6 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         # the lazy rescale of O, once the previous product has completed
         l_nore = e.L("norescale")
         e(f"@!{anyneed} bra {l_nore};")
-
-        def pv_done(k, code, bail):
-            br = o("mad.lo.u32", o("and.b32", k, 1), 8, bars)
-            wait_bar_warp(e, f"{br}+{PFREE}", o("and.b32", o("shr.u32", k, 1), 1), err, code, bail)
 
         pv_done(o("sub.u32", jj, 1), ERR_SOFTMAX, l_end)
         e("tcgen05.fence::after_thread_sync;")

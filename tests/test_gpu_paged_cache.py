@@ -9,7 +9,7 @@ from emmy_ptx_b200.compiler import compile_graph
 from emmy_ptx_b200.ir import Graph
 from emmy_ptx_b200.runtime import Executable
 from tests import pagedref as R
-from tests.test_paged_cache import ATTENDS, FORMS, READS, SPREAD, TENSOR, WRITES, awkward_rows, broken_table, form_opts, same
+from tests.test_paged_cache import ATTENDS, FORMS, READS, SPECIAL, SPREAD, TENSOR, WRITES, awkward_rows, broken_table, form_opts, same, with_specials
 
 pytestmark = pytest.mark.gpu
 
@@ -44,6 +44,19 @@ def test_paged_attention(form, case, dtype, quant):
     assert kinds[0] == FORMS[form]
     ref, bound, _ = R.attention_ref(t, page, window, sinks)
     R.check(got["O"], ref, bound, form)
+
+
+@pytest.mark.parametrize("form", ["rows", "tiles"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("case", SPECIAL, ids=lambda c: "x".join(map(str, c[:5])))
+def test_infinities_and_nans_reach_only_rows_that_see_them(case, dtype, form):
+    C, H, hk, d, n, window, sinks, _ = case
+    t, pages = with_specials(case, dtype, 16)
+    p = irgen.paged_attention_ir(1, C, H, hk, d, pages, 16, t["table"].shape[1], dtype, False, window, sinks)
+    ref, bound, _ = R.attention_ref(t, 16, window, sinks)
+    for ctas in (0, 2):
+        got, _ = go(p, t, {"paged_rows": 64 if form == "rows" else 0, "paged_ctas": ctas, "paged_min_tiles": 1})
+        R.check(got["O"], ref, bound, form, inf_or_nan=True)
 
 
 @pytest.mark.parametrize("quant", [False, True])

@@ -259,6 +259,47 @@ def test_paged_attention_runs_over_many_units(form, case, ctas, quant):
     R.check(got["O"], ref, bound, f"{form} {ctas}")
 
 
+SPECIAL = [
+    # chunk, heads, kv_heads, dim, lens, window, sinks, positions of V rows with an infinity or a NaN
+    (5, 2, 1, 64, 70, None, 0, [65, 67, 69]),
+    (3, 3, 1, 128, 3, None, 0, [0, 1, 2]),                           # the first tile, before any product
+    (6, 2, 2, 64, 200, 70, 3, [1, 127, 128, 131, 199]),                # the window begins for some rows only
+    (1, 2, 1, 64, 130, 70, 3, [2, 59, 60, 129]),                       # one token: keys behind the window are not read
+    (9, 1, 1, 64, 150, 5, 64, [3, 64, 138, 140, 143, 145]),
+]
+
+
+def with_specials(case, dtype, page):
+    """Inputs with infinities and NaNs in the values (and a NaN key) of keys that some rows see and others do not."""
+    C, H, hk, d, n, window, sinks, where = case
+    t, pages = R.make("attend", 1, hk, d, page, -(-n // page), [n], [C], chunk=C, heads=H, dtype=dtype, seed=n)
+    for i, pos in enumerate(where):
+        pg = int(t["table"][0, pos // page])
+        t["VC"][pg, :, pos % page, 3 * i] = (math.inf, -math.inf, math.nan)[i % 3]
+        t["VC"][pg, 0, pos % page, 3] = math.inf                      # the same column with both signs
+    if C > 1:                                                            # seen by the last token alone
+        t["KC"][int(t["table"][0, (n - 1) // page]), 0, (n - 1) % page, 5] = math.nan
+    return t, pages
+
+
+@pytest.mark.parametrize("form", ["rows", "tiles", "oracle"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("case", SPECIAL, ids=lambda c: "x".join(map(str, c[:5])))
+def test_infinities_and_nans_reach_only_rows_that_see_them(case, dtype, form):
+    C, H, hk, d, n, window, sinks, _ = case
+    t, pages = with_specials(case, dtype, 16)
+    p = irgen.paged_attention_ir(1, C, H, hk, d, pages, 16, t["table"].shape[1], dtype, False, window, sinks)
+    ref, bound, _ = R.attention_ref(t, 16, window, sinks)
+    for ctas in (0,) if form == "oracle" else (0, 2):
+        if form == "oracle":
+            got = by_oracle(p, t)
+        else:
+            got, code, _ = PE.run(p, t, {"paged_rows": 64 if form == "rows" else 0, "paged_ctas": ctas, "paged_min_tiles": 1})
+            assert code == 0
+        assert torch.isfinite(got["O"]).any()
+        R.check(got["O"], ref, bound, form, inf_or_nan=form != "oracle")
+
+
 @pytest.mark.parametrize("missing", range(0, 17, 2))
 def test_paged_attention_a_missing_page_masks_no_other(missing):
     # the masks of a ring stage that held a missing page must be gone when the next block comes to it
