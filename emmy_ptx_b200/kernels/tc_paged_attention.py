@@ -16,9 +16,10 @@ CTA a unit instead.
 
 **Roles.**  One thread issues the ``tcgen05.mma``: S(j+1) = Q K_(j+1)^T into one of two 64-column score buffers,
 then O += P(j) V_j.  Four softmax warps hold one row a thread; warps without a row take no part.  A warp loads by
-TMA, one box per page of the tile (at most 64 rows), with the page numbers fetched 32 at a time one batch ahead.  For
-a cache of bytes the boxes land in a raw ring, and two warps convert them into the tiles the products read: with
-0x64 as its upper half a byte b is the f16 number 1024 + b, less 1152 it is b - 128, exactly.  Each quarter warp
+TMA, one box per page of the tile (at most 64 rows), with the page numbers fetched 32 at a time one batch ahead.
+For 16-bit caches one more warp makes a V tile fit for the product (see what is masked): done by the softmax warps, that
+took 86 us in place of 61 for 4 x 1111 tokens with a window of 1024 (24 heads of 64 on 4, f16).  For a cache of bytes
+the boxes land in a raw ring, and two warps convert them into the tiles the products read: with 0x64 as its upper half a byte b is the f16 number 1024 + b, less 1152 it is b - 128, exactly.  Each quarter warp
 takes 64 bytes of rows r and r ^ 5, which the raw ring's swizzle and the tile's put into different banks.  The
 keys' scales multiply the scores' columns, the values' scales multiply P.
 
@@ -67,6 +68,7 @@ SFULL = EMPTY + 8 * STAGES
 PFULL = SFULL + 16
 PFREE = PFULL + 16
 SLOT = PFREE + 16
+VOK = SLOT + 8                   # two barriers: a V tile is fit for the product (16-bit caches)
 KMASK = 192
 KSC = 256
 VSC = KSC + 4 * BKV * 4
@@ -221,7 +223,7 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     if quant:
         threads, soft0, mma_warp = 256, 4, 1
     else:
-        threads, soft0, mma_warp = 192, 2, 1
+        threads, soft0, mma_warp = 224, 2, 1
     idesc_qk = idesc_f16(ROWS, BKV, False, False, half=half)
     idesc_pv = idesc_f16(ROWS, D, False, True, half=p_f16)
     kdesc_hi = smem_desc_hi(16, 1024)
@@ -351,8 +353,8 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         e(f"mbarrier.init.shared::cta.b64 [{bars}+{SFULL + 8 * u}], 1;")
         e(f"mbarrier.init.shared::cta.b64 [{bars}+{PFULL + 8 * u}], 4;")
         e(f"mbarrier.init.shared::cta.b64 [{bars}+{PFREE + 8 * u}], 1;")
-    if scan:
-        e(f"st.shared.v4.b32 [{bars}+{VBAD}], {{{', '.join([o('mov.b32', 0)] * 4)}}};")
+        if not quant:
+            e(f"mbarrier.init.shared::cta.b64 [{bars}+{VOK + 8 * u}], 1;")
     e("fence.mbarrier_init.release.cluster;")
     e("fence.proxy.async.shared::cta;")
     e.label(l_init)
@@ -366,8 +368,10 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     e("bar.sync 0;")
     e("tcgen05.fence::after_thread_sync;")
     taddr = o("ld.shared.b32", f"[{bars}+{SLOT}]")
-    l_end, l_mma, l_soft = e.L("end"), e.L("mma"), e.L("soft")
+    l_end, l_mma, l_soft, l_help = e.L("end"), e.L("mma"), e.L("soft"), e.L("help")
     e(f"@{p_mma} bra {l_mma};")
+    if not quant:
+        e(f"@{e.cond('eq.u32', warp, 6)} bra {l_help};")
     e(f"@{e.cond('ge.u32', warp, soft0)} bra {l_soft};")
     def valid(pg):
         return e.cond("lt.u32", pg, pages)
@@ -587,6 +591,88 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
 
         each_segment("cv", convert, l_end)
 
+    else:
+        # ---------------------------------------------------------------- V made fit for the product (warp 6)
+        e.label(l_help)
+        p_l0h = e.cond("eq.u32", lane, 0)
+        jj_h = o("mov.u32", 0)
+        # a lane takes a row's 16-byte pieces in an order of its own, so that eight lanes fill all banks
+        piece = [o("xor.b32", o("shl.b32", o("and.b32", lane, 7), 4), 16 * i) for i in range(8)]
+
+        def partial(S, key0):
+            """Whether some rows of the unit see a key of the tile that others do not (the same for every thread): a
+            row's own position lies in it, or a row's window begins in it and it is not all sinks."""
+            p_ = e.cond("lt.s32", o("sub.s32", S.w["pos0"], key0), BKV - 1)
+            if window is not None:
+                p1 = e.cond("ge.s32", o("sub.s32", o("sub.s32", S.w["pos1"], window), key0), 0)
+                p2 = e.cond("lt.s32", o("sub.s32", sinks, key0), BKV)
+                e(f"and.pred {p1}, {p1}, {p2};")
+                e(f"or.pred {p_}, {p_}, {p1};")
+            return p_
+
+        def help_(S):
+            """Zeroes the rows of V that no row of the unit sees (past its last token, between sinks and window), and
+            notes the rows that hold an infinity or a NaN where some rows see a key and others do not."""
+            j, jj = o("mov.u32", 0), jj_h
+            l_top, l_seg = e.L("hp"), e.L("hpseg")
+            e.label(l_top)
+            e(f"@{e.cond('ge.u32', j, S.nb)} bra {l_seg};")
+            u_, ph = o("and.b32", jj, 1), o("and.b32", o("shr.u32", jj, 1), 1)
+            key0 = o("shl.b32", S.tile_of(j), 6)
+            bad = [o("mov.b32", 0), o("mov.b32", 0)]
+            l_vok, l_clean = e.L("vok"), e.L("clean")
+            sb = o("mad.lo.u32", u_, 16, bars)
+            wait_bar_warp(e, f"{sb}+{FULL + 8}", ph, err, ERR_LOAD, l_end)
+            va = o("mad.lo.u32", u_, 2 * kv_bytes, o("add.u32", sKV, kv_bytes))
+            vlim = o("sub.s32", S.w["pos1"], key0)
+            pv_ = e.cond("ge.s32", vlim, BKV - 1)
+            if window is not None:
+                lo_k, sk = o("sub.s32", S.w["lo"], key0), o("sub.s32", sinks, key0)
+                p1_, p2_ = e.cond("le.s32", lo_k, 0), e.cond("ge.s32", sk, BKV)
+                e(f"or.pred {p1_}, {p1_}, {p2_};")
+                e(f"and.pred {pv_}, {pv_}, {p1_};")
+            e(f"@{pv_} bra {l_vok};")
+            z_ = o("mov.b32", 0)
+            for h in range(2):
+                r_ = o("add.u32", lane, 32 * h)
+                pz = e.cond("gt.s32", r_, vlim)
+                if window is not None:
+                    pa, pb = e.cond("lt.s32", r_, lo_k), e.cond("ge.s32", r_, sk)
+                    e(f"and.pred {pa}, {pa}, {pb};")
+                    e(f"or.pred {pz}, {pz}, {pa};")
+                ra = o("mad.lo.u32", r_, 128, va)
+                for i in range(8):
+                    pa_ = o("add.u32", ra, piece[i])
+                    for box in range(boxes):
+                        e(f"@{pz} st.shared.v4.b32 [{pa_}+{box * kv_box}], {{{z_}, {z_}, {z_}, {z_}}};")
+            e("fence.proxy.async.shared::cta;")
+            e.label(l_vok)
+            if scan:
+                e(f"@!{partial(S, key0)} bra {l_clean};")
+                for h in range(2):
+                    ra = o("mad.lo.u32", o("add.u32", lane, 32 * h), 128, va)
+                    m_ = None
+                    for i in range(8):
+                        pa_ = o("add.u32", ra, piece[i])
+                        for box in range(boxes):
+                            d_ = [e.r() for _ in range(4)]
+                            e(f"ld.shared.v4.b32 {{{', '.join(d_)}}}, [{pa_}+{box * kv_box}];")
+                            for x in d_:
+                                x = o("and.b32", x, "0x7FFF7FFF")
+                                m_ = x if m_ is None else o("max.u16x2", m_, x)
+                    m_ = o("max.u32", o("and.b32", m_, 65535), o("shr.u32", m_, 16))
+                    e(f"vote.sync.ballot.b32 {bad[h]}, {e.cond('ge.u32', m_, exp_mask)}, -1;")
+                e.label(l_clean)
+                e(f"@{p_l0h} st.shared.v2.b32 [{o('mad.lo.u32', u_, 8, bars)}+{VBAD}], {{{bad[0]}, {bad[1]}}};")
+            e("bar.warp.sync -1;")
+            e(f"@{p_l0h} mbarrier.arrive.shared::cta.b64 _, [{o('mad.lo.u32', u_, 8, bars)}+{VOK}];")
+            e(f"add.u32 {j}, {j}, 1;")
+            e(f"add.u32 {jj}, {jj}, 1;")
+            e(f"bra {l_top};")
+            e.label(l_seg)
+
+        each_segment("h", help_, l_end)
+
     # ------------------------------------------------------------------ MMA issue (one thread)
     e.label(l_mma)
     e(f"@{e.cond('ne.u32', lane, 0)} bra {l_end};")
@@ -623,7 +709,6 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         commit(SFULL + 8 * u)
 
     jj_m, segs = o("mov.u32", 0), o("mov.u32", 0)
-    zero2 = o("mov.u32", 0)
 
     def clear(tile_addr, bad):
         """Writes 0 over the infinities and NaNs of the V tile's rows ``bad`` (two words; one thread, a rare path)."""
@@ -677,6 +762,8 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
             qk(1 - u)
             e.label(l_nok)
             ring(ring_v[u], phase_of(jj))
+            if not quant:
+                wait_bar(e, f"{bars}+{VOK + 8 * u}", phase_of(jj), err, ERR_MMA, l_end)
             wait_bar(e, f"{bars}+{PFULL + 8 * u}", o("and.b32", o("shr.u32", jj, 1), 1), err, ERR_MMA, l_end)
             e("tcgen05.fence::after_thread_sync;")
             pacc = e.cond("ne.u32", j, 0)
@@ -687,7 +774,6 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
                 any_ = o("or.b32", bad[0], bad[1])
                 e(f"@{e.cond('eq.u32', any_, 0)} bra {l_fine};")
                 clear(stg[2 * u + 1], bad)
-                e(f"st.shared.v2.b32 [{bars}+{VBAD + 8 * u}], {{{zero2}, {zero2}}};")
                 e("fence.proxy.async.shared::cta;")
                 e(f"setp.eq.u32 {pacc}, {lane}, {lane};")       # O holds what the rows added, also before the first product
                 e.label(l_fine)
@@ -721,34 +807,22 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     out_cvt = "cvt.rn.f16x2.f32" if dtype == "f16" else "cvt.rn.bf16x2.f32"
     lift = 0.0 if not p_f16 else QUANT_LIFT if quant else F16_LIFT
 
-    def add_specials(S, j, jj, buf, ph, key0, sk, seen, pv_done):
-        """Tiles in which a key is seen by some rows only: finds the V rows that hold an infinity or a NaN (every warp
-        for itself), tells the issuing thread, and adds them to O for the rows that see them."""
-        l_out = e.L("clean")
-        part_ = e.cond("lt.s32", o("sub.s32", S.w["pos0"], key0), BKV - 1)       # some row's own position lies in it
-        if window is not None:
-            # or a row's window begins in it, and it is not all sinks
-            p1 = e.cond("ge.s32", o("sub.s32", o("sub.s32", S.w["pos1"], window), key0), 0)
-            p2 = e.cond("lt.s32", sk, BKV)
-            e(f"and.pred {p1}, {p1}, {p2};")
-            e(f"or.pred {part_}, {part_}, {p1};")
-        e(f"@!{part_} bra {l_out};")                            # the same for every thread
-        wait_bar_warp(e, f"{o('mad.lo.u32', buf, 16, bars)}+{FULL + 8}", ph, err, ERR_SOFTMAX, l_end)
+    def add_specials(S, j, jj, buf, ph, key0, *rest):
+        """Tiles in which a key is seen by some rows only: takes the rare path when the V rows hold an infinity or a NaN.
+        Returns what emits that path, behind the loop: it adds them to O for the rows that see them; it borrows the
+        scores' registers and loads them again."""
+        l_out, l_rare = e.L("clean"), e.L("rare")
+        e(f"@!{partial(S, key0)} bra {l_out};")
+        wait_bar_warp(e, f"{o('mad.lo.u32', buf, 8, bars)}+{VOK}", ph, err, ERR_SOFTMAX, l_end)
+        bad = [e.r(), e.r()]
+        e(f"ld.shared.v2.b32 {{{bad[0]}, {bad[1]}}}, [{o('mad.lo.u32', buf, 8, bars)}+{VBAD}];")
+        e(f"@{e.cond('ne.u32', o('or.b32', bad[0], bad[1]), 0)} bra {l_rare};")
+        e.label(l_out)
+        return lambda: rare(S, j, jj, buf, *rest, bad, l_rare, l_out)
+
+    def rare(S, j, jj, buf, seen, pv_done, load_scores, bad, l_rare, l_out):
+        e.label(l_rare)
         va = o("mad.lo.u32", buf, 2 * kv_bytes, o("add.u32", sKV, kv_bytes))
-        bad = []
-        for h in range(2):
-            ra = o("mad.lo.u32", o("add.u32", lane, 32 * h), 128, va)
-            m_ = None
-            for box in range(boxes):
-                for i in range(8):
-                    d_ = [e.r() for _ in range(4)]
-                    e(f"ld.shared.v4.b32 {{{', '.join(d_)}}}, [{ra}+{box * kv_box + 16 * i}];")
-                    for x in d_:
-                        x = o("and.b32", x, "0x7FFF7FFF")
-                        m_ = x if m_ is None else o("max.u16x2", m_, x)
-            m_ = o("max.u32", o("and.b32", m_, 65535), o("shr.u32", m_, 16))
-            bad.append(o("vote.sync.ballot.b32", e.cond("ge.u32", m_, exp_mask), -1))
-        e(f"@{e.cond('eq.u32', o('or.b32', bad[0], bad[1]), 0)} bra {l_out};")
         # O is this warp's to change between the previous product and this tile's; before the first it is 0
         l_old, l_have = e.L("oldo"), e.L("haveo")
         zf = o("mov.b32", 0)
@@ -761,8 +835,6 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         pv_done(o("sub.u32", jj, 1), ERR_SOFTMAX, l_end)
         e("tcgen05.fence::after_thread_sync;")
         e.label(l_have)
-        p_w = e.cond("eq.u32", o("or.b32", quad, lane), 0)
-        e(f"@{p_w} st.shared.v2.b32 [{o('mad.lo.u32', buf, 8, bars)}+{VBAD}], {{{bad[0]}, {bad[1]}}};")
         row = o("mov.u32", 0)
         l_r, l_n = e.L("sp"), e.L("spn")
         e.label(l_r)
@@ -775,7 +847,7 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         l_c = e.L("spc")
         e.label(l_c)                                            # 32 columns at a time
         oc = o("add.u32", lanebase, col)
-        regs = [e.r("f") for _ in range(32)]
+        regs = s_[:32]
         e(f"tcgen05.ld.sync.aligned.32x32b.x32.b32 {{{', '.join(regs)}}}, [{oc}];")
         e("tcgen05.wait::ld.sync.aligned;")
         ra = o("mad.lo.u32", row, 128, va)
@@ -806,7 +878,9 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         e.label(l_n)
         e(f"add.u32 {row}, {row}, 1;")
         e(f"@{e.cond('lt.u32', row, BKV)} bra {l_r};")
-        e.label(l_out)
+        load_scores()
+        e("tcgen05.wait::ld.sync.aligned;")
+        e(f"bra {l_out};")
 
     def softmax(S):
         w, pos0, pos1, vrows = S.w, S.w["pos0"], S.w["pos1"], S.P.vrows
@@ -872,8 +946,12 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         key0 = o("shl.b32", S.tile_of(j), 6)
         wait_bar_warp(e, f"{bb}+{SFULL}", ph, err, ERR_SOFTMAX, l_end)
         e("tcgen05.fence::after_thread_sync;")
-        for c in range(BKV // 32):
-            e(f"tcgen05.ld.sync.aligned.32x32b.x32.b32 {{{', '.join(s_[32 * c:32 * c + 32])}}}, [{sc_col}+{32 * c}];")
+
+        def load_scores():
+            for c in range(BKV // 32):
+                e(f"tcgen05.ld.sync.aligned.32x32b.x32.b32 {{{', '.join(s_[32 * c:32 * c + 32])}}}, [{sc_col}+{32 * c}];")
+
+        load_scores()
         slot_a = o("and.b32", jj, 3)
         ma = o("mad.lo.u32", slot_a, 8, bars)
         km = [e.r(), e.r()]
@@ -930,40 +1008,15 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         e(f"mov.b64 {pages_}, {{{km[0]}, {km[1]}}};")
         bits = o("and.b64", bits, pages_, cls="rd")
         e(f"mov.b64 {{{m0}, {m1}}}, {bits};")
+        e.label(l_seen)
+        if scan:
+            out_of_line = add_specials(S, j, jj, buf, ph, key0, (m0, m1), pv_done, load_scores)
+        l_kept = e.L("kept")
+        e(f"@{v_all} bra {l_kept};")
         for c in range(BKV):
             t_ = o("and.b32", (m0, m1)[c // 32], 1 << (c % 32) if c % 32 < 31 else -(1 << 31))
             e(f"@{e.cond('eq.u32', t_, 0)} mov.b32 {s_[c]}, 0fFF800000;")
-        e.label(l_seen)
-        if not quant:
-            # rows of V that no row of this CTA sees (past its last token, or between sinks and window) may
-            # hold anything: zero them before the product multiplies them by P = 0
-            l_vok = e.L("vok")
-            vlim = o("sub.s32", pos1, key0)
-            pv_ = e.cond("ge.s32", vlim, BKV - 1)
-            if window is not None:
-                lo_k = o("sub.s32", w["lo"], key0)
-                p1_, p2_ = e.cond("le.s32", lo_k, 0), e.cond("ge.s32", sk, BKV)
-                e(f"or.pred {p1_}, {p1_}, {p2_};")
-                e(f"and.pred {pv_}, {pv_}, {p1_};")
-            e(f"@{pv_} bra {l_vok};")                               # the same for every thread
-            wait_bar_warp(e, f"{o('mad.lo.u32', buf, 16, bars)}+{FULL + 8}", ph, err, ERR_SOFTMAX, l_end)
-            va = o("mad.lo.u32", buf, 2 * kv_bytes, o("add.u32", sKV, kv_bytes))
-            z_ = o("mov.b32", 0)
-            for h in range(2):
-                r_ = o("add.u32", lane, 32 * h)
-                pz = e.cond("gt.s32", r_, vlim)
-                if window is not None:
-                    pa, pb = e.cond("lt.s32", r_, lo_k), e.cond("ge.s32", r_, sk)
-                    e(f"and.pred {pa}, {pa}, {pb};")
-                    e(f"or.pred {pz}, {pz}, {pa};")
-                ra = o("mad.lo.u32", r_, 128, va)
-                for box in range(boxes):
-                    for i in range(8):
-                        e(f"@{pz} st.shared.v4.b32 [{ra}+{box * kv_box + 16 * i}], {{{z_}, {z_}, {z_}, {z_}}};")
-            e("fence.proxy.async.shared::cta;")
-            e.label(l_vok)
-        if scan:
-            add_specials(S, j, jj, buf, ph, key0, sk, (m0, m1), pv_done)
+        e.label(l_kept)
         # the row's maximum: 8 chains of three-input maxima
         lvl = [e.r("f") for _ in range(8)]
         for k in range(8):
@@ -1073,6 +1126,8 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         e(f"add.u32 {j}, {j}, 1;")
         e(f"add.u32 {jj}, {jj}, 1;")
         e(f"bra {l_sj};")
+        if scan:
+            out_of_line()
 
         # epilogue: after the last product, O / l as the output type, or the part's O, m and l in f32
         e.label(l_sdone)
