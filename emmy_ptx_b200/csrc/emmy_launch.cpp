@@ -330,13 +330,9 @@ int emmy_launch(void* function, const uint32_t grid[3], const uint32_t block[3],
   return emmy_launch_ex(function, grid, block, cluster, dyn_smem, stream, args, nargs, 0);
 }
 
-int emmy_launch_ex(void* function, const uint32_t grid[3], const uint32_t block[3],
-                   const uint32_t cluster[3], uint32_t dyn_smem, void* stream, void** args,
-                   uint32_t nargs, uint32_t flags) {
-  if (!function || !grid || !block) return fail(EMMY_ERR_BAD_ARG, "null function/grid/block");
-  if (flags & ~static_cast<uint32_t>(EMMY_LAUNCH_PDL)) return fail(EMMY_ERR_BAD_ARG, "unknown launch flags 0x%x", flags);
-  if (nargs && !args) return fail(EMMY_ERR_BAD_ARG, "null args with nargs > 0");
-  if (int rc = ready()) return rc;
+namespace {
+int launch_here(void* function, const uint32_t grid[3], const uint32_t block[3], const uint32_t cluster[3],
+                uint32_t dyn_smem, void* stream, void** args, uint32_t flags) {
   CUlaunchConfig cfg;
   std::memset(&cfg, 0, sizeof(cfg));
   cfg.gridDimX = grid[0];
@@ -370,6 +366,17 @@ int emmy_launch_ex(void* function, const uint32_t grid[3], const uint32_t block[
   }
   return cu(g_drv.LaunchKernelEx(&cfg, static_cast<CUfunction>(function), args, nullptr),
             "cuLaunchKernelEx");
+}
+}  // namespace
+
+int emmy_launch_ex(void* function, const uint32_t grid[3], const uint32_t block[3],
+                   const uint32_t cluster[3], uint32_t dyn_smem, void* stream, void** args,
+                   uint32_t nargs, uint32_t flags) {
+  if (!function || !grid || !block) return fail(EMMY_ERR_BAD_ARG, "null function/grid/block");
+  if (flags & ~static_cast<uint32_t>(EMMY_LAUNCH_PDL)) return fail(EMMY_ERR_BAD_ARG, "unknown launch flags 0x%x", flags);
+  if (nargs && !args) return fail(EMMY_ERR_BAD_ARG, "null args with nargs > 0");
+  if (int rc = ready()) return rc;
+  return launch_here(function, grid, block, cluster, dyn_smem, stream, args, flags);
 }
 
 int emmy_launch_u64(void* function, const uint32_t grid[3], const uint32_t block[3],
@@ -428,6 +435,7 @@ struct Plan {
   uint32_t align[EMMY_PLAN_MAX_PARAMS];
   PlanTmap tmaps[EMMY_PLAN_MAX_TMAPS];
   uint64_t tail;
+  CUcontext ctx;
 };
 }  // namespace
 
@@ -449,6 +457,7 @@ int emmy_plan_create(void* function, const uint32_t grid[3], const uint32_t bloc
   p->dyn_smem = dyn_smem;
   p->flags = flags;
   p->nparams = nparams;
+  p->ctx = g_ctx;
   for (uint32_t i = 0; i < nparams; ++i) p->align[i] = align[i];
   *plan = p;
   return 0;
@@ -510,7 +519,16 @@ int emmy_plan_launch(void* plan, const uint64_t* params, uint32_t nparams, void*
     vals[nparams] = p->tail;
     args[n++] = &vals[nparams];
   }
-  return emmy_launch_ex(p->function, p->grid, p->block, p->cluster, p->dyn_smem, stream, args, n, p->flags);
+  if (!p->ctx) return fail(EMMY_ERR_NOT_INIT, "emmy_init() had not been called when the plan was made");
+  // in the plan's context, whatever the thread's is, and back to that one
+  CUcontext cur = nullptr;
+  if (int rc = cu(g_drv.CtxGetCurrent(&cur), "cuCtxGetCurrent")) return rc;
+  if (cur != p->ctx)
+    if (int rc = cu(g_drv.CtxSetCurrent(p->ctx), "cuCtxSetCurrent")) return rc;
+  int rc = launch_here(p->function, p->grid, p->block, p->cluster, p->dyn_smem, stream, args, p->flags);
+  if (cur && cur != p->ctx)
+    if (int back = cu(g_drv.CtxSetCurrent(cur), "cuCtxSetCurrent")) return rc ? rc : back;
+  return rc;
 }
 
 int emmy_plan_destroy(void* plan) {

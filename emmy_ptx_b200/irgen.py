@@ -801,8 +801,8 @@ def paged_attention_ir(batch: int, chunk: int, heads: int, kv_heads: int, dim: i
     if sinks and window is None:
         raise ValueError("paged_attention_ir: sinks are the first tokens that stay visible behind a window")
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    if not (math.isfinite(scale) and scale > 0):
-        raise ValueError(f"paged_attention_ir needs a finite scale above 0, not {scale!r}")
+    if not 2.0 ** -64 <= scale <= 2.0 ** 64:                    # times log2(e) a normal f32; a NaN fails too
+        raise ValueError(f"paged_attention_ir needs a scale from 2^-64 to 2^64, not {scale!r}")
     cells = _cells("paged_attention_ir", batch, chunk, heads, 32)
     per, group = dim // 32, heads // kv_heads
     P = range(per)

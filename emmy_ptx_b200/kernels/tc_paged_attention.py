@@ -19,9 +19,10 @@ then O += P(j) V_j.  Four softmax warps hold one row a thread; warps without a r
 TMA, one box per page of the tile (at most 64 rows), with the page numbers fetched 32 at a time one batch ahead.
 For 16-bit caches one more warp makes a V tile fit for the product (see what is masked): done by the softmax warps, that
 took 86 us in place of 61 for 4 x 1111 tokens with a window of 1024 (24 heads of 64 on 4, f16).  For a cache of bytes
-the boxes land in a raw ring, and two warps convert them into the tiles the products read: with 0x64 as its upper half a byte b is the f16 number 1024 + b, less 1152 it is b - 128, exactly.  Each quarter warp
-takes 64 bytes of rows r and r ^ 5, which the raw ring's swizzle and the tile's put into different banks.  The
-keys' scales multiply the scores' columns, the values' scales multiply P.
+the boxes land in a raw ring, and two warps convert them into the tiles the products read: with 0x64 as its upper
+half a byte b is the f16 number 1024 + b, less 1152 it is b - 128, exactly.  Each quarter warp takes 64 bytes of rows
+r and r ^ 5, which the raw ring's swizzle and the tile's put into different banks.  The keys' scales multiply the
+scores' columns, the values' scales multiply P.
 
 **Numerics.**  The score buffers, the running reference and sum, and O are f32.  P is rounded for the tensor core:
 f16 caches take f16 P, to nearest (2^-11), with 2^7 put on the exponent so that small weights keep their bits;

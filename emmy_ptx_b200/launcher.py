@@ -244,9 +244,8 @@ class Device:
         return h
 
     def launch_plan(self, plan, params, stream: int) -> None:
-        """Launch ``plan`` with ``params`` (a ctypes array of 64-bit values) on ``stream``."""
-        if Device._active != self.index:
-            self._use()
+        """Launch ``plan`` with ``params`` (a ctypes array of 64-bit values) on ``stream``, in the context the plan
+        was made in (the thread's own stays current)."""
         rc = self.lib.emmy_plan_launch(plan, params, len(params), stream)
         if rc:
             check(rc, "emmy_plan_launch")

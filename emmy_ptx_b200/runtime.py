@@ -111,6 +111,8 @@ class Executable:
         every entry.  Scratch is the call's own (torch's allocator, so a captured call's belongs to its
         graph): calls of one Executable may overlap on the GPU as long as what they write does not."""
         import torch
+        if not self.plans:
+            raise ValueError(f"kernel {self.records[0]['entry']!r} was closed")
         ptrs = {}
         for name, dtype, shape in self._args:
             t = tensors.get(name)

@@ -218,3 +218,199 @@ def test_a_serving_step_captured_and_replayed(quant):
             same(g[n].cpu(), host[n], f"{n} step {step}")
     for ex in steps:
         ex.check()
+
+
+# ---- calls that overlap, other threads, sizes past 32 bits -------------------------------------
+
+
+def decode_case(quant=False, seed=0, rows=64, B=3, C=1, lens=(700, 90, 1500), H=4, hk=2, d=64, page=16):
+    mp = -(-max(lens) // page)
+    t, pages = R.make("attend", B, hk, d, page, mp, list(lens), [min(C, n) for n in lens], chunk=C, heads=H, quant=quant,
+                      seed=seed)
+    p = irgen.paged_attention_ir(B, C, H, hk, d, pages, page, mp, "bf16", quant)
+    return t, build(p, {"paged_rows": rows, "paged_ctas": 9, "paged_min_tiles": 1})
+
+
+@pytest.mark.parametrize("rows", [0, 64])
+def test_calls_of_one_executable_overlap(rows):
+    """Two streams run one Executable at a time, each with its own inputs, output and (the call's own) scratch."""
+    t, ex = decode_case(rows=rows)
+    assert ex.records[0]["scratch"]
+    sets = [on_gpu(t), on_gpu({**t, "Q": torch.randn(t["Q"].shape).to(t["Q"].dtype)})]
+    ex(sets[0]), ex(sets[1])
+    torch.cuda.synchronize()
+    want = [g["O"].clone() for g in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(20):
+        for g in sets:
+            g["O"].fill_(7)
+        torch.cuda.synchronize()
+        for _ in range(8):
+            for g, s in zip(sets, streams):
+                with torch.cuda.stream(s):
+                    ex(g)
+        torch.cuda.synchronize()
+        for g, w in zip(sets, want):
+            assert torch.equal(g["O"], w)
+    ex.check()
+
+
+def test_two_graphs_of_one_executable_replay_at_once():
+    t, ex = decode_case()
+    sets = [on_gpu(t), on_gpu({**t, "Q": torch.randn(t["Q"].shape).to(t["Q"].dtype)})]
+    want, graphs, streams = [], [], []
+    for g in sets:
+        ex(g)
+        torch.cuda.synchronize()
+        want.append(g["O"].clone())
+        graphs.append(torch.cuda.CUDAGraph())
+        streams.append(torch.cuda.Stream())
+        with torch.cuda.graph(graphs[-1], stream=streams[-1]):
+            for _ in range(4):
+                ex(g)
+    for _ in range(20):
+        for g in sets:
+            g["O"].fill_(7)
+        torch.cuda.synchronize()
+        for gr, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                gr.replay()
+        torch.cuda.synchronize()
+        for g, w in zip(sets, want):
+            assert torch.equal(g["O"], w)
+    ex.check()
+
+
+def test_a_stream_given_by_its_handle():
+    t, ex = decode_case()
+    g = on_gpu(t)
+    ex(g)
+    torch.cuda.synchronize()
+    want = g["O"].clone()
+    s = torch.cuda.Stream()
+    g["O"].fill_(7)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        ex.run(g, s.cuda_stream)
+    s.synchronize()
+    assert torch.equal(g["O"], want)
+
+
+def test_a_call_from_another_thread():
+    """A thread that has made no CUDA call before: the plan brings its context."""
+    import threading
+    t, ex = decode_case()
+    g = on_gpu(t)
+    ex(g)
+    torch.cuda.synchronize()
+    want = g["O"].clone()
+    g["O"].fill_(7)
+    torch.cuda.synchronize()
+    stream, failed = torch.cuda.Stream(), []
+
+    def work():
+        try:
+            ex.run(g, stream.cuda_stream)
+        except Exception as err:                                 # reported by the test's own thread
+            failed.append(err)
+    th = threading.Thread(target=work)
+    th.start()
+    th.join()
+    torch.cuda.synchronize()
+    assert not failed and torch.equal(g["O"], want)
+
+
+def test_an_empty_batch_of_lengths_keeps_what_is_there():
+    """Lengths of zero, nothing new: the write and the read leave everything, attention answers its rows as unseen."""
+    B, H, hk, d, page, mp = 3, 4, 2, 64, 16, 40
+    for quant in (False, True):
+        common = (hk, d, B * mp + 2, page, mp, "bf16", quant)
+        w, _ = R.make("write", B, hk, d, page, mp, [0] * B, [0] * B, quant=quant, seed=1)
+        got, _ = go(irgen.cache_write_ir(B, 1, *common), w)
+        for n in got:
+            same(got[n], w[n], n)
+        r, _ = R.make("read", B, hk, d, page, mp, [0] * B, [0] * B, length=mp * page, quant=quant, seed=1)
+        got, _ = go(irgen.cache_read_ir(B, mp * page, *common), r)
+        for n in got:
+            same(got[n], r[n], n)
+        a, _ = R.make("attend", B, hk, d, page, mp, [0] * B, [0] * B, heads=H, quant=quant, seed=1)
+        for rows in (0, 64):
+            got, _ = go(irgen.paged_attention_ir(B, 1, H, *common), a, {"paged_rows": rows})
+            ref, bound, _ = R.attention_ref(a, page)
+            R.check(got["O"], ref, bound, "empty")
+
+
+@pytest.mark.parametrize("rows", [0, 64])
+@pytest.mark.parametrize("B,C,lens", [(140, 1, 700), (300, 1, 30)])
+def test_more_sequences_than_a_prefix_sum_takes(B, C, lens, rows):
+    H, hk, d, page = 2, 1, 64, 64
+    gen = torch.Generator().manual_seed(B)
+    ls = torch.randint(0, lens + 1, (B,), generator=gen).tolist()
+    mp = -(-lens // page)
+    t, pages = R.make("attend", B, hk, d, page, mp, ls, [min(C, n) for n in ls], chunk=C, heads=H, seed=B)
+    p = irgen.paged_attention_ir(B, C, H, hk, d, pages, page, mp)
+    got, _ = go(p, t, {"paged_rows": rows})
+    ref, bound, _ = R.attention_ref(t, page)
+    R.check(got["O"], ref, bound, "many sequences")
+
+
+@pytest.mark.parametrize("rows", [0, 64])
+@pytest.mark.parametrize("quant", [False, True])
+def test_pages_named_twice(quant, rows):
+    """Sequences that share the pages of a common beginning, and a page named twice by one sequence."""
+    t, pages = R.make("attend", 2, 2, 64, 16, 20, [300, 310], [4, 2], chunk=4, heads=4, quant=quant, seed=8)
+    t["table"][1, :9] = t["table"][0, :9]
+    t["table"][0, 3] = t["table"][0, 5]
+    p = irgen.paged_attention_ir(2, 4, 4, 2, 64, pages, 16, 20, "bf16", quant)
+    ref, bound, _ = R.attention_ref(t, 16)
+    for ctas in (0, 5):
+        got, _ = go(p, t, {"paged_rows": rows, "paged_ctas": ctas, "paged_min_tiles": 1})
+        R.check(got["O"], ref, bound, "shared pages")
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_caches_past_32_bits(quant):
+    """The same pages in a pool whose elements (and bytes) pass 2^32, first, last and around both powers, give the
+    same bits as in a small one."""
+    B, C, H, hk, d, page, mp = 2, 5, 4, 2, 128, 64, 4
+    small, pages = R.make("write", B, hk, d, page, mp, [250, 199], [C, 3], chunk=C, quant=quant, seed=2)
+    a, _ = R.make("attend", B, hk, d, page, mp, [250, 199], [C, 3], chunk=C, heads=H, quant=quant, seed=2)
+    small["Q"], small["O"] = a["Q"], a["O"]
+    r, _ = R.make("read", B, hk, d, page, mp, [250, 199], [C, 3], length=mp * page, quant=quant, seed=2)
+    small["KR"], small["VR"] = r["KR"], r["VR"]
+    for n in ("KC", "VC", "KS", "VS"):
+        if n in a:
+            small[n] = a[n]
+    per = hk * page * d
+    big = (1 << 32) // per + 9
+    half, full = (1 << 31) // per, (1 << 32) // per
+    where = torch.tensor([0, 1, half - 1, half, half + 1, full - 1, full, full + 1, big - 2, big - 1])[:pages]
+    assert len(where) == pages
+    g = on_gpu(small)
+    h = dict(g)
+    h["table"] = where[small["table"].long()].to(torch.int32).cuda()
+    for n in ("KC", "VC", "KS", "VS"):
+        if n in g:
+            h[n] = torch.empty((big, *g[n].shape[1:]), dtype=g[n].dtype, device="cuda")
+            h[n][where.cuda()] = g[n]
+    for n in ("O", "KR", "VR"):
+        h[n] = g[n].clone()
+    for t, n in ((g, pages), (h, big)):
+        common = (hk, d, n, page, mp, "bf16", quant)
+        for p, opts in ((irgen.cache_write_ir(B, C, *common), {}), (irgen.paged_attention_ir(B, C, H, *common), {}),
+                        (irgen.cache_read_ir(B, mp * page, *common), {})):
+            ex = build(p, opts)
+            ex(t)
+            torch.cuda.synchronize()
+            ex.check()
+            ex.close()
+    for n in ("O", "KR", "VR"):
+        same(h[n].cpu(), g[n].cpu(), n)
+    for n in ("KC", "VC", "KS", "VS"):
+        if n in g:
+            same(h[n][where.cuda()].cpu(), g[n].cpu(), n)
+    tiles = [build(irgen.paged_attention_ir(B, C, H, hk, d, n, page, mp, "bf16", quant), {"paged_rows": 0})
+             for n in (pages, big)]
+    tiles[0](g), tiles[1](h)
+    torch.cuda.synchronize()
+    same(h["O"].cpu(), g["O"].cpu(), "tiles")

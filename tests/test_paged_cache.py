@@ -458,3 +458,26 @@ def test_plan_arguments_are_checked_before_the_driver():
     assert lib.emmy_plan_launch(h, bad, 2, None) != 0 and "parameter 1" in launcher.last_error()
     assert lib.emmy_plan_launch(None, d, 2, None) != 0
     assert lib.emmy_plan_destroy(h) == 0
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="needs a library that has no device")
+def test_a_plan_without_a_context_is_not_launched():
+    lib = launcher.load_library()
+    u3, al, h = (ctypes.c_uint32 * 3)(1, 1, 1), (ctypes.c_uint32 * 1)(16), ctypes.c_void_p()
+    assert lib.emmy_plan_create(ctypes.c_void_p(0x1000), u3, u3, None, 0, 0, al, 1, ctypes.byref(h)) == 0
+    assert lib.emmy_plan_launch(h, (ctypes.c_uint64 * 1)(64), 1, None) != 0 and "emmy_init" in launcher.last_error()
+    assert lib.emmy_plan_destroy(h) == 0
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -65, 2.0 ** 65, 1e-38, 1e38])
+def test_scales_whose_products_leave_f32_are_refused(scale):
+    with pytest.raises(ValueError, match="scale"):
+        irgen.paged_attention_ir(**{**GOOD, "heads": 2, "scale": scale})
+
+
+def test_a_closed_executable_refuses(exe):
+    ex, t, dev = exe
+    ex.close()
+    with pytest.raises(ValueError, match="closed"):
+        ex.run(t, 55)
+    assert dev.log == [("destroyed", 0)]
