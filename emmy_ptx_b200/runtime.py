@@ -18,6 +18,7 @@ stream before the call returns, so callers (and CUDA-graph capture) see one stre
 from __future__ import annotations
 
 import ctypes
+import operator
 
 from .compiler import CompiledModule, compile_ir
 from .launcher import Device, EmmyError
@@ -105,6 +106,9 @@ class Executable:
                 cluster=rec.get("cluster", (1, 1, 1)), pdl=bool(rec.get("pdl")), tmaps=tmaps,
                 tail=self.err.data_ptr() if rec.get("extra") else None))
             self._calls.append((names, ctypes.c_uint64 * len(names)))
+        # where an entry's pointers stand among a call's: the arguments, then the scratch
+        order = [name for name, _, _ in self._args] + list(self._temp)
+        self._calls = [(operator.itemgetter(*map(order.index, names)), arr) for names, arr in self._calls]
 
     def _run_plans(self, tensors: dict, stream) -> None:
         """Check the call's tensors (type, shape, layout, device), allocate its scratch on its stream and launch
@@ -113,34 +117,32 @@ class Executable:
         import torch
         if not self.plans:
             raise ValueError(f"kernel {self.records[0]['entry']!r} was closed")
-        ptrs = {}
+        index, vals = self.index, []
         for name, dtype, shape in self._args:
             t = tensors.get(name)
             if t is None:
                 raise ValueError(f"kernel {self.records[0]['entry']!r} needs the tensor {name!r}")
-            if t.dtype is not dtype or t.shape != shape or t.get_device() != self.index or not t.is_contiguous():
+            if t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or t.get_device() != index:
                 raise ValueError(
-                    f"{name!r} must be a contiguous {dtype} tensor of shape {list(shape)} on cuda:{self.index}, not "
+                    f"{name!r} must be a contiguous {dtype} tensor of shape {list(shape)} on cuda:{index}, not "
                     f"{'a strided' if not t.is_contiguous() else 'a'} {t.dtype} of shape {list(t.shape)} on {t.device}")
-            ptrs[name] = t.data_ptr()
-        keep = []
+            vals.append(t.data_ptr())
         if self._temp:
-            device = f"cuda:{self.index}"
+            device = f"cuda:{index}"
             if stream is None:
                 keep = [torch.empty(n, dtype=dt, device=device) for n, dt in self._temp.values()]
             else:
                 with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
                     keep = [torch.empty(n, dtype=dt, device=device) for n, dt in self._temp.values()]
-            for name, t in zip(self._temp, keep):
-                ptrs[name] = t.data_ptr()
+            vals += [t.data_ptr() for t in keep]
         if stream is None:
-            stream = torch.cuda.current_stream(self.index).cuda_stream
-        for plan, (names, arr), rec in zip(self.plans, self._calls, self.records):
+            stream = torch._C._cuda_getCurrentRawStream(index)
+        for plan, (pick, arr), rec in zip(self.plans, self._calls, self.records):
             try:
-                self.dev.launch_plan(plan, arr(*[ptrs[n] for n in names]), stream)
+                self.dev.launch_plan(plan, arr(*pick(vals)), stream)
             except EmmyError:
-                for n in names:
-                    if ptrs[n] % int(rec["align"].get(n, 1)):
+                for n, v in zip(rec["params"], pick(vals)):
+                    if v % int(rec["align"].get(n, 1)):
                         raise ValueError(f"{n!r} must be {rec['align'][n]}-byte aligned for kernel {rec['entry']!r}") from None
                 raise
 
