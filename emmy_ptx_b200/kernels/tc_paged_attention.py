@@ -1206,7 +1206,7 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     plist = [f"\t.param .u64 p_{p}" for p, _, _ in params]
     plist += [f"\t.param .align 64 .b8 p_{t['name']}[128]" for t in tmaps] + ["\t.param .u64 p_err"]
     text = [f".visible .entry {name}(", ",\n".join(plist), ")", f".reqntid {threads}, 1, 1",
-            f".maxnreg {65536 // (2 * threads) // 8 * 8}", "{"]
+            f".maxnreg {65536 // (2 * -(-threads // 128) * 128) // 8 * 8}", "{"]
     text += e.decls() + e.lines + ["\tret;", "}"]
     return {
         "name": name, "kind": "tcgen05_paged_attention", "params": [n for _, n, _ in params],
