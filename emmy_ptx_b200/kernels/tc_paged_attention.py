@@ -1221,13 +1221,14 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
 def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype, window, sinks, names, scratch, ctas,
                min_tiles=MIN_TILES):
     """The second entry: the rows of units of more than one run, o = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.  One
-    block a unit, which finds the unit's runs by the same prefix sums; a warp a row.  Units of one run are written
-    already; rows of units that see no key at all, which no run covers, become 0."""
+    block a unit, which finds the unit's runs by the same prefix sums.  Units of one run are written already; rows of
+    units that see no key at all, which no run covers, become 0.  Bound by the latency of its loads, so a warp has two
+    rows and four parts of each in flight, under a running maximum (@@)."""
     D = dim
     group, tq, ntile, rows = geometry(chunk, heads, kv_heads)
     pairs = batch * ntile
     per_lane = D // 32
-    threads = 256
+    threads = 512
     e = _E()
     o = e.o
 
@@ -1277,68 +1278,66 @@ def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype,
     part_l = at(part, lane, per_lane * 4)
     o_l = at(gptr("p_O"), lane, per_lane * 2)
     vec = f"v{per_lane}"
+    nwarp, at_once = threads // 32, 2                           # rows of a warp at a time
     row = o("mov.u32", warp)
-    l_row, l_out = e.L("row"), e.L("out")
+    l_row, l_out, l_top, l_done = e.L("row"), e.L("out"), e.L("p"), e.L("pd")
     e.label(l_row)
     e(f"@{e.cond('ge.u32', row, P.vrows)} bra {l_out};")
-
-    def part_row(s_):
-        base = o("selp.u32", r_late, o("mad.lo.u32", s_, 2 * rows, r0), e.cond("eq.u32", s_, 0))
-        return o("add.u32", base, row)
-
-    m = o("mov.b32", "0fFF800000", cls="f")
-    s = o("mov.u32", lane)
-    l_m, l_md = e.L("m"), e.L("md")
-    e.label(l_m)
-    e(f"@{e.cond('ge.u32', o('and.b32', s, -32), nact)} bra {l_md};")            # the same for the warp
-    v = o("mov.b32", "0fFF800000", cls="f")
-    e(f"@{e.cond('lt.u32', s, nact)} ld.global.f32 {v}, [{at(ml, part_row(s), 8)}];")
-    e(f"max.f32 {m}, {m}, {v};")
-    e(f"add.u32 {s}, {s}, 32;")
-    e(f"bra {l_m};")
-    e.label(l_md)
-    for d in (16, 8, 4, 2, 1):
-        e(f"max.f32 {m}, {m}, {o('shfl.sync.bfly.b32', m, d, 31, -1, cls='f')};")
-    e(f"@{e.cond('eq.f32', m, '0fFF800000')} mov.b32 {m}, 0f00000000;")
-    acc = [o("mov.b32", "0f00000000", cls="f") for _ in range(per_lane)]
-    l = o("mov.b32", "0f00000000", cls="f")
+    rws = [o("add.u32", row, nwarp * i) if i else row for i in range(at_once)]
+    live = [e.cond("lt.u32", r, P.vrows) for r in rws]
+    none_m, zero = o("mov.b32", "0fFF800000", cls="f"), o("mov.b32", "0f00000000", cls="f")
+    ms, ls = [o("mov.b32", none_m, cls="f") for _ in rws], [o("mov.b32", zero, cls="f") for _ in rws]
+    accs = [[o("mov.b32", zero, cls="f") for _ in range(per_lane)] for _ in rws]
     s = o("mov.u32", 0)
-    l_top, l_done = e.L("p"), e.L("pd")
     e.label(l_top)
     e(f"@{e.cond('ge.u32', s, nact)} bra {l_done};")
     loaded = []
     for u in range(4):
-        su = o("add.u32", s, u)
-        ok = e.cond("lt.u32", su, nact)
-        idx = part_row(su)
-        ms, ls = o("mov.b32", "0fFF800000", cls="f"), o("mov.b32", "0f00000000", cls="f")
-        e(f"@{ok} ld.global.v2.f32 {{{ms}, {ls}}}, [{at(ml, idx, 8)}];")
-        xs = [o("mov.b32", "0f00000000", cls="f") for _ in range(per_lane)]
-        e(f"@{ok} ld.global.{vec}.f32 {{{', '.join(xs)}}}, [{at(part_l, idx, D * 4)}];")
-        loaded.append((ms, ls, xs))
-    for ms, ls, xs in loaded:
-        f = o("ex2.approx.ftz.f32", o("sub.f32", ms, m, cls="f"), cls="f")
-        e(f"fma.rn.f32 {l}, {f}, {ls}, {l};")
-        for a_, x in zip(acc, xs):
-            e(f"fma.rn.f32 {a_}, {f}, {x}, {a_};")
+        su = o("add.u32", s, u) if u else s
+        base = o("selp.u32", r_late, o("mad.lo.u32", su, 2 * rows, r0), e.cond("eq.u32", su, 0))
+        for i, r in enumerate(rws):
+            ok = e.cond("lt.u32", su, nact)
+            e(f"and.pred {ok}, {ok}, {live[i]};")
+            idx = o("add.u32", base, r)
+            pm, pl = o("mov.b32", none_m, cls="f"), o("mov.b32", zero, cls="f")
+            e(f"@{ok} ld.global.v2.f32 {{{pm}, {pl}}}, [{at(ml, idx, 8)}];")
+            xs = [o("mov.b32", zero, cls="f") for _ in range(per_lane)]
+            e(f"@{ok} ld.global.{vec}.f32 {{{', '.join(xs)}}}, [{at(part_l, idx, D * 4)}];")
+            loaded.append((i, pm, pl, xs))
+    for i in range(at_once):
+        mine = [x for x in loaded if x[0] == i]
+        top = ms[i]
+        for _, pm, _, _ in mine:
+            top = o("max.f32", top, pm, cls="f")
+        ref = o("selp.f32", zero, top, e.cond("eq.f32", top, none_m), cls="f")
+        f = o("ex2.approx.ftz.f32", o("sub.f32", ms[i], ref, cls="f"), cls="f")
+        for x in (ls[i], *accs[i]):
+            e(f"mul.f32 {x}, {x}, {f};")
+        for _, pm, pl, xs in mine:
+            f = o("ex2.approx.ftz.f32", o("sub.f32", pm, ref, cls="f"), cls="f")
+            e(f"fma.rn.f32 {ls[i]}, {f}, {pl}, {ls[i]};")
+            for a_, x in zip(accs[i], xs):
+                e(f"fma.rn.f32 {a_}, {f}, {x}, {a_};")
+        e(f"mov.b32 {ms[i]}, {top};")
     e(f"add.u32 {s}, {s}, 4;")
     e(f"bra {l_top};")
     e.label(l_done)
-    p_zero = e.cond("eq.f32", l, "0f00000000")
-    inv = o("rcp.rn.f32", o("selp.f32", "0f3F800000", l, p_zero, cls="f"), cls="f")
-    words = []
-    for x in range(0, per_lane, 2):
-        x0, x1 = (o("mul.f32", acc[x + k], inv, cls="f") for k in range(2))
-        word = o("cvt.rn.f16x2.f32" if dtype == "f16" else "cvt.rn.bf16x2.f32", x1, x0)
-        words.append(o("selp.b32", 0, word, p_zero))
-    t_ = o("div.u32", row, group)
-    ro = o("add.u32", o("mad.lo.u32", t_, heads, base_row), o("sub.u32", row, o("mul.lo.u32", t_, group)))
-    oa = at(o_l, ro, D * 2)
-    if per_lane == 2:
-        e(f"st.global.b32 [{oa}], {words[0]};")
-    else:
-        e(f"st.global.v2.b32 [{oa}], {{{', '.join(words)}}};")
-    e(f"add.u32 {row}, {row}, {threads // 32};")
+    for i, r in enumerate(rws):
+        p_zero = e.cond("eq.f32", ls[i], zero)
+        inv = o("rcp.rn.f32", o("selp.f32", "0f3F800000", ls[i], p_zero, cls="f"), cls="f")
+        words = []
+        for x in range(0, per_lane, 2):
+            x0, x1 = (o("mul.f32", accs[i][x + k], inv, cls="f") for k in range(2))
+            word = o("cvt.rn.f16x2.f32" if dtype == "f16" else "cvt.rn.bf16x2.f32", x1, x0)
+            words.append(o("selp.b32", 0, word, p_zero))
+        t_ = o("div.u32", r, group)
+        ro = o("add.u32", o("mad.lo.u32", t_, heads, base_row), o("sub.u32", r, o("mul.lo.u32", t_, group)))
+        oa = at(o_l, ro, D * 2)
+        if per_lane == 2:
+            e(f"@{live[i]} st.global.b32 [{oa}], {words[0]};")
+        else:
+            e(f"@{live[i]} st.global.v2.b32 [{oa}], {{{', '.join(words)}}};")
+    e(f"add.u32 {row}, {row}, {nwarp * at_once};")
     e(f"bra {l_row};")
     e.label(l_out)
     ln, fn, on = names
