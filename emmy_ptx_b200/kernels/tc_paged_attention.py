@@ -117,8 +117,9 @@ MIN_TILES = 8                    # a run's least tiles: a part of 128 rows is as
 
 def plan_ctas(batch, chunk, heads, kv_heads, page, max_pages, window, sinks, sms=148):
     """CTAs to spread the tiles over, or 0 for one CTA a unit: for sequences of at most 8 tiles, and where the units
-    fill the GPU by themselves.  There the parts and the second launch cost more than equal runs give (a 2048-token
-    chunk over 8192 keys, 1024 units: 393 us against 412; a windowed chunk of 848 units 68 us against 90)."""
+    fill the GPU by themselves.  There the parts and the second launch cost what equal runs give (a 2048-token
+    chunk over 8192 keys, 1024 units: 428 us, 420 with runs; 512 units of cached bytes 129 us either way; a windowed
+    chunk of 848 units 61 us, 74 with runs)."""
     group, tq, ntile, rows = geometry(chunk, heads, kv_heads)
     longest = -(-max_pages * page // BKV)
     if window is not None:
@@ -1220,13 +1221,15 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
 
 def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype, window, sinks, names, scratch, ctas,
                min_tiles=MIN_TILES):
-    """The second entry: the rows of units of more than one run, o = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.  One
-    block a unit, which finds the unit's runs by the same prefix sums.  Units of one run are written already; rows of
-    units that see no key at all, which no run covers, become 0.  Bound by the latency of its loads, so a warp has two
-    rows and four parts of each in flight, under a running maximum (@@)."""
+    """The second entry: the rows of units of more than one run, o = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.  A
+    block for every cut between two runs, which finds by the same prefix sums the unit it lies in, and joins it if it is
+    the unit's first.  Units of one run are written already; warps of more blocks look at a unit each and write 0 where
+    it sees no key at all (no run covers it).  Bound by the latency of its loads: a warp has four rows and two parts of
+    each in flight, under a running maximum.  2 x 2048 tokens over 8192 keys (295 cuts of 64 KiB a part): 14 us; a block
+    a unit, a row of a warp at a time, took 37."""
     D = dim
     group, tq, ntile, rows = geometry(chunk, heads, kv_heads)
-    pairs = batch * ntile
+    pairs, cuts = batch * ntile, ctas - 1
     per_lane = D // 32
     threads = 512
     e = _E()
@@ -1247,38 +1250,57 @@ def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype,
     def place(pair, ok=None):
         return _Place(e, pair, ok, lens, fresh, batch, chunk, group, tq, ntile, max_pages * page, window, sinks)
 
-    kvh, pair = o("rem.u32", cta, kv_heads), o("div.u32", cta, kv_heads)
-    P = place(pair)
-    e(f"@!{P.live} ret;")                                       # a tile of padding
-    run, before = o("mov.u32", 0), o("mov.u32", 0)
-    for k in range(-(-pairs // 32)):
-        q = o("add.u32", lane, 32 * k) if k else lane
-        v = place(q, e.cond("lt.u32", q, pairs)).tiles
-        e(f"add.u32 {run}, {run}, {v};")
-        e(f"@{e.cond('lt.u32', q, pair)} add.u32 {before}, {before}, {v};")
-    run, before = (o("mul.lo.u32", o("redux.sync.add.u32", x, -1), kv_heads) for x in (run, before))
+    vec = f"v{per_lane}"
+    o_l = at(gptr("p_O"), lane, per_lane * 2)
+
+    def first_row(P, kvh):
+        return o("mad.lo.u32", o("mad.lo.u32", P.b, chunk, P.c0), heads, o("mul.lo.u32", kvh, group))
+
+    def out_row(base, r):
+        t_ = o("div.u32", r, group)
+        return o("add.u32", o("mad.lo.u32", t_, heads, base), o("sub.u32", r, o("mul.lo.u32", t_, group)))
+
+    def store(p_, base, r, words):
+        e(f"{p_}st.global.{'b32' if per_lane == 2 else 'v2.b32'} [{at(o_l, out_row(base, r), D * 2)}], "
+          f"{words[0] if per_lane == 2 else '{' + ', '.join(words) + '}'};")
+
+    l_cut, l_zero = e.L("cut"), e.L("zero")
+    e(f"@{e.cond('lt.u32', cta, cuts)} bra {l_cut};")
+    unit = o("mad.lo.u32", o("sub.u32", cta, cuts), threads // 32, warp)
+    e(f"@{e.cond('ge.u32', unit, pairs * kv_heads)} ret;")
+    P = place(o("div.u32", unit, kv_heads))
+    p_ = e.cond("eq.u32", P.tiles, 0)
+    e(f"and.pred {p_}, {p_}, {P.live};")
+    e(f"@!{p_} ret;")
+    base, r, z_ = first_row(P, o("rem.u32", unit, kv_heads)), o("mov.u32", 0), o("mov.b32", 0)
+    e.label(l_zero)
+    store("", base, r, [z_] * (per_lane // 2))
+    e(f"add.u32 {r}, {r}, 1;")
+    e(f"@{e.cond('lt.u32', r, P.vrows)} bra {l_zero};")
+    e("ret;")
+    e.label(l_cut)
+    sums, run = _prefix(e, lane, pairs, lambda q, ok: place(q, ok).tiles, kv_heads)
     per = o("max.u32", o("div.u32", o("add.u32", run, ctas - 1), ctas), min_tiles)
+    pos = o("mul.lo.u32", o("add.u32", cta, 1), per)
+    e(f"@{e.cond('ge.u32', pos, run)} ret;")                    # nothing behind the cut
+    pair, before = _first_behind(e, sums, pos)
+    P = place(pair)
+    kvh = o("div.u32", o("sub.u32", pos, before), P.tiles)
     t0 = o("mad.lo.u32", kvh, P.tiles, before)
     first = o("div.u32", t0, per)
     last = o("div.u32", o("sub.u32", o("add.u32", t0, P.tiles), 1), per)
-    none = e.cond("eq.u32", P.tiles, 0)
-    p_one = e.cond("eq.u32", first, last)
-    some = e.cond("ne.u32", P.tiles, 0)
-    e(f"and.pred {p_one}, {p_one}, {some};")
-    e(f"@{p_one} ret;")                                         # one run: written already
-    nact = o("selp.u32", 0, o("add.u32", o("sub.u32", last, first), 1), none)
+    e(f"@{e.cond('eq.u32', pos, t0)} ret;")                     # between two units
+    e(f"@{e.cond('ne.u32', first, cta)} ret;")                  # not the unit's first cut
+    nact = o("add.u32", o("sub.u32", last, first), 1)
     # the first run reaches the unit as a later segment (part 2 c + 1) unless it begins with it
     late = o("selp.u32", 1, 0, e.cond("ne.u32", t0, o("mul.lo.u32", first, per)))
     r0 = o("mad.lo.u32", o("mul.lo.u32", first, 2), rows, 0)
     r_late = o("mad.lo.u32", late, rows, r0)
-    base_row = o("mad.lo.u32", P.b, chunk, P.c0)
-    base_row = o("mad.lo.u32", base_row, heads, o("mul.lo.u32", kvh, group))
+    base_row = first_row(P, kvh)
     part = gptr("p_part")
     ml = o("add.s64", part, 2 * ctas * rows * D * 4, cls="rd")
     part_l = at(part, lane, per_lane * 4)
-    o_l = at(gptr("p_O"), lane, per_lane * 2)
-    vec = f"v{per_lane}"
-    nwarp, at_once = threads // 32, 2                           # rows of a warp at a time
+    nwarp, at_once, parts = threads // 32, 4, 2                 # rows of a warp at a time, parts of each
     row = o("mov.u32", warp)
     l_row, l_out, l_top, l_done = e.L("row"), e.L("out"), e.L("p"), e.L("pd")
     e.label(l_row)
@@ -1292,7 +1314,7 @@ def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype,
     e.label(l_top)
     e(f"@{e.cond('ge.u32', s, nact)} bra {l_done};")
     loaded = []
-    for u in range(4):
+    for u in range(parts):
         su = o("add.u32", s, u) if u else s
         base = o("selp.u32", r_late, o("mad.lo.u32", su, 2 * rows, r0), e.cond("eq.u32", su, 0))
         for i, r in enumerate(rws):
@@ -1319,7 +1341,7 @@ def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype,
             for a_, x in zip(accs[i], xs):
                 e(f"fma.rn.f32 {a_}, {f}, {x}, {a_};")
         e(f"mov.b32 {ms[i]}, {top};")
-    e(f"add.u32 {s}, {s}, 4;")
+    e(f"add.u32 {s}, {s}, {parts};")
     e(f"bra {l_top};")
     e.label(l_done)
     for i, r in enumerate(rws):
@@ -1330,13 +1352,7 @@ def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype,
             x0, x1 = (o("mul.f32", accs[i][x + k], inv, cls="f") for k in range(2))
             word = o("cvt.rn.f16x2.f32" if dtype == "f16" else "cvt.rn.bf16x2.f32", x1, x0)
             words.append(o("selp.b32", 0, word, p_zero))
-        t_ = o("div.u32", r, group)
-        ro = o("add.u32", o("mad.lo.u32", t_, heads, base_row), o("sub.u32", r, o("mul.lo.u32", t_, group)))
-        oa = at(o_l, ro, D * 2)
-        if per_lane == 2:
-            e(f"@{live[i]} st.global.b32 [{oa}], {words[0]};")
-        else:
-            e(f"@{live[i]} st.global.v2.b32 [{oa}], {{{', '.join(words)}}};")
+        store(f"@{live[i]} ", base_row, r, words)
     e(f"add.u32 {row}, {row}, {nwarp * at_once};")
     e(f"bra {l_row};")
     e.label(l_out)
@@ -1346,5 +1362,5 @@ def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype,
             f".reqntid {threads}, 1, 1", "{"]
     text += e.decls() + e.lines + ["\tret;", "}"]
     return {"name": name, "kind": "paged_attention_join", "params": [n for _, n, _ in params], "raw_entry": text,
-            "grid": [pairs * kv_heads, 1, 1], "block": [threads, 1, 1], "dyn_smem": 0,
+            "grid": [cuts + -(-pairs * kv_heads // (threads // 32)), 1, 1], "block": [threads, 1, 1], "dyn_smem": 0,
             "align": {n: a_ for _, n, a_ in params}, "zero_outputs": [], "pdl": True}
