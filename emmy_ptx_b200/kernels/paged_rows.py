@@ -49,6 +49,14 @@ def supported(dim, chunk, heads, kv_heads, page) -> bool:
     return dim in (64, 128) and page % 8 == 0 and chunk * (heads // kv_heads) <= MAX_ROWS
 
 
+def few_rows(quant) -> int:
+    """The most rows a unit of this form has unless it is asked for (``paged_rows``) or the tcgen05 form does not take
+    the pages; larger units take that.  16 sequences of up to 5000 tokens, 4 key heads of 128, us here and there: bf16 16
+    rows 33 and 35, 24 rows 43 and 37, 64 rows 72 and 39; bytes (whose conversion costs the other form more) 32 rows 39
+    and 41, 40 rows 47 and 41, 64 rows 59 and 43."""
+    return 32 if quant else 16
+
+
 def shape(dim, chunk, heads, kv_heads, quant):
     """(rows, 16-row tiles, warps, ring stages, bytes of a stage) of a CTA."""
     rows = chunk * (heads // kv_heads)
@@ -77,9 +85,9 @@ MIN_TILES = 4                    # a run's least tiles: one for each of four war
 def plan_ctas(batch, chunk, heads, kv_heads, dim, quant, page, max_pages, window, sinks, sms=148):
     """CTAs to spread the tiles over, or 0 for one CTA a unit: for sequences of at most 8 tiles (a second launch
     would cost more than their keys), for windows when there are units for every SM (all units are alike
-    then) and for batches whose prefix sums would take long (they have many units).  Twice as many as are on the GPU
-    at a time for few rows (a batch of 48 in bytes: 90 us against 92 with one wave); one wave for more rows,
-    whose parts cost more (a draft of 40 rows: 47 us against 55)."""
+    then) and for batches whose prefix sums would take long (they have many units).  As many as are on the GPU at a time:
+    twice as many give a batch of 48 sequences the same (137 us in bf16, 90 and 92 in bytes) and one of 16 less (35 us
+    against 31 in bf16, 33 against 29 in bytes)."""
     longest = -(-max_pages * page // 64)
     units = batch * kv_heads
     if window is not None:
@@ -90,7 +98,7 @@ def plan_ctas(batch, chunk, heads, kv_heads, dim, quant, page, max_pages, window
         return 0
     rows, _, warps, _, _ = shape(dim, chunk, heads, kv_heads, quant)
     resident = 65536 // (max_registers(rows, quant) * 32 * warps)
-    return (2 if rows <= 8 else 1) * resident * sms
+    return resident * sms
 
 
 def _tiles_of(e, at, lens_ptr, fresh_ptr, b, ok, chunk, cap, window, sinks):

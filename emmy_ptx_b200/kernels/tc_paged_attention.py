@@ -112,7 +112,7 @@ def geometry(chunk, heads, kv_heads):
 
 
 MAX_SPREAD_PAIRS = 256           # (sequence, token tile) pairs each CTA takes prefix sums of
-MIN_TILES = 8                    # a run's least tiles: a part of 128 rows is as many bytes as two of them
+MIN_TILES = 4                    # a run's least tiles (one sequence of 5000 tokens, 40 rows: 20.5 us; 24.6 with 8)
 
 
 def plan_ctas(batch, chunk, heads, kv_heads, page, max_pages, window, sinks, sms=148):
@@ -1222,11 +1222,12 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
 def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype, window, sinks, names, scratch, ctas,
                min_tiles=MIN_TILES):
     """The second entry: the rows of units of more than one run, o = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.  A
-    block for every cut between two runs, which finds by the same prefix sums the unit it lies in, and joins it if it is
-    the unit's first.  Units of one run are written already; warps of more blocks look at a unit each and write 0 where
-    it sees no key at all (no run covers it).  Bound by the latency of its loads: a warp has four rows and two parts of
-    each in flight, under a running maximum.  2 x 2048 tokens over 8192 keys (295 cuts of 64 KiB a part): 14 us; a block
-    a unit, a row of a warp at a time, took 37."""
+    block for every cut between two runs: it finds by the same prefix sums the unit that the cut lies in, and the unit's
+    cuts share its rows.  Units of one run are written already; warps of more blocks look at a unit each and write 0
+    where it sees no key at all (no run covers it).  Bound by the latency of its loads, so a warp has eight of them in
+    flight, under a running maximum: two parts of four rows, or eight of one where there are many parts.  2 x
+    2048 tokens over 8192 keys (295 cuts, parts of 64 KiB): 14 us, 37 by a block a unit and a row of a warp at a time; one
+    sequence of 5000 tokens in 79 parts: 6 us, 16 where one block joined a unit."""
     D = dim
     group, tq, ntile, rows = geometry(chunk, heads, kv_heads)
     pairs, cuts = batch * ntile, ctas - 1
@@ -1290,7 +1291,10 @@ def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype,
     first = o("div.u32", t0, per)
     last = o("div.u32", o("sub.u32", o("add.u32", t0, P.tiles), 1), per)
     e(f"@{e.cond('eq.u32', pos, t0)} ret;")                     # between two units
-    e(f"@{e.cond('ne.u32', first, cta)} ret;")                  # not the unit's first cut
+    ncut = o("sub.u32", last, first)
+    nth = o("sub.u32", cta, first)
+    row0 = o("div.u32", o("mul.lo.u32", nth, P.vrows), ncut)
+    row1 = o("div.u32", o("mad.lo.u32", nth, P.vrows, P.vrows), ncut)
     nact = o("add.u32", o("sub.u32", last, first), 1)
     # the first run reaches the unit as a later segment (part 2 c + 1) unless it begins with it
     late = o("selp.u32", 1, 0, e.cond("ne.u32", t0, o("mul.lo.u32", first, per)))
@@ -1300,62 +1304,72 @@ def join_entry(name, batch, chunk, heads, kv_heads, dim, page, max_pages, dtype,
     part = gptr("p_part")
     ml = o("add.s64", part, 2 * ctas * rows * D * 4, cls="rd")
     part_l = at(part, lane, per_lane * 4)
-    nwarp, at_once, parts = threads // 32, 4, 2                 # rows of a warp at a time, parts of each
-    row = o("mov.u32", warp)
-    l_row, l_out, l_top, l_done = e.L("row"), e.L("out"), e.L("p"), e.L("pd")
-    e.label(l_row)
-    e(f"@{e.cond('ge.u32', row, P.vrows)} bra {l_out};")
-    rws = [o("add.u32", row, nwarp * i) if i else row for i in range(at_once)]
-    live = [e.cond("lt.u32", r, P.vrows) for r in rws]
+    nwarp = threads // 32
     none_m, zero = o("mov.b32", "0fFF800000", cls="f"), o("mov.b32", "0f00000000", cls="f")
-    ms, ls = [o("mov.b32", none_m, cls="f") for _ in rws], [o("mov.b32", zero, cls="f") for _ in rws]
-    accs = [[o("mov.b32", zero, cls="f") for _ in range(per_lane)] for _ in rws]
-    s = o("mov.u32", 0)
-    e.label(l_top)
-    e(f"@{e.cond('ge.u32', s, nact)} bra {l_done};")
-    loaded = []
-    for u in range(parts):
-        su = o("add.u32", s, u) if u else s
-        base = o("selp.u32", r_late, o("mad.lo.u32", su, 2 * rows, r0), e.cond("eq.u32", su, 0))
+
+    def join_rows(at_once, parts):
+        """The block's rows, ``at_once`` of a warp at a time and ``parts`` parts of each."""
+        row = o("add.u32", row0, warp)
+        l_row, l_out, l_top, l_done = e.L("row"), e.L("out"), e.L("p"), e.L("pd")
+        e.label(l_row)
+        e(f"@{e.cond('ge.u32', row, row1)} bra {l_out};")
+        rws = [o("add.u32", row, nwarp * i) if i else row for i in range(at_once)]
+        live = [e.cond("lt.u32", r, row1) for r in rws]
+        ms, ls = [o("mov.b32", none_m, cls="f") for _ in rws], [o("mov.b32", zero, cls="f") for _ in rws]
+        accs = [[o("mov.b32", zero, cls="f") for _ in range(per_lane)] for _ in rws]
+        s = o("mov.u32", 0)
+        e.label(l_top)
+        e(f"@{e.cond('ge.u32', s, nact)} bra {l_done};")
+        loaded = []
+        for u in range(parts):
+            su = o("add.u32", s, u) if u else s
+            base = o("selp.u32", r_late, o("mad.lo.u32", su, 2 * rows, r0), e.cond("eq.u32", su, 0))
+            for i, r in enumerate(rws):
+                ok = e.cond("lt.u32", su, nact)
+                e(f"and.pred {ok}, {ok}, {live[i]};")
+                idx = o("add.u32", base, r)
+                pm, pl = o("mov.b32", none_m, cls="f"), o("mov.b32", zero, cls="f")
+                e(f"@{ok} ld.global.v2.f32 {{{pm}, {pl}}}, [{at(ml, idx, 8)}];")
+                xs = [o("mov.b32", zero, cls="f") for _ in range(per_lane)]
+                e(f"@{ok} ld.global.{vec}.f32 {{{', '.join(xs)}}}, [{at(part_l, idx, D * 4)}];")
+                loaded.append((i, pm, pl, xs))
+        for i in range(at_once):
+            mine = [x for x in loaded if x[0] == i]
+            top = ms[i]
+            for _, pm, _, _ in mine:
+                top = o("max.f32", top, pm, cls="f")
+            ref = o("selp.f32", zero, top, e.cond("eq.f32", top, none_m), cls="f")
+            f = o("ex2.approx.ftz.f32", o("sub.f32", ms[i], ref, cls="f"), cls="f")
+            for x in (ls[i], *accs[i]):
+                e(f"mul.f32 {x}, {x}, {f};")
+            for _, pm, pl, xs in mine:
+                f = o("ex2.approx.ftz.f32", o("sub.f32", pm, ref, cls="f"), cls="f")
+                e(f"fma.rn.f32 {ls[i]}, {f}, {pl}, {ls[i]};")
+                for a_, x in zip(accs[i], xs):
+                    e(f"fma.rn.f32 {a_}, {f}, {x}, {a_};")
+            e(f"mov.b32 {ms[i]}, {top};")
+        e(f"add.u32 {s}, {s}, {parts};")
+        e(f"bra {l_top};")
+        e.label(l_done)
         for i, r in enumerate(rws):
-            ok = e.cond("lt.u32", su, nact)
-            e(f"and.pred {ok}, {ok}, {live[i]};")
-            idx = o("add.u32", base, r)
-            pm, pl = o("mov.b32", none_m, cls="f"), o("mov.b32", zero, cls="f")
-            e(f"@{ok} ld.global.v2.f32 {{{pm}, {pl}}}, [{at(ml, idx, 8)}];")
-            xs = [o("mov.b32", zero, cls="f") for _ in range(per_lane)]
-            e(f"@{ok} ld.global.{vec}.f32 {{{', '.join(xs)}}}, [{at(part_l, idx, D * 4)}];")
-            loaded.append((i, pm, pl, xs))
-    for i in range(at_once):
-        mine = [x for x in loaded if x[0] == i]
-        top = ms[i]
-        for _, pm, _, _ in mine:
-            top = o("max.f32", top, pm, cls="f")
-        ref = o("selp.f32", zero, top, e.cond("eq.f32", top, none_m), cls="f")
-        f = o("ex2.approx.ftz.f32", o("sub.f32", ms[i], ref, cls="f"), cls="f")
-        for x in (ls[i], *accs[i]):
-            e(f"mul.f32 {x}, {x}, {f};")
-        for _, pm, pl, xs in mine:
-            f = o("ex2.approx.ftz.f32", o("sub.f32", pm, ref, cls="f"), cls="f")
-            e(f"fma.rn.f32 {ls[i]}, {f}, {pl}, {ls[i]};")
-            for a_, x in zip(accs[i], xs):
-                e(f"fma.rn.f32 {a_}, {f}, {x}, {a_};")
-        e(f"mov.b32 {ms[i]}, {top};")
-    e(f"add.u32 {s}, {s}, {parts};")
-    e(f"bra {l_top};")
-    e.label(l_done)
-    for i, r in enumerate(rws):
-        p_zero = e.cond("eq.f32", ls[i], zero)
-        inv = o("rcp.rn.f32", o("selp.f32", "0f3F800000", ls[i], p_zero, cls="f"), cls="f")
-        words = []
-        for x in range(0, per_lane, 2):
-            x0, x1 = (o("mul.f32", accs[i][x + k], inv, cls="f") for k in range(2))
-            word = o("cvt.rn.f16x2.f32" if dtype == "f16" else "cvt.rn.bf16x2.f32", x1, x0)
-            words.append(o("selp.b32", 0, word, p_zero))
-        store(f"@{live[i]} ", base_row, r, words)
-    e(f"add.u32 {row}, {row}, {nwarp * at_once};")
-    e(f"bra {l_row};")
-    e.label(l_out)
+            p_zero = e.cond("eq.f32", ls[i], zero)
+            inv = o("rcp.rn.f32", o("selp.f32", "0f3F800000", ls[i], p_zero, cls="f"), cls="f")
+            words = []
+            for x in range(0, per_lane, 2):
+                x0, x1 = (o("mul.f32", accs[i][x + k], inv, cls="f") for k in range(2))
+                word = o("cvt.rn.f16x2.f32" if dtype == "f16" else "cvt.rn.bf16x2.f32", x1, x0)
+                words.append(o("selp.b32", 0, word, p_zero))
+            store(f"@{live[i]} ", base_row, r, words)
+        e(f"add.u32 {row}, {row}, {nwarp * at_once};")
+        e(f"bra {l_row};")
+        e.label(l_out)
+
+    l_many = e.L("many")
+    e(f"@{e.cond('gt.u32', nact, 4)} bra {l_many};")
+    join_rows(4, 2)
+    e("ret;")
+    e.label(l_many)
+    join_rows(1, 8)
     ln, fn, on = names
     params = [("lens", ln, 4), ("fresh", fn, 4), ("O", on, 8), ("part", scratch, 32)]
     text = [f".visible .entry {name}(", ",\n".join(f"\t.param .u64 p_{p}" for p, _, _ in params), ")",

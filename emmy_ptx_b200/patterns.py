@@ -526,15 +526,16 @@ def _lower_paged_attention(graph, node, kw, prefix, options):
     geo = {k: kw[k] for k in ("batch", "chunk", "heads", "kv_heads", "page", "max_pages", "window", "sinks")}
     sms = int(options.get("sms", 148))
     rows = kw["chunk"] * (kw["heads"] // kw["kv_heads"])
-    few = (pr.supported(kw["dim"], kw["chunk"], kw["heads"], kw["kv_heads"], kw["page"])
-           and rows <= int(options.get("paged_rows", pr.MAX_ROWS)))
+    tiles = tpa.supported(kw["dim"], kw["heads"], kw["kv_heads"], kw["page"])
+    most = int(options.get("paged_rows", pr.few_rows(kw["quant"]) if tiles else pr.MAX_ROWS))
+    few = pr.supported(kw["dim"], kw["chunk"], kw["heads"], kw["kv_heads"], kw["page"]) and rows <= most
     name = node.op.name
     names = [*node.inputs, node.outputs[0].name]
     scratch = f"{prefix}{name}__part"
     if few:
         form, build = pr, pr.paged_rows_entry
         ctas = pr.plan_ctas(**geo, dim=kw["dim"], quant=kw["quant"], sms=sms)
-    elif tpa.supported(kw["dim"], kw["heads"], kw["kv_heads"], kw["page"]):
+    elif tiles:
         form, build = tpa, tpa.paged_attention_entry
         ctas = tpa.plan_ctas(**geo, sms=sms)
     else:

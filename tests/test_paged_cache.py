@@ -325,8 +325,8 @@ def test_paged_attention_all_pages_missing_is_zero(quant, rows):
 
 
 def test_paged_attention_lowering_rule():
-    """What the tensor cores take: head dim 64 or 128; pages of whole 8-row pieces for at most 64 rows a unit, and
-    above that a group of at most 128 heads and pages that tile 64 keys; a changed nest stays on the CUDA
+    """What the tensor cores take: head dim 64 or 128; pages of whole 8-row pieces for few rows a unit (at most 64
+    where the tcgen05 form does not take the pages), else a group of at most 128 heads and pages that tile 64 keys; a changed nest stays on the CUDA
     cores."""
     def kind(change=None, **kw):
         base = dict(batch=1, chunk=1, heads=2, kv_heads=1, dim=64, pages=4, page=16, max_pages=2)
@@ -334,8 +334,9 @@ def test_paged_attention_lowering_rule():
         if change:
             change(p.graph["nodes"]["paged_attention"])
         return compile_graph(Graph.from_dict(p.graph), p.meta()).kernels[0]["kind"]
-    assert kind() == kind(page=24) == kind(heads=64) == kind(chunk=32) == "paged_attention_rows"
-    assert kind(heads=65) == kind(chunk=33) == "tcgen05_paged_attention"
+    assert kind() == kind(page=24) == kind(heads=16) == kind(chunk=8) == "paged_attention_rows"
+    assert kind(heads=64, page=24) == kind(chunk=32, page=96) == kind(heads=32, quant=True) == "paged_attention_rows"
+    assert kind(heads=17) == kind(chunk=9) == kind(heads=33, quant=True) == "tcgen05_paged_attention"
     assert kind(chunk=40, dim=128, page=192, window=3, sinks=1, scale=0.25) == "tcgen05_paged_attention"
     for kw in (dict(dim=32), dict(dim=256), dict(page=4), dict(page=12), dict(heads=129), dict(chunk=40, page=24),
                dict(chunk=40, page=96)):
