@@ -57,11 +57,13 @@ def few_rows(quant) -> int:
     return 32 if quant else 16
 
 
-def shape(dim, chunk, heads, kv_heads, quant):
-    """(rows, 16-row tiles, warps, ring stages, bytes of a stage) of a CTA."""
+def shape(dim, chunk, heads, kv_heads, quant, wide=False):
+    """(rows, 16-row tiles, warps, ring stages, bytes of a stage) of a CTA.  ``wide``: few units of up to 16 rows, one
+    CTA each, that are bound by the chain of a warp's blocks, take eight warps (one sequence of 333 tokens, 8 key heads
+    of 128: 6.9 us, 8.7 with four; 16 such sequences 8.8 and 11.2)."""
     rows = chunk * (heads // kv_heads)
     mt = -(-rows // 16)
-    warps = {1: 4, 2: 4, 3: 3, 4: 4}[mt]
+    warps = 8 if wide and mt == 1 else {1: 4, 2: 4, 3: 3, 4: 4}[mt]
     stage_bytes = 2 * block_keys(quant) * dim * (1 if quant else 2)
     return rows, mt, warps, (16384 if quant else 8192) // stage_bytes, stage_bytes
 
@@ -112,12 +114,13 @@ def _tiles_of(e, at, lens_ptr, fresh_ptr, b, ok, chunk, cap, window, sinks):
 
 
 def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_pages, dtype, quant, window, sinks,
-                     scale, names, scratch, ctas, min_tiles=MIN_TILES, prefix=""):
+                     scale, names, scratch, ctas, min_tiles=MIN_TILES, prefix="", sms=148):
     """The launch record and PTX; arguments as :func:`.tc_paged_attention.paged_attention_entry`, with ``ctas`` CTAs
     to spread the tiles over (0: one a unit) in runs of at least ``min_tiles``."""
     D = dim
     group = heads // kv_heads
-    rows, mt, warps, stages, stage_b = shape(dim, chunk, heads, kv_heads, quant)
+    wide = not ctas and batch * kv_heads <= (1 if quant else 2) * sms             # all of them on the GPU at a time
+    rows, mt, warps, stages, stage_b = shape(dim, chunk, heads, kv_heads, quant, wide)
     streams = warps // mt
     threads = 32 * warps
     grid = ctas or batch * kv_heads

@@ -7,6 +7,7 @@ missing, every call raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -43,7 +44,7 @@ SIGNATURES = {
     "emmy_plan_add_tmap": [vp, ctypes.c_uint32, ctypes.c_int, ctypes.c_uint32, c_u64p, c_u64p, c_u32p, ctypes.c_int,
                            ctypes.c_int],
     "emmy_plan_set_tail": [vp, ctypes.c_uint64],
-    "emmy_plan_launch": [vp, c_u64p, ctypes.c_uint32, vp],
+    "emmy_plan_launch": [vp, vp, ctypes.c_uint32, vp],
     "emmy_plan_destroy": [vp],
     "emmy_event_create": [ctypes.POINTER(vp)],
     "emmy_event_destroy": [vp],
@@ -128,6 +129,9 @@ def check(code: int, what: str) -> None:
 def dims3(v) -> ctypes.Array:
     v = [int(x) for x in (list(v) + [1, 1, 1])[:3]]
     return (ctypes.c_uint32 * 3)(*v)
+
+
+_PACK = [struct.Struct(f"={n}Q") for n in range(17)]           # a plan's parameters as the C side reads them
 
 
 class Device:
@@ -244,9 +248,10 @@ class Device:
         return h
 
     def launch_plan(self, plan, params, stream: int) -> None:
-        """Launch ``plan`` with ``params`` (a ctypes array of 64-bit values) on ``stream``, in the context the plan
-        was made in (the thread's own stays current)."""
-        rc = self.lib.emmy_plan_launch(plan, params, len(params), stream)
+        """Launch ``plan`` with ``params`` (64-bit integers) on ``stream``, in the context the plan was made in (the
+        thread's own stays current)."""
+        n = len(params)
+        rc = self.lib.emmy_plan_launch(plan, _PACK[n].pack(*params), n, stream)
         if rc:
             check(rc, "emmy_plan_launch")
         self.launches += 1

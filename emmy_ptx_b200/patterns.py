@@ -30,6 +30,7 @@ on the CUDA cores.
 """
 from __future__ import annotations
 
+import functools
 import json
 import os
 
@@ -533,7 +534,7 @@ def _lower_paged_attention(graph, node, kw, prefix, options):
     names = [*node.inputs, node.outputs[0].name]
     scratch = f"{prefix}{name}__part"
     if few:
-        form, build = pr, pr.paged_rows_entry
+        form, build = pr, functools.partial(pr.paged_rows_entry, sms=sms)
         ctas = pr.plan_ctas(**geo, dim=kw["dim"], quant=kw["quant"], sms=sms)
     elif tiles:
         form, build = tpa, tpa.paged_attention_entry

@@ -105,10 +105,10 @@ class Executable:
                 fn, rec["grid"], rec["block"], rec.get("dyn_smem", 0), [int(rec["align"].get(n, 1)) for n in names],
                 cluster=rec.get("cluster", (1, 1, 1)), pdl=bool(rec.get("pdl")), tmaps=tmaps,
                 tail=self.err.data_ptr() if rec.get("extra") else None))
-            self._calls.append((names, ctypes.c_uint64 * len(names)))
+            self._calls.append(names)
         # where an entry's pointers stand among a call's: the arguments, then the scratch
         order = [name for name, _, _ in self._args] + list(self._temp)
-        self._calls = [(operator.itemgetter(*map(order.index, names)), arr) for names, arr in self._calls]
+        self._calls = [operator.itemgetter(*map(order.index, names)) for names in self._calls]
 
     def _run_plans(self, tensors: dict, stream) -> None:
         """Check the call's tensors (type, shape, layout, device), allocate its scratch on its stream and launch
@@ -137,9 +137,9 @@ class Executable:
             vals += [t.data_ptr() for t in keep]
         if stream is None:
             stream = torch._C._cuda_getCurrentRawStream(index)
-        for plan, (pick, arr), rec in zip(self.plans, self._calls, self.records):
+        for plan, pick, rec in zip(self.plans, self._calls, self.records):
             try:
-                self.dev.launch_plan(plan, arr(*pick(vals)), stream)
+                self.dev.launch_plan(plan, pick(vals), stream)
             except EmmyError:
                 for n, v in zip(rec["params"], pick(vals)):
                     if v % int(rec["align"].get(n, 1)):
