@@ -11,8 +11,9 @@ one.  The tiles of all units, in a row, are cut into equal runs, one for each CT
 SM, half its TMEM columns and shared memory each, so that one's loads and softmax run beside the other's
 products): every CTA takes prefix sums over the units and so finds its own run, whatever the lengths are.  A unit of
 more than one run leaves parts in f32 (O, the row's reference m and its sum l) and a second entry joins them
-(o = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s).  Batches of very many units, and very short sequences, take one
-CTA a unit instead.
+(o = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s).  Where the units fill the GPU by
+themselves, and for very short sequences, a CTA takes one unit, the longest units first: every CTA counts how many come
+before its own (4 x 512 tokens behind 333 to 4096 keys, bytes: 100 us, 129 in order of the table).
 
 **Roles.**  One thread issues the ``tcgen05.mma``: S(j+1) = Q K_(j+1)^T into one of two 64-column score buffers,
 then O += P(j) V_j.  Four softmax warps hold one row a thread; warps without a row take no part.  A warp loads by
@@ -117,9 +118,9 @@ MIN_TILES = 4                    # a run's least tiles (one sequence of 5000 tok
 
 def plan_ctas(batch, chunk, heads, kv_heads, page, max_pages, window, sinks, sms=148):
     """CTAs to spread the tiles over, or 0 for one CTA a unit: for sequences of at most 8 tiles, and where the units
-    fill the GPU by themselves.  There the parts and the second launch cost what equal runs give (a 2048-token
-    chunk over 8192 keys, 1024 units: 428 us, 420 with runs; 512 units of cached bytes 129 us either way; a windowed
-    chunk of 848 units 61 us, 74 with runs)."""
+    fill the GPU by themselves.  There the parts and the second launch cost more than equal runs give (a 2048-token
+    chunk over 8192 keys, 1024 units: 418 us, 420 with runs; 512 units of cached bytes 100 and 129; a windowed
+    chunk of 848 units 59 and 74)."""
     group, tq, ntile, rows = geometry(chunk, heads, kv_heads)
     longest = -(-max_pages * page // BKV)
     if window is not None:
@@ -203,7 +204,7 @@ def _first_behind(e, sums, start):
 
 
 def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_pages, dtype, quant, window, sinks,
-                          scale, names, scratch, ctas, min_tiles=MIN_TILES, prefix=""):
+                          scale, names, scratch, ctas, min_tiles=MIN_TILES, prefix="", sms=148):
     """The launch record and PTX; ``names``: Q, KC, VC, (KS, VS,) table, lens, fresh, O; ``scratch``: the parts'
     buffer, all their O rows and then their m and l."""
     D = dim
@@ -231,6 +232,8 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     kdesc_hi = smem_desc_hi(16, 1024)
     vdesc_hi = smem_desc_hi(kv_box, 1024)
     cscale = _f32(scale * LOG2E)
+    # one CTA a unit, more of them than the GPU holds at a time, of sequences that may differ
+    order = not ctas and batch > 1 and pairs <= MAX_SPREAD_PAIRS and pairs * kv_heads > 2 * sms
     SCOL = D                                 # score buffers behind O's columns
     e = _E()
     o = e.o
@@ -257,6 +260,37 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     def place(pair, ok=None):
         return _Place(e, pair, ok, lens, fresh, batch, chunk, group, tq, ntile, cap, window, sinks)
 
+    def by_length(nth):
+        """The pair with the nth most tiles, so that the longest units start first and no long one is left for the end:
+        each thread counts how many come before its own."""
+        keys, mine = o("mov.u32", f"{prefix}{name}_order"), []
+        for k in range(-(-pairs // threads)):
+            q = o("add.u32", tid, threads * k)
+            ok = e.cond("lt.u32", q, pairs)
+            key = o("min.u32", place(q, ok).tiles, (1 << 22) - 1)
+            key = o("mad.lo.u32", key, 512, o("sub.u32", 2 * MAX_SPREAD_PAIRS - 1, q))      # ties: the earlier pair
+            e(f"@{ok} st.shared.b32 [{o('mad.lo.u32', q, 4, keys)}], {key};")
+            mine.append((q, ok, key, o("mov.u32", 0)))
+        quads = -(-pairs // 4)
+        pad = e.cond("lt.u32", tid, 4 * quads - pairs)
+        e(f"@{pad} st.shared.b32 [{o('mad.lo.u32', tid, 4, keys)}+{4 * pairs}], {o('mov.b32', 0)};")
+        e("bar.sync 0;")
+        at_, last_, l_top = o("mov.u32", keys), o("add.u32", keys, 16 * quads), e.L("rank")
+        e.label(l_top)
+        x = [e.r() for _ in range(4)]
+        e(f"ld.shared.v4.b32 {{{', '.join(x)}}}, [{at_}];")
+        for _, _, key, rank in mine:
+            for y in x:
+                e(f"@{e.cond('gt.u32', y, key)} add.u32 {rank}, {rank}, 1;")
+        e(f"add.u32 {at_}, {at_}, 16;")
+        e(f"@{e.cond('lt.u32', at_, last_)} bra {l_top};")
+        for q, ok, _, rank in mine:
+            hit = e.cond("eq.u32", rank, nth)
+            e(f"and.pred {hit}, {hit}, {ok};")
+            e(f"@{hit} st.shared.b32 [{keys}+{4 * MAX_SPREAD_PAIRS}], {q};")
+        e("bar.sync 0;")
+        return o("ld.shared.b32", f"[{keys}+{4 * MAX_SPREAD_PAIRS}]")
+
     if ctas:
         e("griddepcontrol.launch_dependents;")                  # the join's blocks may come up and wait
         sums, run = _prefix(e, lane, pairs, lambda q, ok: place(q, ok).tiles, kv_heads)
@@ -266,8 +300,8 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
         stop = o("min.u32", o("add.u32", start, per), run)
         pair0, before0 = _first_behind(e, sums, start)
     else:
-        kvh0 = o("rem.u32", cta, kv_heads)
-        S0 = place(o("div.u32", cta, kv_heads))
+        kvh0, nth = o("rem.u32", cta, kv_heads), o("div.u32", cta, kv_heads)
+        S0 = place(by_length(nth) if order else nth)
         e(f"@!{S0.live} ret;")                                  # a tile of padding
 
     class Segment:
@@ -1211,7 +1245,8 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     text += e.decls() + e.lines + ["\tret;", "}"]
     return {
         "name": name, "kind": "tcgen05_paged_attention", "params": [n for _, n, _ in params],
-        "raw_entry": text, "raw_decls": [f".extern .shared .align 1024 .b8 {smem_sym}[];"],
+        "raw_entry": text, "raw_decls": [f".extern .shared .align 1024 .b8 {smem_sym}[];",
+                                        *([f".shared .align 16 .b8 {prefix}{name}_order[{4 * MAX_SPREAD_PAIRS + 16}];"] if order else [])],
         "grid": [grid, 1, 1], "block": [threads, 1, 1],
         "dyn_smem": q_bytes + (2 * kv_bytes + 4 * raw_b + AUX_BYTES if quant else STAGES * kv_bytes + KSC) + 1024,
         "align": {n: a_ for _, n, a_ in params}, "zero_outputs": [], "tmaps": tmaps,

@@ -30,7 +30,6 @@ on the CUDA cores.
 """
 from __future__ import annotations
 
-import functools
 import json
 import os
 
@@ -534,7 +533,7 @@ def _lower_paged_attention(graph, node, kw, prefix, options):
     names = [*node.inputs, node.outputs[0].name]
     scratch = f"{prefix}{name}__part"
     if few:
-        form, build = pr, functools.partial(pr.paged_rows_entry, sms=sms)
+        form, build = pr, pr.paged_rows_entry
         ctas = pr.plan_ctas(**geo, dim=kw["dim"], quant=kw["quant"], sms=sms)
     elif tiles:
         form, build = tpa, tpa.paged_attention_entry
@@ -543,7 +542,7 @@ def _lower_paged_attention(graph, node, kw, prefix, options):
         return None
     ctas = int(options.get("paged_ctas", ctas))
     least = int(options.get("paged_min_tiles", form.MIN_TILES))
-    main = build(name, **kw, names=names, scratch=scratch, ctas=ctas, min_tiles=least, prefix=prefix)
+    main = build(name, **kw, names=names, scratch=scratch, ctas=ctas, min_tiles=least, prefix=prefix, sms=sms)
     join = None
     if ctas:
         join = form.join_entry(f"{name}_join", **geo, dim=kw["dim"], dtype=kw["dtype"], names=names[-3:], scratch=scratch,

@@ -482,3 +482,17 @@ def test_a_closed_executable_refuses(exe):
     with pytest.raises(ValueError, match="closed"):
         ex.run(t, 55)
     assert dev.log == [("destroyed", 0)]
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_units_start_with_the_longest(quant):
+    """More units than an SM count of 1 holds: which unit a CTA takes goes by the lengths (equal ones and none among
+    them), and every unit is taken once."""
+    B, C, H, hk, d, page, mp = 5, 130, 1, 1, 64, 64, 5
+    t, pages = R.make("attend", B, hk, d, page, mp, [140, 300, 0, 140, 219], [130, 70, 0, 130, 3], chunk=C, heads=H,
+                      quant=quant, seed=6)
+    p = irgen.paged_attention_ir(B, C, H, hk, d, pages, page, mp, "bf16", quant)
+    got, code, mod = PE.run(p, t, {"sms": 1, "paged_ctas": 0})
+    assert code == 0 and mod.kernels[0]["grid"] == [10, 1, 1] and "_order" in mod.ptx
+    ref, bound, _ = R.attention_ref(t, page)
+    R.check(got["O"], ref, bound, "longest first")
