@@ -119,8 +119,8 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
     to spread the tiles over (0: one a unit) in runs of at least ``min_tiles``."""
     D = dim
     group = heads // kv_heads
-    wide = not ctas and batch * kv_heads <= (1 if quant else 2) * sms             # all of them on the GPU at a time
-    rows, mt, warps, stages, stage_b = shape(dim, chunk, heads, kv_heads, quant, wide)
+    eight = not ctas and batch * kv_heads <= (1 if quant else 2) * sms            # all of them on the GPU at a time
+    rows, mt, warps, stages, stage_b = shape(dim, chunk, heads, kv_heads, quant, eight)
     streams = warps // mt
     threads = 32 * warps
     grid = ctas or batch * kv_heads
