@@ -84,18 +84,27 @@ MAX_SPREAD_BATCH = 128           # sequences whose lengths each CTA takes prefix
 MIN_TILES = 4                    # a run's least tiles: one for each of four warps
 
 
+def _longest(chunk, page, max_pages, window, sinks):
+    """The most tiles a unit can have."""
+    longest = -(-max_pages * page // 64)
+    return longest if window is None else min(longest, -(-sinks // 64) + (window + chunk - 1) // 64 + 2)
+
+
+def most_tiles(batch, chunk, heads, kv_heads, page, max_pages, window, sinks):
+    """The most tiles all units can have."""
+    return batch * kv_heads * _longest(chunk, page, max_pages, window, sinks)
+
+
 def plan_ctas(batch, chunk, heads, kv_heads, dim, quant, page, max_pages, window, sinks, sms=148):
     """CTAs to spread the tiles over, or 0 for one CTA a unit: for sequences of at most 8 tiles (a second launch
     would cost more than their keys), for windows when there are units for every SM (all units are alike
     then) and for batches whose prefix sums would take long (they have many units).  As many as are on the GPU at a time:
     twice as many give a batch of 48 sequences the same (137 us in bf16, 90 and 92 in bytes) and one of 16 less (35 us
     against 31 in bf16, 33 against 29 in bytes)."""
-    longest = -(-max_pages * page // 64)
+    longest = _longest(chunk, page, max_pages, window, sinks)
     units = batch * kv_heads
-    if window is not None:
-        longest = min(longest, -(-sinks // 64) + (window + chunk - 1) // 64 + 2)
-        if units >= 2 * sms:
-            return 0
+    if window is not None and units >= 2 * sms:
+        return 0
     if longest <= 8 or batch > MAX_SPREAD_BATCH or units * longest >= 1 << 31:
         return 0
     rows, _, warps, _, _ = shape(dim, chunk, heads, kv_heads, quant)

@@ -116,17 +116,30 @@ MAX_SPREAD_PAIRS = 256           # (sequence, token tile) pairs each CTA takes p
 MIN_TILES = 4                    # a run's least tiles (one sequence of 5000 tokens, 40 rows: 20.5 us; 24.6 with 8)
 
 
+def _longest(chunk, heads, kv_heads, page, max_pages, window, sinks):
+    """The most tiles a unit can have."""
+    longest = -(-max_pages * page // BKV)
+    if window is None:
+        return longest
+    _, tq, _, _ = geometry(chunk, heads, kv_heads)
+    return min(longest, -(-sinks // BKV) + (window + min(tq, chunk) - 1) // BKV + 2)
+
+
+def most_tiles(batch, chunk, heads, kv_heads, page, max_pages, window, sinks):
+    """The most tiles all units can have."""
+    return (batch * geometry(chunk, heads, kv_heads)[2] * kv_heads
+            * _longest(chunk, heads, kv_heads, page, max_pages, window, sinks))
+
+
 def plan_ctas(batch, chunk, heads, kv_heads, page, max_pages, window, sinks, sms=148):
     """CTAs to spread the tiles over, or 0 for one CTA a unit: for sequences of at most 8 tiles, and where the units
     fill the GPU by themselves.  There the parts and the second launch cost more than equal runs give (a 2048-token
     chunk over 8192 keys, 1024 units: 418 us, 420 with runs; 512 units of cached bytes 100 and 129; a windowed
     chunk of 848 units 59 and 74)."""
-    group, tq, ntile, rows = geometry(chunk, heads, kv_heads)
-    longest = -(-max_pages * page // BKV)
-    if window is not None:
-        longest = min(longest, -(-sinks // BKV) + (window + min(tq, chunk) - 1) // BKV + 2)
-    pairs = batch * ntile
-    if longest <= 8 or pairs > MAX_SPREAD_PAIRS or pairs * kv_heads >= 2 * sms:
+    pairs = batch * geometry(chunk, heads, kv_heads)[2]
+    longest = _longest(chunk, heads, kv_heads, page, max_pages, window, sinks)
+    if (longest <= 8 or pairs > MAX_SPREAD_PAIRS or pairs * kv_heads >= 2 * sms
+            or pairs * kv_heads * longest >= 1 << 31):
         return 0
     return 2 * sms
 

@@ -542,6 +542,10 @@ def _lower_paged_attention(graph, node, kw, prefix, options):
         return None
     ctas = int(options.get("paged_ctas", ctas))
     least = int(options.get("paged_min_tiles", form.MIN_TILES))
+    if not 0 <= ctas <= 1 << 14 or not 1 <= least <= 1 << 16:
+        raise ValueError(f"paged_ctas is 0 to 2^14 and paged_min_tiles 1 to 2^16, not {ctas} and {least}")
+    if ctas and form.most_tiles(**geo) >= 1 << 31:              # a run's place is a 32-bit number
+        raise ValueError(f"paged_ctas={ctas} with 2^31 tiles and more")
     main = build(name, **kw, names=names, scratch=scratch, ctas=ctas, min_tiles=least, prefix=prefix, sms=sms)
     join = None
     if ctas:

@@ -496,3 +496,21 @@ def test_units_start_with_the_longest(quant):
     assert code == 0 and mod.kernels[0]["grid"] == [10, 1, 1] and "_order" in mod.ptx
     ref, bound, _ = R.attention_ref(t, page)
     R.check(got["O"], ref, bound, "longest first")
+
+
+@pytest.mark.parametrize("opts", [{"paged_ctas": -1}, {"paged_ctas": 1 << 15}, {"paged_min_tiles": 0},
+                                  {"paged_min_tiles": 1 << 17}])
+@pytest.mark.parametrize("rows", [0, 64])
+def test_options_out_of_range_are_refused(opts, rows):
+    p = irgen.paged_attention_ir(2, 1, 2, 1, 64, 8, 64, 4)
+    with pytest.raises(ValueError, match="paged_ctas"):
+        compile_graph(Graph.from_dict(p.graph), p.meta(), {**opts, "paged_rows": rows})
+
+
+@pytest.mark.parametrize("rows", [0, 64])
+def test_more_tiles_than_32_bits_are_not_cut_into_runs(rows):
+    p = irgen.paged_attention_ir(128, 1, 2, 2, 64, 1 << 20, 64, (1 << 24) - 1)
+    for opts in ({}, {"paged_ctas": 0}):
+        assert len(compile_graph(Graph.from_dict(p.graph), p.meta(), {**opts, "paged_rows": rows}).kernels) == 1
+    with pytest.raises(ValueError, match="tiles"):
+        compile_graph(Graph.from_dict(p.graph), p.meta(), {"paged_ctas": 8, "paged_rows": rows})
