@@ -22,12 +22,16 @@ meets the other warps once, at the end.
   or fewer use half of the tile's registers.  Units of more than 16 rows give each 16 rows their own warps, which
   read the same keys from L1 and L2.
 * **Numerics** as in the tensor-memory form: scores, sums and O in f32; P in f16 (to nearest, lifted by 2^7) for
-  f16 caches, in two bf16 parts (2^-14 together) for bf16 caches and bytes; bytes are converted exactly.
+  f16 caches and bytes, in two bf16 parts (2^-14 together) for bf16 caches; bytes are converted to f16 exactly.
   The reference of a row is raised when a score exceeds it by 2^8, so most blocks need no maximum.
 
 * **What is masked** keeps its promise: V rows that no row of the unit sees become 0 in registers, and where some rows
   see a key and others do not, an infinity or a NaN in its V row is taken out of the product and put back by two
   products of indicators (which rows see the key, which elements are +inf or NaN, -inf or NaN).
+
+Measured on one B200 (8 key heads of 128, 4 query heads each): 48 sequences of 17 to 8192 tokens, bf16, 830 MB: the
+kernel 133 us, 6.26 TB/s (0.97 of a copy), the call 139; the same in bytes 84 and 90 us, where issue slots are the
+busiest resource; one sequence of 333 tokens 6.9 us.
 
 The tcgen05 form holds a row a thread: four rows keep 4 of its 128 softmax threads busy, and each tile passes
 through TMA, MMA, TMEM and back.
