@@ -440,8 +440,8 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
     if quant:
         c64, c1152 = o("mov.b32", "0x64646464"), o("mov.b32", "0x64806480")
         c6400 = o("mov.b32", "0x64006400")
-        # P carries the values' scales over vref, a power of two at least half the largest scale the warp's rows met:
-        # P is at most 2^15 in f16, and what is 2^-20 of the largest scale's still has 11 bits
+        # P carries the values' scales over vref, a power of two at least half the largest scale (of either sign) the
+        # warp's rows met: P is at most 2^15 in f16, and what is 2^-20 of the largest scale's still has 11 bits
         vref = o("mov.b32", "0f00800000", cls="f")
         vinv = o("mov.b32", "0f7E800000", cls="f")
     l_top, l_done = e.L("blk"), e.L("blkd")
@@ -532,7 +532,8 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
     if quant:
         ymax = o("mov.b32", "0f00000000", cls="f")
         for a in range(NT):
-            e(f"max.f32 {ymax}, {ymax}, {o('max.f32', ys[a][0], ys[a][1], cls='f')};")    # a NaN drops out
+            for y in ys[a]:                                     # of either sign; a NaN drops out
+                e(f"max.f32 {ymax}, {ymax}, {o('abs.f32', y, cls='f')};")
         p_ = e.cond("ge.f32", o("mul.f32", ymax, vinv, cls="f"), "0f40000000")
         e(f"or.pred {need}, {need}, {p_};")
     anyneed = o("vote.sync.any.pred", need, -1, cls="p")

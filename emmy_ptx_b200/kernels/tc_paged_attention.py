@@ -29,8 +29,8 @@ scores' columns, the values' scales multiply P.
 f16 caches take f16 P, to nearest (2^-11), with 2^7 put on the exponent so that small weights keep their bits;
 bf16 caches take P as two bf16 parts, truncated, 2^-14 together.  Bytes are multiplied in f16: a bf16 Q row is
 brought to 2^14 by a power of two (exact but for numbers 2^-28 of its largest), and P carries the values' scales over
-a running power of two, at least half the largest scale so far, so that it stays below 2^15 and what is 2^-20 of the
-largest still has 11 bits.  O is rescaled only when the row's maximum grew by more than 2^8, or that power did.
+a running power of two, at least half the largest scale so far (scales have any sign: the largest magnitude), so that it
+stays below 2^15 and what is 2^-20 of the largest still has 11 bits.  O is rescaled only when the row's maximum grew by more than 2^8, or that power did.
 
 **What is masked.**  Scores past the row's own position, outside its window or of a page that the table does not
 name become -inf; a row that sees nothing ends as 0.  Rows of a V tile that no row of the CTA sees are zeroed in
@@ -602,7 +602,7 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
                     p1, p2 = e.cond("ge.u32", kk, w["lo"]), e.cond("lt.u32", kk, sinks)
                     e(f"or.pred {p1}, {p1}, {p2};")
                     e(f"and.pred {pk1}, {pk1}, {p1};")
-                e(f"@{pk1} max.f32 {big}, {big}, {vsv[i]};")        # a NaN drops out
+                e(f"@{pk1} max.f32 {big}, {big}, {o('abs.f32', vsv[i], cls='f')};")        # a NaN drops out
             bigb = o("redux.sync.max.u32", o("mov.b32", big), -1)
             bigb = o("min.u32", o("and.b32", bigb, "0x7F800000"), "0x7E000000")
             grow = e.cond("gt.u32", bigb, vpow)

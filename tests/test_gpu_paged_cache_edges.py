@@ -1,0 +1,34 @@
+"""The paged key/value cache at the edges of what its definition allows, on a B200 against plain float64 (the CPU's
+cases and references: :mod:`tests.test_paged_cache_edges`, :mod:`tests.pagedref`)."""
+import pytest
+import torch
+
+from emmy_ptx_b200.compiler import compile_graph
+from emmy_ptx_b200.ir import Graph
+from emmy_ptx_b200.runtime import Executable
+from tests import pagedref as R
+from tests.test_paged_cache_edges import SIGNED, SIGNS, signed_case
+
+pytestmark = pytest.mark.gpu
+
+
+def go(p, t, opts=None):
+    ex = Executable(compile_graph(Graph.from_dict(p.graph), p.meta(), opts or {}), device=0)
+    g = {k: v.cuda() for k, v in t.items()}
+    ex(g)
+    torch.cuda.synchronize()
+    ex.check()
+    ex.close()
+    return {a.name: g[a.name].cpu() for a in p.outputs}
+
+
+@pytest.mark.parametrize("opts", [{"paged_rows": 0}, {"paged_rows": 64}, {"patterns": False}],
+                         ids=["tiles", "rows", "CUDA-cores"])
+@pytest.mark.parametrize("signs", SIGNS)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("case", SIGNED, ids=["decode", "draft-runs"])
+def test_scales_of_any_sign(case, dtype, signs, opts):
+    t, p = signed_case(case, dtype, signs)
+    got = go(p, t, {**case[-1], **opts})
+    ref, bound, _ = R.attention_ref(t, case[5])
+    R.check(got["O"], ref, bound, signs)
