@@ -22,7 +22,8 @@ meets the other warps once, at the end.
   or fewer use half of the tile's registers.  Units of more than 16 rows give each 16 rows their own warps, which
   read the same keys from L1 and L2.
 * **Numerics** as in the tensor-memory form: scores, sums and O in f32; P in f16 (to nearest, lifted by 2^7) for
-  f16 caches and bytes, in two bf16 parts (2^-14 together) for bf16 caches; bytes are converted to f16 exactly.
+  f16 caches and bytes, in two bf16 parts (2^-14 together, at most 1) for bf16 caches; bytes are converted to f16
+  exactly.
   The reference of a row is raised when a score exceeds it by 2^8, so most blocks need no maximum.
 
 * **What is masked** keeps its promise: V rows that no row of the unit sees become 0 in registers, and where some rows
@@ -41,10 +42,9 @@ from __future__ import annotations
 import math
 
 from .ptxasm import wait_bar_warp
-from .tc_paged_attention import F16_LIFT, LOG2E, RESCALE, _E, _f32, _unit
+from .tc_paged_attention import LOG2E, RESCALE, _E, _f32, _unit, lift_of
 
 MAX_ROWS = 64
-QUANT_LIFT = 6.0                 # bytes: P's exponent is lifted by one less, since its scale may be twice vref
 ERR_ROWS = 77                    # a block's copy never completed
 
 
@@ -436,7 +436,7 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
     n = o("mov.u32", stream)
     rd, rbit = o("mov.u32", 0), o("mov.u32", 1)                # the stage to read next, and its bit
     l_fail = e.L("fail")
-    lift = 0.0 if not p_f16 else QUANT_LIFT if quant else F16_LIFT
+    lift = lift_of(dtype, quant)
     if quant:
         c64, c1152 = o("mov.b32", "0x64646464"), o("mov.b32", "0x64806480")
         c6400 = o("mov.b32", "0x64006400")
@@ -715,6 +715,13 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
         for d_ in (1, 2):
             e(f"add.f32 {l[h]}, {l[h]}, {o('shfl.sync.bfly.b32', l[h], d_, 31, -1, cls='f')};")
     e("bar.sync 0;")
+    # bytes: O times the scales' power, both sums by 2^-14 first, so that weights are at most 1 (as in bf16): no sum here
+    # is larger than that of p v
+    out_lift = -RESCALE if quant else lift
+    if quant:
+        vout = o("mul.f32", vref, _f32(2.0 ** (out_lift - lift)), cls="f")
+        for h in hs:
+            e(f"mul.f32 {l[h]}, {l[h]}, {_f32(2.0 ** (out_lift - lift))};")
     obase = o("mad.lo.u32", warp, RW * orow, sbase)
     mlb = o("add.u32", sbase, warps * RW * orow)
 
@@ -730,7 +737,7 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
                 for x0 in range(0, piece, 4):
                     vals = [acc[i * piece + x0 + x][2 * h + j] for x in range(4)]
                     if quant:
-                        vals = [o("mul.f32", x, vref, cls="f") for x in vals]
+                        vals = [o("mul.f32", x, vout, cls="f") for x in vals]
                     e(f"st.shared.v4.f32 [{ra}+{(i * span + j * piece + x0) * 4}], {{{', '.join(vals)}}};")
         ma = o("mad.lo.u32", o("mad.lo.u32", warp, RW, rr), 8, mlb)
         e(f"@{p_t0} st.shared.v2.f32 [{ma}], {{{m[h]}, {l[h]}}};")
@@ -793,7 +800,7 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
         pa_ = at(at(gptr("p_part"), wide(pi, D * 4)), wide(ch, 32))
         e(f"st.global.v8.f32 [{pa_}], {{{', '.join(ov)}}};")
         mla = at(at(gptr("p_part"), 2 * ctas * rows * D * 4), wide(pi, 8))
-        meff = o("sub.f32", mm, _f32(lift), cls="f")
+        meff = o("sub.f32", mm, _f32(out_lift), cls="f")
         e(f"@{e.cond('eq.u32', ch, 0)} st.global.v2.f32 [{mla}], {{{meff}, {lt}}};")
     e.label(l_next)
     e(f"add.u32 {item}, {item}, {threads};")

@@ -27,7 +27,7 @@ scores' columns, the values' scales multiply P.
 
 **Numerics.**  The score buffers, the running reference and sum, and O are f32.  P is rounded for the tensor core:
 f16 caches take f16 P, to nearest (2^-11), with 2^7 put on the exponent so that small weights keep their bits;
-bf16 caches take P as two bf16 parts, truncated, 2^-14 together.  Bytes are multiplied in f16: a bf16 Q row is
+bf16 caches take P as two bf16 parts, truncated, 2^-14 together, of 2^(s - m - 8): at most 1.  Bytes are multiplied in f16: a bf16 Q row is
 brought to 2^14 by a power of two (exact but for numbers 2^-28 of its largest), and P carries the values' scales over
 a running power of two, at least half the largest scale so far (scales have any sign: the largest magnitude), so that it
 stays below 2^15 and what is 2^-20 of the largest still has 11 bits.  O is rescaled only when the row's maximum grew by more than 2^8, or that power did.
@@ -79,7 +79,13 @@ VBAD = 240                       # two words per score buffer: rows of the V til
 QSC = VSC + 4 * BKV * 4
 RAWSC = QSC + 4 * ROWS
 AUX_BYTES = RAWSC + 2 * 2 * BKV * 4
-QUANT_LIFT = 6.0                 # bytes: P may carry up to twice the power its scales stand over
+QUANT_LIFT = 6.0                 # bytes: P's exponent is lifted by one less, since its scale may be twice vref
+
+
+def lift_of(dtype, quant) -> float:
+    """What P's exponent is lifted by.  In bf16, whose exponents reach as far as f32's, it is lowered by what the
+    reference may lag behind, so that weights are at most 1 and a sum of p v is no larger than with the row's maximum."""
+    return QUANT_LIFT if quant else F16_LIFT if dtype == "f16" else -RESCALE
 
 
 def _f32(v: float) -> str:
@@ -854,7 +860,8 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
     s_ = [e.r("f") for _ in range(BKV)]
     jj_s = o("mov.u32", 0)
     out_cvt = "cvt.rn.f16x2.f32" if dtype == "f16" else "cvt.rn.bf16x2.f32"
-    lift = 0.0 if not p_f16 else QUANT_LIFT if quant else F16_LIFT
+    lift = lift_of(dtype, quant)
+    out_lift = -RESCALE if quant else lift                     # of the parts: weights of at most 1 before vref comes in
 
     def add_specials(S, j, jj, buf, ph, key0, *rest):
         """Tiles in which a key is seen by some rows only: takes the rare path when the V rows hold an infinity or a NaN.
@@ -1188,8 +1195,6 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
             e(f"@{e.cond('ne.u32', S.nb, S.P.tiles)} bra {l_part};")            # the unit has other runs too
         p_zero = e.cond("eq.f32", lsum, "0f00000000")
         inv = o("rcp.rn.f32", o("selp.f32", "0f3F800000", lsum, p_zero, cls="f"), cls="f")
-        if quant:
-            e(f"mul.f32 {inv}, {inv}, {vref};")
         oa = at(o_ptr, wide(S.row_index(rowl), row_b))
         for c in range(D // 32):
             regs = s_[:32]
@@ -1199,6 +1204,8 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
             for k in range(16):
                 x0 = o("mul.f32", regs[2 * k], inv, cls="f")
                 x1 = o("mul.f32", regs[2 * k + 1], inv, cls="f")
+                if quant:                                       # not inv * vref: that may fall below f32's normal numbers
+                    x0, x1 = o("mul.f32", x0, vref, cls="f"), o("mul.f32", x1, vref, cls="f")
                 words.append(o("selp.b32", 0, o(out_cvt, x1, x0), p_zero))
             for i in range(2):
                 e(f"@{p_row} st.global.v8.b32 [{oa}+{64 * c + 32 * i}], {{{', '.join(words[8 * i:8 * i + 8])}}};")
@@ -1209,18 +1216,21 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
             part = o("add.u32", o("shl.b32", cta, 1), o("selp.u32", 1, 0, e.cond("ne.u32", S.now, start)))
             pi = o("mad.lo.u32", part, rows, rowl)
             pa = at(gptr("p_part"), wide(pi, D * 4))
+            if quant:
+                vout = o("mul.f32", vref, _f32(2.0 ** (out_lift - lift)), cls="f")
+                e(f"mul.f32 {lsum}, {lsum}, {_f32(2.0 ** (out_lift - lift))};")
             for c in range(D // 32):
                 regs = s_[:32]
                 e(f"tcgen05.ld.sync.aligned.32x32b.x32.b32 {{{', '.join(regs)}}}, [{lanebase}+{32 * c}];")
                 e("tcgen05.wait::ld.sync.aligned;")
                 if quant:
                     for x in regs:
-                        e(f"mul.f32 {x}, {x}, {vref};")
+                        e(f"mul.f32 {x}, {x}, {vout};")
                 for i in range(4):
                     e(f"@{p_row} st.global.v8.f32 [{pa}+{128 * c + 32 * i}], {{{', '.join(regs[8 * i:8 * i + 8])}}};")
             mla = at(at(gptr("p_part"), 2 * ctas * rows * D * 4), wide(pi, 8))
             # the parts' O and l stand for 2^-negm; a part that saw nothing has m = -inf
-            meff = o("sub.f32", mref, _f32(lift), cls="f")
+            meff = o("sub.f32", mref, _f32(out_lift), cls="f")
             e(f"@{p_row} st.global.v2.f32 [{mla}], {{{meff}, {lsum}}};")
         e.label(l_noepi)
 

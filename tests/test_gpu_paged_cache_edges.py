@@ -7,7 +7,7 @@ from emmy_ptx_b200.compiler import compile_graph
 from emmy_ptx_b200.ir import Graph
 from emmy_ptx_b200.runtime import Executable
 from tests import pagedref as R
-from tests.test_paged_cache_edges import SIGNED, SIGNS, signed_case
+from tests.test_paged_cache_edges import RANGES, SIGNED, SIGNS, check_scaled, ramp_case, signed_case
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +32,18 @@ def test_scales_of_any_sign(case, dtype, signs, opts):
     got = go(p, t, {**case[-1], **opts})
     ref, bound, _ = R.attention_ref(t, case[5])
     R.check(got["O"], ref, bound, signs)
+
+
+@pytest.mark.parametrize("opts", [{"paged_ctas": 0}, {"paged_ctas": 3, "paged_min_tiles": 1}], ids=["whole", "runs"])
+@pytest.mark.parametrize("rows", [0, 64])
+@pytest.mark.parametrize("n", [230, 8000])
+@pytest.mark.parametrize("quant,k", [*RANGES, (True, 112), (False, 112)])
+def test_values_near_the_ends_of_f32(quant, k, n, rows, opts):
+    if k == 119 and n == 8000:
+        k = 114                                               # the weights sum to more: 2^119 would leave f32 with any kernel
+    t, big, p = ramp_case(quant, k, n)
+    base = go(p, t, {**opts, "paged_rows": rows})["O"]
+    got = go(p, big, {**opts, "paged_rows": rows})["O"]
+    ref, bound, _ = R.attention_ref(t, 16)
+    R.check(base, ref, bound, "before")
+    check_scaled(got, base, k)

@@ -38,3 +38,55 @@ def test_scales_of_any_sign(case, dtype, signs, rows):
     assert code == 0
     ref, bound, _ = R.attention_ref(t, case[5])
     R.check(got["O"], ref, bound, signs)
+
+
+# ---- values near both ends of f32 ------------------------------------------------------------
+
+
+def ramp_case(quant, k, n=230):
+    """Scores that grow by almost 2^8 along the keys (a kernel that takes its reference from the first ones has weights
+    up to 2^8 here), values times 2^k.  Values of one sign, so that no sum cancels."""
+    d, page = 64, 16
+    t, pages = R.make("attend", 1, 1, d, page, -(-n // page), [n], [2], chunk=2, heads=2, quant=quant, seed=4)
+    u = torch.ones(d)
+    x = torch.zeros(pages, 1, page, d)
+    for j in range(n):
+        x[int(t["table"][0, j // page]), 0, j % page] = u * (j / n) * 5.4 / 8
+    t["Q"][:] = 1.0                                           # the last key's score: 64 * 5.4 / 8 / 8
+    v = (x + 1) * torch.rand(x.shape, generator=torch.Generator().manual_seed(1)).add(0.25)
+    for name, y in (("K", x), ("V", v)):
+        if quant:
+            t[name + "C"], t[name + "S"] = R.quantise(y.to(torch.bfloat16))
+        else:
+            t[name + "C"] = y.to(torch.bfloat16)
+    big = dict(t)
+    if quant:
+        big["VS"] = t["VS"] * 2.0 ** k
+    else:
+        big["VC"] = t["VC"] * 2.0 ** k
+    return t, big, irgen.paged_attention_ir(1, 2, 2, 1, d, pages, page, -(-n // page), "bf16", quant)
+
+
+#: bytes down to scales of 2^-126, both kinds up to sums of 2^127 with weights of at most 1
+RANGES = [(False, 119), (True, 119), (True, -119)]
+
+
+def check_scaled(got, base, k):
+    """Values times 2^k give the output times 2^k: everything between is a product with a power of two, exact but where
+    it leaves the normal numbers (by 2^-141 here, which may turn the last rounding: one step of bf16)."""
+    want = base.double() * 2.0 ** k
+    err = (got.double() - want).abs()
+    assert bool((err <= (2.0 ** -7 * want.abs() + 2.0 ** -133 if k < 0 else 0 * want)).all()), (err / want).max()
+
+
+@pytest.mark.parametrize("opts", [{}, {"paged_ctas": 3, "paged_min_tiles": 1}], ids=["whole", "runs"])
+@pytest.mark.parametrize("rows", [0, 64])
+@pytest.mark.parametrize("quant,k", RANGES)
+def test_values_near_the_ends_of_f32(quant, k, rows, opts):
+    t, big, p = ramp_case(quant, k)
+    base, c0, _ = PE.run(p, t, {**opts, "paged_rows": rows})
+    got, c1, _ = PE.run(p, big, {**opts, "paged_rows": rows})
+    assert c0 == c1 == 0
+    ref, bound, _ = R.attention_ref(t, 16)
+    R.check(base["O"], ref, bound, "before")
+    check_scaled(got["O"], base["O"], k)
