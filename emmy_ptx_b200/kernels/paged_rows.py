@@ -42,7 +42,7 @@ from __future__ import annotations
 import math
 
 from .ptxasm import wait_bar_warp
-from .tc_paged_attention import LOG2E, RESCALE, _E, _f32, _unit, lift_of
+from .tc_paged_attention import LOG2E, RESCALE, _E, _f32, _unit, lift_of, q_most
 
 MAX_ROWS = 64
 ERR_ROWS = 77                    # a block's copy never completed
@@ -387,7 +387,7 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
                     e(f"@{okr} ld.global.nc.v4.b32 {{{', '.join(d_)}}}, [{src}+{hb * 128 + i * per_p + 16 * x}];")
                     got += d_
         if q_f16 and not half:
-            # bf16 to f16: the row times a power of two that brings its largest number to 2^14 (at most 2^40), exact
+            # bf16 to f16: the row times a power of two that brings its largest number to 2^14 (see q_most), exact
             # but for numbers 2^-28 of the largest and less; the scores take the inverse
             big = None
             for x in got:
@@ -397,7 +397,7 @@ def paged_rows_entry(name, batch, chunk, heads, kv_heads, dim, pages, page, max_
             for d_ in (1, 2):
                 big = o("max.u32", big, o("shfl.sync.bfly.b32", big, d_, 31, -1))
             ex = o("sub.s32", 127 + 14, o("shr.u32", big, 7))     # 14 less the largest's exponent
-            ex = o("min.s32", ex, 40)
+            ex = o("min.s32", ex, q_most(scale))
             up = o("shl.b32", o("add.s32", ex, 127), 23, cls="f")
             down = o("shl.b32", o("sub.s32", 127, ex), 23, cls="f")
             crow.append(o("mul.f32", down, cscale, cls="f"))

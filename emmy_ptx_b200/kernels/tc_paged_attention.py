@@ -27,10 +27,11 @@ scores' columns, the values' scales multiply P.
 
 **Numerics.**  The score buffers, the running reference and sum, and O are f32.  P is rounded for the tensor core:
 f16 caches take f16 P, to nearest (2^-11), with 2^7 put on the exponent so that small weights keep their bits;
-bf16 caches take P as two bf16 parts, truncated, 2^-14 together, of 2^(s - m - 8): at most 1.  Bytes are multiplied in f16: a bf16 Q row is
-brought to 2^14 by a power of two (exact but for numbers 2^-28 of its largest), and P carries the values' scales over
-a running power of two, at least half the largest scale so far (scales have any sign: the largest magnitude), so that it
-stays below 2^15 and what is 2^-20 of the largest still has 11 bits.  O is rescaled only when the row's maximum grew by more than 2^8, or that power did.
+bf16 caches take P as two bf16 parts, truncated, 2^-14 together, lowered by the 2^8 the reference may lag behind.  Bytes
+are multiplied in f16: a bf16 Q row is brought to 2^14 by a power of two (exact but for numbers 2^-28 of its largest: see
+:func:`q_most`), and P carries the values' scales over a running power of two, at least half the largest scale so far (by
+magnitude), so that it stays below 2^15 and what is 2^-20 of the largest still has 11 bits.  O is rescaled only when the
+row's maximum grew by more than 2^8, or that power did.
 
 **What is masked.**  Scores past the row's own position, outside its window or of a page that the table does not
 name become -inf; a row that sees nothing ends as 0.  Rows of a V tile that no row of the CTA sees are zeroed in
@@ -44,6 +45,7 @@ Every wait is bounded and reports a code (71-76); TMEM is always freed.
 """
 from __future__ import annotations
 
+import math
 import struct
 
 from .ptxasm import Asm, idesc_f16, smem_desc_hi, wait_bar, wait_bar_warp
@@ -86,6 +88,13 @@ def lift_of(dtype, quant) -> float:
     """What P's exponent is lifted by.  In bf16, whose exponents reach as far as f32's, it is lowered by what the
     reference may lag behind, so that weights are at most 1 and a sum of p v is no larger than with the row's maximum."""
     return QUANT_LIFT if quant else F16_LIFT if dtype == "f16" else -RESCALE
+
+
+def q_most(scale) -> int:
+    """The largest power of two that a bf16 Q row is multiplied by for f16: the row's scores take its inverse with the
+    scale, and both stay normal f32 numbers.  Rows whose largest number is 2^(14 - q_most) or more (2^-109 with the
+    usual scale at dim 128) reach 2^14; a row of zeros takes any power."""
+    return min(126, 126 + math.frexp(scale * LOG2E)[1] - 1)
 
 
 def _f32(v: float) -> str:
@@ -953,7 +962,7 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
                 rr_.append(r_)
             for d_, r_ in zip(ws, rr_):
                 if recast:
-                    # the row's largest number to 2^14 by a power of two (at most 2^40), then f16: see above
+                    # the row's largest number to 2^14 by a power of two, then f16: see above
                     big = None
                     for x in d_:
                         a_ = o("and.b32", x, "0x7FFF7FFF")
@@ -963,7 +972,7 @@ def paged_attention_entry(name, batch, chunk, heads, kv_heads, dim, pages, page,
                     while k_ < per_row:
                         big = o("max.u32", big, o("shfl.sync.bfly.b32", big, k_, 31, -1))
                         k_ *= 2
-                    ex = o("min.s32", o("sub.s32", 127 + 14, o("shr.u32", big, 7)), 40)
+                    ex = o("min.s32", o("sub.s32", 127 + 14, o("shr.u32", big, 7)), q_most(scale))
                     up = o("shl.b32", o("add.s32", ex, 127), 23, cls="f")
                     down = o("shl.b32", o("sub.s32", 127, ex), 23, cls="f")
                     qsa = o("mad.lo.u32", r_, 4, bars)

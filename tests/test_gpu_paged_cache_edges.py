@@ -7,7 +7,7 @@ from emmy_ptx_b200.compiler import compile_graph
 from emmy_ptx_b200.ir import Graph
 from emmy_ptx_b200.runtime import Executable
 from tests import pagedref as R
-from tests.test_paged_cache_edges import RANGES, SIGNED, SIGNS, check_scaled, ramp_case, signed_case
+from tests.test_paged_cache_edges import QSIZES, RANGES, SIGNED, SIGNS, check_scaled, ramp_case, signed_case, sized_case
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +47,11 @@ def test_values_near_the_ends_of_f32(quant, k, n, rows, opts):
     ref, bound, _ = R.attention_ref(t, 16)
     R.check(base, ref, bound, "before")
     check_scaled(got, base, k)
+
+
+@pytest.mark.parametrize("rows", [0, 64])
+@pytest.mark.parametrize("q2,k2,scale", QSIZES)
+def test_queries_of_any_size_over_bytes(q2, k2, scale, rows):
+    t, p = sized_case(q2, k2, scale)
+    ref, bound, _ = R.attention_ref(t, 16, scale=scale)
+    R.check(go(p, t, {"paged_rows": rows})["O"], ref, bound, "sizes")

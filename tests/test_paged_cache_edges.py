@@ -90,3 +90,28 @@ def test_values_near_the_ends_of_f32(quant, k, rows, opts):
     ref, bound, _ = R.attention_ref(t, 16)
     R.check(base["O"], ref, bound, "before")
     check_scaled(got["O"], base["O"], k)
+
+
+# ---- queries of any size over a cache of bytes -----------------------------------------------
+
+
+QSIZES = [(-60, 60, None), (-97, 97, None), (-109, 100, 64.0), (-40, 97, 2.0 ** -60), (100, -100, None), (-26, 26, None)]
+
+
+def sized_case(q2, k2, scale):
+    """Queries times 2^q2 against key scales times 2^k2: ordinary scores, times 2^(q2 + k2)."""
+    t, pages = R.make("attend", 1, 2, 64, 16, 8, [120], [2], chunk=2, heads=4, quant=True, seed=11)
+    t["Q"] = t["Q"] * 2.0 ** q2
+    t["Q"][0, 1, 1] = 0.0                                     # a row of zeros: the mean of the values
+    t["KS"] = t["KS"] * 2.0 ** k2
+    return t, irgen.paged_attention_ir(1, 2, 4, 2, 64, pages, 16, 8, "bf16", True, scale=scale)
+
+
+@pytest.mark.parametrize("rows", [0, 64])
+@pytest.mark.parametrize("q2,k2,scale", QSIZES)
+def test_queries_of_any_size_over_bytes(q2, k2, scale, rows):
+    t, p = sized_case(q2, k2, scale)
+    got, code, _ = PE.run(p, t, {"paged_rows": rows})
+    assert code == 0
+    ref, bound, _ = R.attention_ref(t, 16, scale=scale)
+    R.check(got["O"], ref, bound, "sizes")
