@@ -552,7 +552,10 @@ def _lower_paged_attention(graph, node, kw, prefix, options):
         join = form.join_entry(f"{name}_join", **geo, dim=kw["dim"], dtype=kw["dtype"], names=names[-3:], scratch=scratch,
                                ctas=ctas, min_tiles=least)
     main["args"] = _args_of(graph, node)
-    return [main, join] if join else main
+    if not join:
+        return main
+    join["args"] = [a for a in main["args"] if a["name"] in join["params"]]
+    return [main, join]
 
 
 def _flat(body):

@@ -6,9 +6,10 @@ record lists (``zero_outputs``, tools/stress.py:106-111), checks every pointer's
 what the emitted code assumes, encodes TMA descriptors for tensor-core kernels, and launches
 the entries in order on the caller's stream.  Buffers are caller-owned tensors on the device.
 
-Modules whose records list their tensors (``"args"``: the paged-cache operators) go a shorter way: each entry has a
-launch plan in the C library, a call checks its tensors against the list and passes pointers, and scratch
-that a record marks ``"per_call"`` is allocated by the call.
+Records may list their tensors (``"args"``: the paged-cache operators): a call checks those tensors against the lists.
+Scratch that a record marks ``"per_call"`` is allocated by the call.  Modules whose records all have lists (and need
+nothing else of the general path) go a shorter way: each entry has a launch plan in the C library, and a call passes
+pointers.
 
 An entry whose record says ``"stream": 1`` runs on the Executable's side stream instead, so that it
 overlaps the main stream's next entries; ``"after": [entry, ...]`` names entries it must follow
@@ -18,6 +19,7 @@ stream before the call returns, so callers (and CUDA-graph capture) see one stre
 from __future__ import annotations
 
 import ctypes
+import math
 import operator
 
 from .compiler import CompiledModule, compile_ir
@@ -80,24 +82,41 @@ class Executable:
         if any(spec.get("kind") == "errword" for rec in compiled.kernels for spec in rec.get("extra", [])):
             self.err = self._device_tensor((4,), torch.int32)
             self.err.zero_()
-        # a module whose first record lists its tensors ("args") is launched from plans
+        args: dict = {}                      # what a call's tensors must be: name -> (dtype, shape)
+        self._temp = {}                      # scratch each call allocates: name -> (element count, dtype)
+        for rec in compiled.kernels:
+            for a in rec.get("args", []):
+                want = (torch_dtype(a["dtype"]), tuple(a["shape"]))
+                if args.setdefault(a["name"], want) != want:
+                    raise ValueError(f"two kernels of the module take {a['name']!r}, as {args[a['name']]} and {want}")
+            for spec in rec.get("scratch", []):
+                if spec.get("per_call"):
+                    self._temp[spec["name"]] = (math.prod(int(x) for x in spec["shape"]), torch_dtype(spec["dtype"]))
+        self._args = [(name, *want) for name, want in args.items()]
         self.plans = None
-        if compiled.kernels and compiled.kernels[0].get("args"):
+        if compiled.kernels and all(self._plannable(rec) for rec in compiled.kernels):
             self._make_plans()
+        # alignments to check before the first launch: those that it does not check itself
+        aligns = [rec.get("align", {}) for rec in compiled.kernels]
+        self._aligned = []
+        for i, name in enumerate(args):
+            need = max((int(a.get(name, 1)) for a in aligns), default=1)
+            if need > (int(aligns[0].get(name, 1)) if self.plans else 1):
+                self._aligned.append((i, name, need))
+
+    @staticmethod
+    def _plannable(rec: dict) -> bool:
+        """Whether a plan holds all that a launch of the entry takes: listed tensors and the call's own scratch, nothing
+        zeroed, no second stream, no parameter but pointers, tensor maps and the status word."""
+        return (bool(rec.get("args")) and all(spec.get("per_call") for spec in rec.get("scratch", []))
+                and all(spec.get("kind") == "errword" for spec in rec.get("extra", []))
+                and not any(rec.get(k) for k in ("zero_outputs", "stream", "after", "exchange", "self_zeroing")))
 
     def _make_plans(self) -> None:
-        """One launch plan per entry, and what a call's tensors must be."""
-        import torch
-        self._args = [(a["name"], torch_dtype(a["dtype"]), tuple(a["shape"])) for a in self.records[0]["args"]]
+        """One launch plan per entry."""
         self._calls = []
-        self._temp = {}                      # scratch each call allocates: name -> (element count, dtype)
         self.plans = []
         for rec, fn in zip(self.records, self.funcs):
-            for spec in rec.get("scratch", []):
-                n = 1
-                for x in spec["shape"]:
-                    n *= int(x)
-                self._temp[spec["name"]] = (n, torch_dtype(spec["dtype"]))
             names = rec["params"]
             tmaps = [(names.index(s["tensor"]), _TMAP_DTYPE[s["dtype"]], s["dims"], s["strides"], s["box"],
                       _SWIZZLE[s.get("swizzle", "128B")], s.get("l2promo", 2)) for s in rec.get("tmaps", [])]
@@ -110,33 +129,45 @@ class Executable:
         order = [name for name, _, _ in self._args] + list(self._temp)
         self._calls = [operator.itemgetter(*map(order.index, names)) for names in self._calls]
 
-    def _run_plans(self, tensors: dict, stream) -> None:
-        """Check the call's tensors (type, shape, layout, device), allocate its scratch on its stream and launch
-        every entry.  Scratch is the call's own (torch's allocator, so a captured call's belongs to its
-        graph): calls of one Executable may overlap on the GPU as long as what they write does not."""
-        import torch
-        if not self.plans:
-            raise ValueError(f"kernel {self.records[0]['entry']!r} was closed")
+    def _check(self, tensors: dict) -> list:
+        """The addresses of the listed tensors; refuses another type, shape, layout, device or alignment."""
         index, vals = self.index, []
         for name, dtype, shape in self._args:
             t = tensors.get(name)
             if t is None:
-                raise ValueError(f"kernel {self.records[0]['entry']!r} needs the tensor {name!r}")
+                owner = next(r["entry"] for r in self.records if any(a["name"] == name for a in r.get("args", [])))
+                raise ValueError(f"kernel {owner!r} needs the tensor {name!r}")
             if t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or t.get_device() != index:
                 raise ValueError(
                     f"{name!r} must be a contiguous {dtype} tensor of shape {list(shape)} on cuda:{index}, not "
                     f"{'a strided' if not t.is_contiguous() else 'a'} {t.dtype} of shape {list(t.shape)} on {t.device}")
             vals.append(t.data_ptr())
-        if self._temp:
-            device = f"cuda:{index}"
-            if stream is None:
-                keep = [torch.empty(n, dtype=dt, device=device) for n, dt in self._temp.values()]
-            else:
-                with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
-                    keep = [torch.empty(n, dtype=dt, device=device) for n, dt in self._temp.values()]
-            vals += [t.data_ptr() for t in keep]
+        for i, name, need in self._aligned:
+            if vals[i] % need:
+                raise ValueError(f"{name!r} must be {need}-byte aligned")
+        return vals
+
+    def _call_scratch(self, stream) -> dict:
+        """The scratch of one call, allocated on its stream (torch's allocator, so a captured call's belongs to its
+        graph): calls of one Executable may overlap on the GPU as long as what they write does not."""
+        import torch
+        device = f"cuda:{self.index}"
         if stream is None:
-            stream = torch._C._cuda_getCurrentRawStream(index)
+            return {name: torch.empty(n, dtype=dt, device=device) for name, (n, dt) in self._temp.items()}
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+            return {name: torch.empty(n, dtype=dt, device=device) for name, (n, dt) in self._temp.items()}
+
+    def _run_plans(self, tensors: dict, stream) -> None:
+        """Check the call's tensors, allocate its scratch and launch every entry."""
+        import torch
+        if not self.plans:
+            raise ValueError(f"kernel {self.records[0]['entry']!r} was closed")
+        vals = self._check(tensors)
+        if self._temp:
+            keep = self._call_scratch(stream)
+            vals += [t.data_ptr() for t in keep.values()]
+        if stream is None:
+            stream = torch._C._cuda_getCurrentRawStream(self.index)
         for plan, pick, rec in zip(self.plans, self._calls, self.records):
             try:
                 self.dev.launch_plan(plan, pick(vals), stream)
@@ -169,8 +200,8 @@ class Executable:
         from .launcher import ATTR_NUM_REGS
         return self.dev.func_attribute(self.funcs[i], ATTR_NUM_REGS)
 
-    def _tmap(self, spec: dict, t) -> ctypes.Array:
-        key = (spec["name"], t.data_ptr(), tuple(t.shape))
+    def _tmap(self, entry: str, spec: dict, t) -> ctypes.Array:
+        key = (entry, spec["name"], t.data_ptr(), tuple(t.shape))
         hit = self._tmap_cache.get(key)
         if hit is not None:
             return hit
@@ -221,7 +252,7 @@ class Executable:
                 keep.append(v)
                 args.append(ctypes.cast(ctypes.byref(v), ctypes.c_void_p).value)
             for spec in rec.get("tmaps", []):
-                blob = self._tmap(spec, tensors[spec["tensor"]])
+                blob = self._tmap(rec["entry"], spec, tensors[spec["tensor"]])
                 keep.append(blob)
                 args.append(blob.addr)
             for spec in rec.get("extra", []):
@@ -258,6 +289,10 @@ class Executable:
         import torch
         if self.plans is not None:
             return self._run_plans(tensors, stream)
+        if self._args:
+            self._check(tensors)
+        if self._temp:
+            tensors = {**tensors, **self._call_scratch(stream)}
         if stream is None:
             stream = torch.cuda.current_stream(self.index).cuda_stream
         if self.side is None:

@@ -3,11 +3,14 @@ cases and references: :mod:`tests.test_paged_cache_edges`, :mod:`tests.pagedref`
 import pytest
 import torch
 
+from emmy_ptx_b200 import data
 from emmy_ptx_b200.compiler import compile_graph
 from emmy_ptx_b200.ir import Graph
 from emmy_ptx_b200.runtime import Executable
 from tests import pagedref as R
-from tests.test_paged_cache_edges import QSIZES, RANGES, SIGNED, SIGNS, check_scaled, ramp_case, signed_case, sized_case
+from tests.test_paged_cache_edges import (QSIZES, RANGES, RUNS, SIGNED, SIGNS, check_scaled, joined, other_first, ramp_case, signed_case,
+                                          sized_case, step_problems, step_refs)
+from tests.test_paged_cache import same
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +58,78 @@ def test_queries_of_any_size_over_bytes(q2, k2, scale, rows):
     t, p = sized_case(q2, k2, scale)
     ref, bound, _ = R.attention_ref(t, 16, scale=scale)
     R.check(go(p, t, {"paged_rows": rows})["O"], ref, bound, "sizes")
+
+
+def step_graph(more=(), opts=None):
+    t, problems = step_problems()
+    g, meta = joined(*more, *problems)
+    return t, Executable(compile_graph(Graph.from_dict(g), meta, opts or RUNS), device=0)
+
+
+def check_step(g, t):
+    want, ref, bound = step_refs(t, False)
+    R.check(g["O"], ref, bound, "step")
+    for n in ("KC", "VC", "KR", "VR"):
+        same(g[n].cpu(), want[n], n)
+
+
+def test_a_serving_step_as_one_graph():
+    """Write, attend and read back as one module's plans: called, and captured and replayed with other inputs."""
+    t, ex = step_graph()
+    assert len(ex.plans) == 4
+    g = {k: v.cuda() for k, v in t.items()}
+    ex(g)
+    torch.cuda.synchronize()
+    check_step(g, t)
+    graph, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=s):
+        ex(g)
+    gen = torch.Generator().manual_seed(9)
+    host = {k: v.cpu().clone() for k, v in g.items()}
+    for n in ("K", "V", "Q"):
+        host[n] = torch.randn(host[n].shape, generator=gen).to(host[n].dtype)
+        g[n].copy_(host[n])
+    host["lens"] += 1
+    g["lens"].copy_(host["lens"])
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    check_step(g, host)
+    ex.check()
+
+
+def test_a_cache_operator_beside_another_kernel():
+    """A kernel that is no cache operator in the same module: the general path, on the current stream, on a stream
+    given by its handle, and captured."""
+    q = other_first()
+    t, ex = step_graph([q])
+    assert ex.plans is None
+    t = {**t, **data.make_inputs(q)}
+    g = {k: v.cuda() for k, v in t.items()}
+    x = next(a.name for a in q.inputs)
+    total = t[x].double().sum().item()
+    tol = t[x].numel() * 2.0 ** -24 * t[x].double().abs().sum().item()            # an f32 sum in any order
+
+    def fresh():
+        for n in t:
+            g[n].copy_(t[n])
+        torch.cuda.synchronize()
+
+    def check():
+        torch.cuda.synchronize()
+        check_step(g, t)
+        assert abs(g["out"].double().sum().item() - total) <= tol
+    ex(g)
+    check()
+    fresh()
+    s = torch.cuda.Stream()
+    ex.run(g, s.cuda_stream)
+    check()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        ex(g)
+    for _ in range(2):
+        fresh()
+        graph.replay()
+        check()
+    ex.check()

@@ -1,11 +1,19 @@
 """The paged key/value cache at the edges of what its definition allows, on the CPU (emulated kernels, recording
 devices) against plain float64."""
+import ctypes
+import json
+from types import SimpleNamespace
+
 import pytest
 import torch
 
-from emmy_ptx_b200 import irgen
+from emmy_ptx_b200 import data, irgen, launcher
+from emmy_ptx_b200.compiler import compile_graph
+from emmy_ptx_b200.ir import Graph
+from emmy_ptx_b200.runtime import Executable
 from tests import pagedemu as PE
 from tests import pagedref as R
+from tests.test_paged_cache import same
 
 #: scales as other programs may leave them: a factor for every token of every head
 SIGNS = {"negative": lambda n: -torch.ones(n), "alternating": lambda n: 1.0 - 2.0 * (torch.arange(n) % 2),
@@ -115,3 +123,201 @@ def test_queries_of_any_size_over_bytes(q2, k2, scale, rows):
     assert code == 0
     ref, bound, _ = R.attention_ref(t, 16, scale=scale)
     R.check(got["O"], ref, bound, "sizes")
+
+
+# ---- several kernels in one graph ------------------------------------------------------------
+
+
+def joined(*problems):
+    """(graph, meta) of the problems' kernels one after the other, tensors of one name shared."""
+    nodes = {}
+    for p in problems:
+        nodes.update({n: x for n, x in p.graph["nodes"].items() if x["op"] == "KernelOp"})
+    made = {o["name"] for x in nodes.values() for o in x["outputs"]}
+    ins = {n: x for p in problems for n, x in p.graph["nodes"].items() if x["op"] == "InputOp" and n not in made}
+    graph = {"nodes": {**ins, **nodes}, "inputs": list(ins), "outputs": sorted(made)}
+    return graph, {"kernels": [k for p in problems for k in p.meta()["kernels"]]}
+
+
+def step_problems(quant=False):
+    """A decode step's write, attention and read back, and all their tensors."""
+    B, H, hk, d, page, mp = 2, 4, 2, 64, 16, 6
+    lens = [30, 61]
+    w, pages = R.make("write", B, hk, d, page, mp, lens, [1, 1], quant=quant, seed=3)
+    a, _ = R.make("attend", B, hk, d, page, mp, lens, [1, 1], heads=H, quant=quant, seed=4)
+    r, _ = R.make("read", B, hk, d, page, mp, lens, [1, 1], length=mp * page, quant=quant, seed=5)
+    c = (hk, d, pages, page, mp, "bf16", quant)
+    return {**r, **a, **w}, (irgen.cache_write_ir(B, 1, *c), irgen.paged_attention_ir(B, 1, H, *c),
+                             irgen.cache_read_ir(B, mp * page, *c))
+
+
+def step_refs(t, quant, page=16):
+    """The tensors after the step, and the attention's bound."""
+    t = {**t, **R.write_ref(t, page, quant)}
+    ref, bound, _ = R.attention_ref(t, page)
+    return {**t, **R.read_ref(t, page, "bf16")}, ref, bound
+
+
+class Recorder:
+    """A device that notes what it is asked to launch, from plans and without; see :class:`tests.test_paged_cache.PlanDevice`."""
+
+    def __init__(self):
+        self.plans, self.log, self.maps = [], [], []
+
+    def load_ptx(self, ptx):
+        return "module"
+
+    def function(self, mod, entry):
+        return entry
+
+    def set_max_dyn_smem(self, fn, nbytes):
+        pass
+
+    def plan(self, fn, *args, **kw):
+        self.plans.append(fn)
+        return fn
+
+    def launch_plan(self, plan, params, stream):
+        self.log.append(("plan", plan, list(params), stream))
+
+    def launch(self, fn, grid, block, dyn_smem, stream, arg_ptrs, cluster=(1, 1, 1), pdl=False):
+        self.log.append(("launch", fn, [ctypes.cast(a, ctypes.POINTER(ctypes.c_uint64))[0] for a in arg_ptrs], stream))
+
+    def launch_u64(self, fn, grid, block, dyn_smem, stream, params, align=None, pdl=False):
+        self.log.append(("launch", fn, list(params), stream))
+
+    def tmap_encode_tiled(self, out_buf, dtype, gaddr, dims, strides, box, **kw):
+        self.maps.append((gaddr, tuple(box)))
+
+    def memset_d32(self, ptr, value, count, stream):
+        self.log.append(("zero", ptr, count, stream))
+
+    def destroy_plan(self, plan):
+        pass
+
+    def unload(self, mod):
+        pass
+
+
+class HostExecutable(Executable):
+    def _device_tensor(self, shape, dtype):
+        return torch.empty(shape, dtype=dtype)
+
+    def _call_scratch(self, stream):
+        return {n: torch.empty(k, dtype=dt) for n, (k, dt) in self._temp.items()}
+
+
+@pytest.fixture
+def recorder(monkeypatch):
+    dev = Recorder()
+    monkeypatch.setattr(launcher.Device, "get", classmethod(lambda cls, index=0: dev))
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)          # CPU tensors pass for cuda:0's
+    return dev
+
+
+def shifted(x, by=2):
+    """The same tensor ``by`` bytes past a 64-byte boundary."""
+    raw = torch.empty(x.numel() * x.element_size() + 128, dtype=torch.uint8)
+    at = -raw.data_ptr() % 64 + by
+    y = raw[at:at + x.numel() * x.element_size()].view(x.dtype).view(x.shape)
+    return y.copy_(x)
+
+
+RUNS = {"paged_ctas": 3, "paged_min_tiles": 1}
+
+
+def host_executable(problems, opts=None):
+    g, meta = joined(*problems)
+    return HostExecutable(compile_graph(Graph.from_dict(g), meta, opts or {}), device=0)
+
+
+def test_a_graph_of_cache_operators_runs_from_plans(recorder):
+    t, problems = step_problems()
+    ex = host_executable(problems, RUNS)
+    names = ["cache_write", "paged_attention", "paged_attention_join", "cache_read"]
+    assert [r["entry"] for r in ex.records] == names == recorder.plans
+    ex.run(t, 55)
+    assert [(x[0], x[1], x[3]) for x in recorder.log] == [("plan", n, 55) for n in names]
+    for (_, _, ptrs, _), rec in zip(recorder.log, ex.records):
+        want = [t[n].data_ptr() if n in t else None for n in rec["params"]]
+        assert [x for x, y in zip(ptrs, want) if y is not None] == [y for y in want if y is not None]
+    part = [x[2][ex.records[i]["params"].index("paged_attention__paged_attention__part")] for i, x in enumerate(recorder.log)
+            if i in (1, 2)]
+    assert part[0] == part[1] and part[0]
+    for name in ("K", "Q", "KR"):                                  # every kernel's tensors are checked before any launch
+        for other in (t[name].float(), shifted(t[name]))[:1 if name == "K" else 2]:      # K's plan checks K itself
+            recorder.log.clear()
+            with pytest.raises(ValueError, match=repr(name)):
+                ex.run({**t, name: other}, 55)
+            assert recorder.log == []
+
+
+def other_first():
+    """A kernel that zeroes its output before it runs, beside the cache's."""
+    return irgen.SMALL["c2"]()
+
+
+@pytest.mark.parametrize("first", [True, False])
+def test_a_cache_operator_beside_another_kernel(recorder, first):
+    t, problems = step_problems()
+    q = other_first()
+    t = {**t, **data.make_inputs(q)}
+    ex = host_executable([q, problems[1]] if first else [problems[1], q], RUNS)
+    assert ex.plans is None and recorder.plans == []
+    ex.run(t, 55)
+    mine = [("launch", "paged_attention"), ("launch", "paged_attention_join")]
+    other = [("zero", t["out"].data_ptr()), ("launch", q.entry)]
+    assert [x[:2] for x in recorder.log] == (other + mine if first else mine + other)
+    calls = {x[1]: x[2] for x in recorder.log if x[0] == "launch"}
+    for rec in ex.records:
+        for n, x in zip(rec["params"], calls[rec["entry"]]):
+            if n in t:
+                assert x == t[n].data_ptr(), (rec["entry"], n)
+    i, j = (r["params"].index("paged_attention__paged_attention__part") for r in ex.records if "join" in r["entry"]
+            or r["entry"] == "paged_attention")
+    assert calls["paged_attention"][i] == calls["paged_attention_join"][j]
+    for other in (t["Q"][:, :, :3], shifted(t["Q"])):
+        recorder.log.clear()
+        with pytest.raises(ValueError, match="'Q'"):
+            ex.run({**t, "Q": other}, 55)
+        assert recorder.log == []
+
+
+def test_two_attentions_of_one_graph_have_their_own_tensor_maps(recorder):
+    # both name their map of the pool alike; their boxes differ
+    B, H, hk, d, page, mp = 1, 2, 1, 64, 64, 3
+    t, pages = R.make("attend", B, hk, d, page, mp, [150], [1], heads=H)
+    b, _ = R.make("attend", B, hk, d, page, mp, [150], [70], chunk=70, heads=H)
+    one = irgen.paged_attention_ir(B, 1, H, hk, d, pages, page, mp)
+    many = irgen.paged_attention_ir(B, 70, H, hk, d, pages, page, mp)
+    many.graph = json.loads(json.dumps(many.graph).replace('"Q"', '"Q2"').replace('"O"', '"O2"').replace(
+        '"paged_attention"', '"chunk_attention"'))
+    many.entry = "chunk_attention"
+    for a in many.args:
+        a.name = {"Q": "Q2", "O": "O2"}.get(a.name, a.name)
+    q = other_first()
+    t = {**t, "Q2": b["Q"], "O2": b["O"], **data.make_inputs(q)}
+    ex = host_executable([one, many, q])
+    assert [r["kind"] for r in ex.records[:2]] == ["paged_attention_rows", "tcgen05_paged_attention"] and ex.plans is None
+    ex.run(t, 55)
+    boxes = [tuple(s["box"]) for r in ex.records[:2] for s in r["tmaps"]]
+    assert [x for _, x in recorder.maps] == boxes and boxes[0] != boxes[2]
+    ex.run(t, 55)
+    assert len(recorder.maps) == len(boxes)                       # kept for the same pointers
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_a_serving_step_as_one_graph_emulated(quant):
+    t, problems = step_problems(quant)
+    g, meta = joined(*problems)
+    mod = compile_graph(Graph.from_dict(g), meta, RUNS)
+    specs = {a.name: a for p in problems for a in p.args}
+    outs = [specs[n] for n in g["outputs"]]
+    whole = SimpleNamespace(args=list(specs.values()), outputs=outs)
+    got, code, _ = PE.run(whole, t, mod=mod)
+    assert code == 0
+    want, ref, bound = step_refs(t, quant)
+    R.check(got["O"], ref, bound, "step")
+    for n in got:
+        if n != "O":
+            same(got[n], want[n], n)
