@@ -13,7 +13,7 @@ from emmy_ptx_b200.ir import Graph
 from emmy_ptx_b200.runtime import Executable
 from tests import pagedemu as PE
 from tests import pagedref as R
-from tests.test_paged_cache import same
+from tests.test_paged_cache import PlanDevice, same
 
 #: scales as other programs may leave them: a factor for every token of every head
 SIGNS = {"negative": lambda n: -torch.ones(n), "alternating": lambda n: 1.0 - 2.0 * (torch.arange(n) % 2),
@@ -321,3 +321,35 @@ def test_a_serving_step_as_one_graph_emulated(quant):
     for n in got:
         if n != "O":
             same(got[n], want[n], n)
+
+
+# ---- what the documents promise of addresses -------------------------------------------------
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_tensors_on_32_byte_boundaries_are_taken(recorder, monkeypatch, quant):
+    # what a plan's first entry checks itself is checked by the stand-in of tests.test_paged_cache
+    dev = PlanDevice()
+    monkeypatch.setattr(launcher.Device, "get", classmethod(lambda cls, index=0: dev))
+    t, problems = step_problems(quant)
+    for p, opts in [(problems[0], {}), (problems[1], {}), (problems[1], {"paged_rows": 0}), (problems[2], {})]:
+        ex = HostExecutable(compile_graph(Graph.from_dict(p.graph), p.meta(), opts), device=0)
+        mine = {a.name: shifted(t[a.name], 32) for a in p.args}
+        ex.run(mine, 55)
+        assert dev.log
+        for rec in ex.records:
+            for n, a in rec["align"].items():
+                assert a <= 32, (rec["entry"], n)
+        # 16 bytes are enough for what is loaded in pieces of 16, and refused before a launch where they are not
+        for name, a in ex.records[0]["align"].items():
+            if name in t:
+                dev.log.clear()
+                call = {**mine, name: shifted(t[name], 16)}
+                if a <= 16:
+                    ex.run(call, 55)
+                    assert dev.log
+                else:
+                    assert name in ("KC", "VC", "KR", "VR", "O")
+                    with pytest.raises(ValueError, match=f"'{name}' must be 32-byte"):
+                        ex.run(call, 55)
+                    assert dev.log == []
