@@ -700,8 +700,11 @@ class KernelEmitter:
         base = self.preg[buf]
         if var.is_const():
             return base, imm
-        if math.prod(self.shapes.get(buf, ())) > (1 << 32 if var.nonneg() else 1 << 31) - 1:
-            # the offset would wrap (or read as negative) and address other memory
+        lo, hi = var.range()
+        least, most = (0, (1 << 32) - 1) if var.nonneg() else (-(1 << 31), (1 << 31) - 1)
+        exact = var.single_atom() is not None if lo is None else least <= lo and hi <= most
+        if not exact and math.prod(self.shapes.get(buf, ())) > most:
+            # the offset could wrap (or read as negative) and address other memory
             raise Unsupported(f"buffer {buf!r} of shape {list(self.shapes[buf])} needs element offsets past the "
                               f"32-bit ones this form computes")
         key = ("gaddr", buf, var.key, esize)

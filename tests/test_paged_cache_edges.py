@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from emmy_ptx_b200 import data, irgen, launcher
+from emmy_ptx_b200.codegen.generic import Unsupported
 from emmy_ptx_b200.compiler import compile_graph
 from emmy_ptx_b200.ir import Graph
 from emmy_ptx_b200.runtime import Executable
@@ -353,3 +354,31 @@ def test_tensors_on_32_byte_boundaries_are_taken(recorder, monkeypatch, quant):
                     with pytest.raises(ValueError, match=f"'{name}' must be 32-byte"):
                         ex.run(call, 55)
                     assert dev.log == []
+
+
+# ---- buffers past 32 bits on the CUDA-core path ----------------------------------------------
+
+
+def big_buffer(shape, index, extra=()):
+    """y[i] = x[index] of 1024 elements, x of ``shape``."""
+    i = irgen
+    body = [i.Tile([i.Axis("i", 1024)], [*extra, i.Load(["a"], "x", index, "f32"), i.Write("y", ["a"], [i.V("i")], "f32")])]
+    args = [i.TensorSpec("x", shape, "f32"), i.TensorSpec("at", (1024,), "i32", ("randint", 0, 8)),
+            i.TensorSpec("y", (1024,), "f32", output=True)]
+    p = i.Problem("big", "test", "big", i._graph("big", args, body), args, grid=8, block=128)
+    return lambda: compile_graph(Graph.from_dict(p.graph), p.meta())
+
+
+def test_a_low_part_of_a_large_buffer_is_addressed():
+    i = irgen
+    at = [i.Load(["k"], "at", [i.V("i")], "i32")]
+    huge = 1 << 33
+    big_buffer((huge,), [i.V("i")])()                              # a range that is known, and short
+    big_buffer((1 << 10, huge >> 10), [0, i.Bin("*", i.V("i"), 4)])()
+    big_buffer((1 << 10, huge >> 10), [i.Bin("/", i.V("i"), 256), i.V("i")])()          # up to 3 rows of 2^23
+    big_buffer((huge,), [i.V("k")], at)()                          # a 32-bit number as it is
+    with pytest.raises(Unsupported, match="32-bit"):               # rows up to 1023 of 2^23: past 2^32
+        big_buffer((1 << 10, huge >> 10), [i.V("i"), 0])()
+    with pytest.raises(Unsupported, match="32-bit"):               # a row that only the data know
+        big_buffer((1 << 10, huge >> 10), [i.V("k"), i.V("i")], at)()
+    big_buffer((1 << 10, (1 << 31 >> 10) - 1), [i.V("k"), i.V("i")], at)()
