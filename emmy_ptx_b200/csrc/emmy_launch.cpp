@@ -520,13 +520,13 @@ int emmy_plan_launch(void* plan, const uint64_t* params, uint32_t nparams, void*
     args[n++] = &vals[nparams];
   }
   if (!p->ctx) return fail(EMMY_ERR_NOT_INIT, "emmy_init() had not been called when the plan was made");
-  // in the plan's context, whatever the thread's is, and back to that one
+  // in the plan's context, whatever the thread's is (also none), and back to that
   CUcontext cur = nullptr;
   if (int rc = cu(g_drv.CtxGetCurrent(&cur), "cuCtxGetCurrent")) return rc;
   if (cur != p->ctx)
     if (int rc = cu(g_drv.CtxSetCurrent(p->ctx), "cuCtxSetCurrent")) return rc;
   int rc = launch_here(p->function, p->grid, p->block, p->cluster, p->dyn_smem, stream, args, p->flags);
-  if (cur && cur != p->ctx)
+  if (cur != p->ctx)
     if (int back = cu(g_drv.CtxSetCurrent(cur), "cuCtxSetCurrent")) return rc ? rc : back;
   return rc;
 }

@@ -120,8 +120,8 @@ int emmy_tmap_encode_tiled(void* tmap, int dtype, uint32_t rank, uint64_t global
  * after the pointers) and one last 64-bit value (the status word's address).  emmy_plan_launch checks
  * the pointers' alignment (EMMY_ERR_BAD_ARG), encodes the maps and launches; it keeps its working
  * memory on the stack, so calls on one plan may overlap.  It launches in the context that was selected
- * when the plan was made and leaves the thread's own current.  A plan must be destroyed before its
- * module is unloaded.  No reference counterpart. */
+ * when the plan was made and leaves the thread's own current (none, where it had none).  A plan must be
+ * destroyed before its module is unloaded.  No reference counterpart. */
 #define EMMY_PLAN_MAX_PARAMS 16
 #define EMMY_PLAN_MAX_TMAPS 4
 int emmy_plan_create(void* function, const uint32_t grid[3], const uint32_t block[3],

@@ -1,5 +1,8 @@
 """The paged key/value cache at the edges of what its definition allows, on a B200 against plain float64 (the CPU's
 cases and references: :mod:`tests.test_paged_cache_edges`, :mod:`tests.pagedref`)."""
+import ctypes
+import threading
+
 import pytest
 import torch
 
@@ -133,3 +136,35 @@ def test_a_cache_operator_beside_another_kernel():
         graph.replay()
         check()
     ex.check()
+
+
+def test_a_thread_without_a_context_has_none_after_a_call():
+    cuda = ctypes.CDLL("libcuda.so.1")
+    t, problems = step_problems()
+    p = problems[0]
+    ex = Executable(compile_graph(Graph.from_dict(p.graph), p.meta()), device=0)
+    g = {k: v.cuda() for k, v in t.items()}
+    stream, seen = torch.cuda.Stream(), []
+    torch.cuda.synchronize()
+
+    def current():
+        ctx = ctypes.c_void_p()
+        assert cuda.cuCtxGetCurrent(ctypes.byref(ctx)) == 0
+        return ctx.value
+
+    def work():
+        seen.append(current())
+        ex.run(g, stream.cuda_stream)
+        seen.append(current())
+    th = threading.Thread(target=work)
+    th.start()
+    th.join()
+    stream.synchronize()
+    assert seen == [None, None]
+    want = R.write_ref(t, 16, False)
+    for n in want:
+        same(g[n].cpu(), want[n], n)
+    assert current() is not None
+    mine = current()
+    ex(g)
+    assert current() == mine
