@@ -382,3 +382,38 @@ def test_a_low_part_of_a_large_buffer_is_addressed():
     with pytest.raises(Unsupported, match="32-bit"):               # a row that only the data know
         big_buffer((1 << 10, huge >> 10), [i.V("k"), i.V("i")], at)()
     big_buffer((1 << 10, (1 << 31 >> 10) - 1), [i.V("k"), i.V("i")], at)()
+
+
+# ---- the byte rows' scale --------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_the_scale_is_the_product_with_the_rounded_inverse(dtype):
+    """s = max|x| * f32(1/127), which for some rows is not max|x| / 127 rounded to f32: there by one f32 step (both
+    round once, the constant is half a step off at most), which moves a stored value by half a step s / 2 at most
+    more than the rounding, as the byte may be the next one where x / s lies next to a half."""
+    dt = R.DT[dtype]
+    top = 1 + torch.arange(1 << (7 if dtype == "bf16" else 10)) / (1 << (7 if dtype == "bf16" else 10))
+    x = torch.randn(len(top), 64, generator=torch.Generator().manual_seed(2)).clamp(-0.99, 0.99)
+    x[:, 5] = top
+    x = x.to(dt)
+    by, s = R.quantise(x)
+    quotient = (x.double().abs().amax(-1) / 127).float()
+    other = s != quotient
+    assert 4 <= int(other.sum()) < len(s)
+    step = (s.view(torch.int32) - quotient.view(torch.int32)).abs()
+    assert int(step.max()) == 1
+    # bytes * s is within half a step of x: |q - x / s| <= 1/2, and the ratio's own rounding (half a step of f32 at 127)
+    err = ((by.double() - 128) * s.double()[:, None] - x.double()).abs() / s.double()[:, None]
+    assert float(err.max()) <= 0.5 + 127 * R.EPS
+    x = x[other][:8]
+    n = len(x)
+    t, pages = R.make("write", 1, 1, 64, 8, 2, [n], [n], chunk=n, dtype=dtype, quant=True)
+    t["K"][0, :, 0], t["V"][0, :, 0] = x, -x
+    p = irgen.cache_write_ir(1, n, 1, 64, pages, 8, 2, dtype, True)
+    want = R.write_ref(t, 8, True)
+    for opts in ({}, {"patterns": False}):
+        got, code, _ = PE.run(p, t, opts)
+        assert code == 0
+        for name in want:
+            same(got[name], want[name], name)
