@@ -744,7 +744,7 @@ def cache_write_ir(batch: int, chunk: int, kv_heads: int, dim: int, pages: int, 
 def cache_read_ir(batch: int, length: int, kv_heads: int, dim: int, pages: int, page: int, max_pages: int,
                   dtype: str = "bf16", quant: bool = False) -> Problem:
     """KR, VR [batch, length, kv_heads, dim]: the first min(lens[b], length) tokens of every sequence,
-    gathered from their pages in order; with ``quant`` (byte - 128) * scale, rounded once to ``dtype``.
+    gathered from their pages in order; with ``quant`` (byte - 128) * scale in f32, rounded to ``dtype``.
     Rows past a sequence's end, and rows whose page the table does not name, are left as they were."""
     _cache_dims("cache_read_ir", dtype, quant, batch=batch, length=length, kv_heads=kv_heads, dim=dim, pages=pages,
                 page=page, max_pages=max_pages)
@@ -781,15 +781,23 @@ def cache_read_ir(batch: int, length: int, kv_heads: int, dim: int, pages: int, 
 def paged_attention_ir(batch: int, chunk: int, heads: int, kv_heads: int, dim: int, pages: int, page: int,
                        max_pages: int, dtype: str = "bf16", quant: bool = False, window: int | None = None,
                        sinks: int = 0, scale: float | None = None) -> Problem:
-    """O = softmax(Q K^T * scale) V of a chunk of new tokens over the paged cache, causal, f32 math.
+    """O = softmax(Q K^T * scale) V of a chunk of new tokens over the paged cache, causal.
 
     Q, O [batch, chunk, heads, dim]; query head h reads key head h // (heads / kv_heads).  The new tokens'
     own keys and values are in the cache already (:func:`cache_write_ir` runs first).  A token at position p
     sees the keys 0..p, or with ``window`` those of p - window + 1..p and the first ``sinks`` ones.  One warp per
     query row and the online softmax of :func:`attention_ir` with its safe maximum; keys that are not
     seen are skipped, so whatever their rows hold cannot reach the result.  A row that sees no key (or
-    only keys whose score is -inf) ends as 0.  (Lowered to the tensor cores, an infinity in the values of a key that a
-    row does see may come out as NaN there, since P is multiplied in parts one of which can be 0.)"""
+    only keys whose score is -inf) ends as 0.
+
+    The nest computes in f32 throughout.  Lowered to the tensor cores (the default where sizes allow; the compile option
+    ``patterns: False`` keeps the nest), scores, softmax statistics and O stay in f32, and
+
+    * the weights are rounded: to f16 (2^-11) for f16 caches and bytes, to two bf16 parts (2^-14) for bf16 caches;
+    * over bytes, numbers of a bf16 query row below 2^-28 of its largest lose bits, key scales reach up to 2^96, and a
+      value whose scale is below 2^-20 of the largest one near it loses bits of its weight (below 2^-31: all);
+    * an infinity in the values of a key that a row does see may come out as NaN there, since P is multiplied in
+      parts one of which can be 0."""
     _cache_dims("paged_attention_ir", dtype, quant, batch=batch, chunk=chunk, heads=heads, kv_heads=kv_heads, dim=dim,
                 pages=pages, page=page, max_pages=max_pages)
     if heads % kv_heads:

@@ -1,7 +1,8 @@
 """A paged key/value cache written and read back: one pass of wide loads and stores over the tokens.
 
-Both kernels are bound by HBM bytes (and, for a decode step, by the chain lengths -> table -> row), so they do
-nothing but move rows 16 or 32 bytes a thread:
+They move rows 16 or 32 bytes a thread and compute no more than a row needs.  In 16 bits they are bound by HBM; a decode
+step by the chain lengths -> table -> row; the quantising write by its instructions (72 % of the issue slots of
+its active cycles), the read of bytes by the latency of lengths -> table -> row and scale -> store (52 warps an SM, 53 %):
 
 * **write** (:func:`..irgen.cache_write_ir`): dim / 8 lanes a row, 16 bytes of K and of V each.  For a cache of
   bytes the lanes find max|x| on the 16-bit patterns (their order without the sign is the numbers' order, and the
@@ -13,8 +14,9 @@ nothing but move rows 16 or 32 bytes a thread:
   (byte - 128) is exact in f32 (0x4B000000 | b is 2^23 + b), times the scale, rounded once more to the output.
 
 Measured on one B200: a decode step's write (64 tokens, 8 heads of 128, bf16) 2.0 us on the GPU in a run of calls; 16
-sequences of 100 to 4096 tokens of bytes read back (8 heads of 64, f16, 107 MB) 20-22 us, 4.8-5.2 TB/s; 8 prompts of 300
-to 2048 tokens quantised and read back 45-47 us for both calls.
+sequences of 100 to 4096 tokens of bytes read back (8 heads of 64, f16, 107 MB) 20-24 us, 4.4-5.2 TB/s, and from a bf16
+cache of 8 heads of 128 (280 MB) 43 us, 6.5 TB/s; 8 prompts of 300 to 2048 tokens written in bf16 20 us (101 MB),
+quantised and read back 38-41 us for both calls.
 
 Offsets into the pool are 64-bit.
 """

@@ -31,8 +31,8 @@ meets the other warps once, at the end.
   products of indicators (which rows see the key, which elements are +inf or NaN, -inf or NaN).
 
 Measured on one B200 (8 key heads of 128, 4 query heads each): 48 sequences of 17 to 8192 tokens, bf16, 830 MB: the
-kernel 133 us, 6.26 TB/s (0.97 of a copy), the call 139; the same in bytes 84 and 90 us, where issue slots are the
-busiest resource; one sequence of 333 tokens 6.9 us.
+kernel 133 us, 6.25 TB/s (0.97 of a copy), the call 136-141; the same in bytes 86 and 94-98 us, where issue slots are the
+busiest resource (51 % of the active cycles); one sequence of 333 tokens 6.9 us.
 
 The tcgen05 form holds a row a thread: four rows keep 4 of its 128 softmax threads busy, and each tile passes
 through TMA, MMA, TMEM and back.
@@ -75,7 +75,8 @@ def shape(dim, chunk, heads, kv_heads, quant, wide=False):
 def max_registers(rows, quant) -> int:
     """Registers a thread: 128 for at most 8 rows of a 16-bit cache, where 16 warps an SM with one 8 KiB block each
     keep HBM busy (a batch of 48 at 137 us; 139 with 168 registers); 168 where there is more arithmetic (the same
-    batch in bytes: 90 us with two blocks a warp, 94 at 128 registers)."""
+    batch in bytes: 90 us with two blocks a warp, 94 at 128 registers).  The cap of 128 spills 24 to 68 bytes a thread at
+    dim 128 in bf16, also in the forms that it was not measured for (a CTA a unit: few short sequences, windows)."""
     return 128 if rows <= 8 and not quant else 168
 
 
@@ -84,7 +85,10 @@ def block_keys(quant) -> int:
     return 32 if quant else 16
 
 
-MAX_SPREAD_BATCH = 128           # sequences whose lengths each CTA takes prefix sums of
+# Sequences whose lengths each CTA takes prefix sums of.  Above it a unit has one CTA, in the table's order.  Sequences of
+# 17 to 3000 tokens, 8 key heads of 128, bf16, against their bytes at a copy's rate: 128 of them 143 us over 125, 129 of
+# them 152 over 126, 256 of them 262 over 244; with one key head 256 units are too few to even out: 53 over 30.
+MAX_SPREAD_BATCH = 128
 MIN_TILES = 4                    # a run's least tiles: one for each of four warps
 
 

@@ -16,8 +16,8 @@ themselves, and for very short sequences, a CTA takes one unit, the longest unit
 before its own (4 x 512 tokens behind 333 to 4096 keys, bytes: 100 us, 129 in order of the table).
 
 **Roles.**  One thread issues the ``tcgen05.mma``: S(j+1) = Q K_(j+1)^T into one of two 64-column score buffers,
-then O += P(j) V_j.  Four softmax warps hold one row a thread; warps without a row take no part.  A warp loads by
-TMA, one box per page of the tile (at most 64 rows), with the page numbers fetched 32 at a time one batch ahead.
+then O += P(j) V_j.  Four softmax warps hold one row a thread; a warp without a row works on zeros like the others (the
+barriers count four).  A warp loads by TMA, one box per page of the tile (at most 64 rows), with the page numbers fetched 32 at a time one batch ahead.
 For 16-bit caches one more warp makes a V tile fit for the product (see what is masked): done by the softmax warps, that
 took 86 us in place of 61 for 4 x 1111 tokens with a window of 1024 (24 heads of 64 on 4, f16).  For a cache of bytes
 the boxes land in a raw ring, and two warps convert them into the tiles the products read: with 0x64 as its upper
@@ -150,7 +150,8 @@ def plan_ctas(batch, chunk, heads, kv_heads, page, max_pages, window, sinks, sms
     """CTAs to spread the tiles over, or 0 for one CTA a unit: for sequences of at most 8 tiles, and where the units
     fill the GPU by themselves.  There the parts and the second launch cost more than equal runs give (a 2048-token
     chunk over 8192 keys, 1024 units: 418 us, 420 with runs; 512 units of cached bytes 100 and 129; a windowed
-    chunk of 848 units 59 and 74)."""
+    chunk of 848 units 59 and 74).  Nor for more pairs than :data:`MAX_SPREAD_PAIRS`, which also go in the table's order:
+    not measured, right for any number."""
     pairs = batch * geometry(chunk, heads, kv_heads)[2]
     longest = _longest(chunk, heads, kv_heads, page, max_pages, window, sinks)
     if (longest <= 8 or pairs > MAX_SPREAD_PAIRS or pairs * kv_heads >= 2 * sms
