@@ -154,7 +154,11 @@ class Executable:
         device = f"cuda:{self.index}"
         if stream is None:
             return {name: torch.empty(n, dtype=dt, device=device) for name, (n, dt) in self._temp.items()}
-        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+        if stream == 2:
+            raise ValueError("2 is the per-thread default stream, another one in every thread: give a stream's own handle")
+        # 0 and 1 stand for the default stream; torch takes neither for an external one (0: a stream of its pool)
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if stream not in (0, 1)
+                               else torch.cuda.default_stream(device)):
             return {name: torch.empty(n, dtype=dt, device=device) for name, (n, dt) in self._temp.items()}
 
     def _run_plans(self, tensors: dict, stream) -> None:

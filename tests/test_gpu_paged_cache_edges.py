@@ -168,3 +168,48 @@ def test_a_thread_without_a_context_has_none_after_a_call():
     mine = current()
     ex(g)
     assert current() == mine
+
+
+def test_the_default_stream_by_its_handle(monkeypatch):
+    t, problems = step_problems()
+    p = problems[1]
+    ex = Executable(compile_graph(Graph.from_dict(p.graph), p.meta(), RUNS), device=0)
+    g = {k: v.cuda() for k, v in t.items()}
+    ref, bound, _ = R.attention_ref(t, 16)
+    seen, empty, side = [], torch.empty, torch.cuda.Stream()
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: (seen.append(torch.cuda.current_stream().cuda_stream), empty(*a, **kw))[1])
+    for current in (torch.cuda.default_stream(), side):
+        for handle, want in ((0, 0), (1, 0), (side.cuda_stream, side.cuda_stream)):
+            g["O"].fill_(7)
+            torch.cuda.synchronize()
+            seen.clear()
+            with torch.cuda.stream(current):
+                ex.run(g, handle)
+            torch.cuda.synchronize()
+            assert seen == [want]
+            R.check(g["O"], ref, bound, handle)
+    ex.check()
+
+
+def test_a_call_captured_by_its_handle_owns_its_scratch():
+    """What the graph's call allocated stays the graph's: memory taken and filled later is not what a replay writes."""
+    t, problems = step_problems()
+    p = problems[1]
+    ex = Executable(compile_graph(Graph.from_dict(p.graph), p.meta(), RUNS), device=0)
+    g = {k: v.cuda() for k, v in t.items()}
+    ref, bound, _ = R.attention_ref(t, 16)
+    s, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=s):
+        ex.run(g, s.cuda_stream)
+    with torch.cuda.stream(s):
+        n = sum(k for k, _ in ex._temp.values())
+        junk = [torch.full((n,), float("nan"), device="cuda") for _ in range(32)]
+    for _ in range(3):
+        g["O"].fill_(7)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        R.check(g["O"], ref, bound, "replay")
+    assert all(bool(x.isnan().all()) for x in junk)
+    ex.check()

@@ -1,5 +1,6 @@
 """The paged key/value cache at the edges of what its definition allows, on the CPU (emulated kernels, recording
 devices) against plain float64."""
+import contextlib
 import ctypes
 import json
 from types import SimpleNamespace
@@ -417,3 +418,40 @@ def test_the_scale_is_the_product_with_the_rounded_inverse(dtype):
         assert code == 0
         for name in want:
             same(got[name], want[name], name)
+
+
+# ---- streams by their handles ----------------------------------------------------------------
+
+
+class PlanExecutable(Executable):
+    """Allocates a call's scratch as the real one does."""
+
+    def _device_tensor(self, shape, dtype):
+        return torch.empty(shape, dtype=dtype)
+
+
+def test_a_call_allocates_on_the_stream_it_launches_on(recorder, monkeypatch):
+    # 0 and 1 are the handles of the default stream, which torch makes no external stream of (it gives another one, or
+    # refuses); 2 is another stream in every thread
+    t, problems = step_problems()
+    p = problems[1]
+    ex = PlanExecutable(compile_graph(Graph.from_dict(p.graph), p.meta(), RUNS), device=0)
+    on, empty = [], torch.empty
+
+    @contextlib.contextmanager
+    def stream(s):
+        on.append(s)
+        yield
+        on.append(None)
+    monkeypatch.setattr(torch.cuda, "stream", stream)
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda h, device=None: ("external", h, str(device)))
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: ("default", str(device)))
+    monkeypatch.setattr(torch, "empty", lambda *a, device=None, **kw: empty(*a, **kw))
+    for handle, want in ((55, ("external", 55, "cuda:0")), (0, ("default", "cuda:0")), (1, ("default", "cuda:0"))):
+        on.clear()
+        ex.run(t, handle)
+        assert on == [want, None] and recorder.log[-1][-1] == handle
+    recorder.log.clear()
+    with pytest.raises(ValueError, match="per-thread"):
+        ex.run(t, 2)
+    assert recorder.log == []
