@@ -204,8 +204,9 @@ class Executable:
         from .launcher import ATTR_NUM_REGS
         return self.dev.func_attribute(self.funcs[i], ATTR_NUM_REGS)
 
-    def _tmap(self, entry: str, spec: dict, t) -> ctypes.Array:
-        key = (entry, spec["name"], t.data_ptr(), tuple(t.shape))
+    def _tmap(self, spec: dict, t) -> ctypes.Array:
+        # by the record's own entry, which the blob keeps: several kernels of a module may name their maps alike
+        key = (id(spec), t.data_ptr(), tuple(t.shape))
         hit = self._tmap_cache.get(key)
         if hit is not None:
             return hit
@@ -215,6 +216,7 @@ class Executable:
         self.dev.tmap_encode_tiled(ctypes.c_void_p(blob.addr), _TMAP_DTYPE[spec["dtype"]], t.data_ptr(), dims, strides,
                                    spec["box"], swizzle=_SWIZZLE[spec.get("swizzle", "128B")],
                                    l2promo=spec.get("l2promo", 2))
+        blob.spec = spec
         self._tmap_cache[key] = blob
         return blob
 
@@ -256,7 +258,7 @@ class Executable:
                 keep.append(v)
                 args.append(ctypes.cast(ctypes.byref(v), ctypes.c_void_p).value)
             for spec in rec.get("tmaps", []):
-                blob = self._tmap(rec["entry"], spec, tensors[spec["tensor"]])
+                blob = self._tmap(spec, tensors[spec["tensor"]])
                 keep.append(blob)
                 args.append(blob.addr)
             for spec in rec.get("extra", []):
