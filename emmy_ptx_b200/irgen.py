@@ -795,7 +795,8 @@ def paged_attention_ir(batch: int, chunk: int, heads: int, kv_heads: int, dim: i
 
     * the weights are rounded: to f16 (2^-11) for f16 caches and bytes, to two bf16 parts (2^-14) for bf16 caches;
     * over bytes, numbers of a bf16 query row below 2^-28 of its largest lose bits, key scales reach up to 2^96, and a
-      value whose scale is below 2^-20 of the largest one near it loses bits of its weight (below 2^-31: all);
+      value whose scale is below 2^-20 of the largest one in its unit (the rows and keys of one CTA) loses bits of its weight: by
+      2^-31 of the largest value there a key, at most;
     * an infinity in the values of a key that a row does see may come out as NaN there, since P is multiplied in
       parts one of which can be 0."""
     _cache_dims("paged_attention_ir", dtype, quant, batch=batch, chunk=chunk, heads=heads, kv_heads=kv_heads, dim=dim,

@@ -23,7 +23,7 @@ SIGNS = {"negative": lambda n: -torch.ones(n), "alternating": lambda n: 1.0 - 2.
 SIGNED = [
     # batch, chunk, heads, kv_heads, dim, page, max_pages, lens, fresh, options
     (1, 1, 4, 1, 64, 16, 8, [100], [1], {}),
-    (2, 3, 4, 2, 128, 16, 13, [200, 40], [3, 2], {"paged_ctas": 5, "paged_min_tiles": 1}),
+    (2, 3, 2, 1, 128, 16, 9, [130, 20], [3, 2], {"paged_ctas": 3, "paged_min_tiles": 1}),
 ]
 
 
