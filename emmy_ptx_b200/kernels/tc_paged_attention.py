@@ -15,15 +15,15 @@ more than one run leaves parts in f32 (O, the row's reference m and its sum l) a
 themselves, and for very short sequences, a CTA takes one unit, the longest units first: every CTA counts how many come
 before its own (4 x 512 tokens behind 333 to 4096 keys, bytes: 100 us, 129 in order of the table).
 
-**Roles.**  One thread issues the ``tcgen05.mma``: S(j+1) = Q K_(j+1)^T into one of two 64-column score buffers,
-then O += P(j) V_j.  Four softmax warps hold one row a thread; a warp without a row works on zeros like the others (the
-barriers count four).  A warp loads by TMA, one box per page of the tile (at most 64 rows), with the page numbers fetched 32 at a time one batch ahead.
-For 16-bit caches one more warp makes a V tile fit for the product (see what is masked): done by the softmax warps, that
-took 86 us in place of 61 for 4 x 1111 tokens with a window of 1024 (24 heads of 64 on 4, f16).  For a cache of bytes
-the boxes land in a raw ring, and two warps convert them into the tiles the products read: with 0x64 as its upper
-half a byte b is the f16 number 1024 + b, less 1152 it is b - 128, exactly.  Each quarter warp takes 64 bytes of rows
-r and r ^ 5, which the raw ring's swizzle and the tile's put into different banks.  The keys' scales multiply the
-scores' columns, the values' scales multiply P.
+**Roles.**  One thread issues the ``tcgen05.mma``: S(j+1) = Q K_(j+1)^T into one of two 64-column score buffers, then
+O += P(j) V_j.  Four softmax warps hold one row a thread; a warp without a row works on zeros like the others (the
+barriers count four).  A warp loads by TMA, one box per page of the tile (at most 64 rows), with the page numbers
+fetched 32 at a time one batch ahead.  For 16-bit caches one more warp makes a V tile fit for the product (see what is
+masked): done by the softmax warps, that took 86 us in place of 61 for 4 x 1111 tokens with a window of 1024 (24 heads
+of 64 on 4, f16).  For a cache of bytes the boxes land in a raw ring, and two warps convert them into the tiles the
+products read: with 0x64 as its upper half a byte b is the f16 number 1024 + b, less 1152 it is b - 128, exactly.
+Each quarter warp takes 64 bytes of rows r and r ^ 5, which the raw ring's swizzle and the tile's put into different
+banks.  The keys' scales multiply the scores' columns, the values' scales multiply P.
 
 **Numerics.**  The score buffers, the running reference and sum, and O are f32.  P is rounded for the tensor core:
 f16 caches take f16 P, to nearest (2^-11), with 2^7 put on the exponent so that small weights keep their bits;
