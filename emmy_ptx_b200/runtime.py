@@ -295,6 +295,8 @@ class Executable:
         import torch
         if self.plans is not None:
             return self._run_plans(tensors, stream)
+        if self.module is None:
+            raise ValueError(f"kernel {self.records[0]['entry']!r} was closed")
         if self._args:
             self._check(tensors)
         if self._temp:

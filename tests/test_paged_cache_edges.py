@@ -285,6 +285,16 @@ def test_a_cache_operator_beside_another_kernel(recorder, first):
         assert recorder.log == []
 
 
+def test_a_closed_executable_of_several_kernels_refuses(recorder):
+    t, problems = step_problems()
+    q = other_first()
+    ex = host_executable([q, problems[1]], RUNS)
+    ex.close()
+    with pytest.raises(ValueError, match="closed"):
+        ex.run({**t, **data.make_inputs(q)}, 55)
+    assert recorder.log == []
+
+
 def test_two_attentions_of_one_graph_have_their_own_tensor_maps(recorder):
     # both name their map of the pool alike; their boxes differ
     B, H, hk, d, page, mp = 1, 2, 1, 64, 64, 3
