@@ -22,8 +22,8 @@ SIGNS = {"negative": lambda n: -torch.ones(n), "alternating": lambda n: 1.0 - 2.
          "large-negative": lambda n: torch.where(torch.arange(n) % 7 == 3, -1024.0, 1.0)}
 SIGNED = [
     # batch, chunk, heads, kv_heads, dim, page, max_pages, lens, fresh, options
-    (1, 1, 4, 1, 64, 16, 8, [100], [1], {}),
-    (2, 3, 2, 1, 128, 16, 9, [130, 20], [3, 2], {"paged_ctas": 3, "paged_min_tiles": 1}),
+    (1, 1, 4, 1, 128, 16, 5, [70], [1], {}),
+    (2, 3, 2, 1, 64, 16, 9, [130, 20], [3, 2], {"paged_ctas": 3, "paged_min_tiles": 1}),
 ]
 
 
@@ -40,8 +40,7 @@ def signed_case(case, dtype, signs):
 
 @pytest.mark.parametrize("rows", [0, 64])
 @pytest.mark.parametrize("signs", SIGNS)
-@pytest.mark.parametrize("dtype", ["bf16", "f16"])
-@pytest.mark.parametrize("case", SIGNED, ids=["decode", "draft-runs"])
+@pytest.mark.parametrize("case,dtype", [(SIGNED[0], "f16"), (SIGNED[1], "bf16")], ids=["decode-f16", "draft-runs-bf16"])
 def test_scales_of_any_sign(case, dtype, signs, rows):
     t, p = signed_case(case, dtype, signs)
     got, code, _ = PE.run(p, t, {**case[-1], "paged_rows": rows})
